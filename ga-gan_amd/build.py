@@ -19,10 +19,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 OUT = os.path.join(HERE, 'libsgops.so')
 OBJ_DIR = os.path.join(HERE, 'build')
+# Without packed float32 arithmetic: the compiler forms v_pk_{add,mul,fma}_f32 from ordinary scalar code, and some of their operand
+# forms have given wrong results on MI355X now and then.  (The host pass warns that it does not know the feature.)
 CFLAGS = ['-O3', '-std=c++17', '--offload-arch=gfx950', '-fPIC', '-Wall', '-Wno-unused-function',
-          '-Wno-unused-const-variable']
-# per-source additions.  The epilogues of the band and one-pass up-sampling kernels run beside matrix instructions, where packed float32 vector
-# instructions (what the SLP vectoriser makes of adjacent scalar multiplies) cost more than the two scalar ones.
+          '-Wno-unused-const-variable', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+# per-source additions: in the band and one-pass up-sampling kernels the vectoriser's pairs of adjacent scalars only cost moves.
 EXTRA_CFLAGS = {'sg_band3x3': ['-fno-slp-vectorize'], 'sg_convup_fir': ['-fno-slp-vectorize']}
 
 

@@ -6,8 +6,8 @@
 //     16-byte packet per plane plus 8 bytes on either side for the filter's reach) is scattered into the four output
 //     rows it contributes to: acc[row][column] += f[i][t] * in[column + t].  The four partial rows live in
 //     registers and rotate; the row that has received its fourth contribution is finished and stored.
-//   * The two planes sit in the halves of 64-bit register pairs, so all multiply-adds are packed (v_pk_fma_f32 with
-//     the tap broadcast): 8 vector instructions per output for a full 4 x 4 filter, separable or not.
+//   * The two planes sit in the halves of 64-bit register pairs, and a multiply-add on a pair is two scalar
+//     ones with the tap broadcast: 16 vector instructions per output for a full 4 x 4 filter, separable or not.
 //   * A wave's 64 lanes cover 512 consecutive columns (narrower planes: whole rows of several bands): every load and
 //     store instruction moves contiguous runs of up to a kilobyte per plane.  The loads of the row after next are requested before a row's arithmetic.
 //   * The optional layer epilogue (demodulation, noise, bias, leaky ReLU, gain, clamp) runs on the finished row.
@@ -364,7 +364,7 @@ int launch_down2_pad(const sg_upfirdn2d_params& p, hipStream_t stream) {
 // tensors).  Only every other row and column of the zero-stuffed plane is non-zero, so an output reads 2 x 2 taps: a
 // lane's 16 output columns read one packet per plane plus one element on either side (loaded as 8 bytes), and input
 // row r completes the output rows e = 2r - 3, 2r - 2 (its filter rows 3 and 2 on top of what row r - 1 left) and
-// starts the rows 2r - 1, 2r (filter rows 1 and 0), with e = output row - pad_y0.  No rotation, 2 packed
+// starts the rows 2r - 1, 2r (filter rows 1 and 0), with e = output row - pad_y0.  No rotation, 4
 // multiply-adds per output.
 struct AddendRows { uint4 v[2][2][2]; };     // [output row of the pair an input row completes][plane][half of the lane's 16 columns]
 

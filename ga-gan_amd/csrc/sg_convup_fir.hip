@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) conv_up2_fir_kernel(UpFirArgs g) 
                     nz[0] = lo4.x; nz[1] = lo4.y; nz[2] = lo4.z; nz[3] = lo4.w;
                     nz[4] = hi4.x; nz[5] = hi4.y; nz[6] = hi4.z; nz[7] = hi4.w;
                 }
-                // pairs of adjacent columns (adjacent registers of an accumulator) go through packed multiply-adds; the
+                // pairs of adjacent columns (adjacent registers of an accumulator) go through multiply-adds two at a time; the
                 // filter taps carry the demodulation coefficient and the gain (t0..t3)
                 f32x2_t z[2][2];    // [px][pair]
 #pragma unroll
