@@ -19,7 +19,10 @@ SYMBOLS = ('sg_version', 'sg_last_error', 'sg_init', 'sg_upfirdn2d_out_size', 's
            'sg_conv2d_workspace_bytes', 'sg_conv2d_wgrad_workspace_bytes', 'sg_conv_up2_fir', 'sg_conv_up2_fir_supported',
            'sg_upfirdn2d_add', 'sg_upfirdn2d_add_supported', 'sg_upfirdn2d_kernel', 'sg_planes_segments', 'sg_scale_planes', 'sg_dot_planes',
            'sg_styles', 'sg_styles_backward', 'sg_pack_weights',
-           'sg_conv2d_prepared_weight_bytes', 'sg_conv2d_prepare_weights', 'sg_conv2d_supports_addend')
+           'sg_conv2d_prepared_weight_bytes', 'sg_conv2d_prepare_weights', 'sg_conv2d_supports_addend',
+           'sg_linear', 'sg_linear_workspace_bytes', 'sg_linear_backward', 'sg_linear_backward_workspace_bytes',
+           'sg_embedding', 'sg_embedding_backward', 'sg_embedding_backward_workspace_bytes',
+           'sg_adam_step_list', 'sg_grad_norm', 'sg_grad_norm_workspace_bytes', 'sg_scale_grads')
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float64: 3}
 
@@ -104,6 +107,16 @@ def lib():
         for name in ('sg_conv2d_workspace_bytes', 'sg_conv2d_wgrad_workspace_bytes', 'sg_conv2d_prepared_weight_bytes'):
             getattr(handle, name).argtypes = [vp]
             getattr(handle, name).restype = ctypes.c_size_t
+        size_t = ctypes.c_size_t
+        for name, args in (('sg_linear', [vp] * 5 + [size_t, vp]), ('sg_linear_backward', [vp] * 9 + [size_t, vp]),
+                           ('sg_embedding', [vp] * 3), ('sg_embedding_backward', [vp] * 4 + [size_t, vp]), ('sg_adam_step_list', [vp, vp]),
+                           ('sg_grad_norm', [vp, f32, f32, f32, vp, vp, size_t, vp]), ('sg_scale_grads', [vp] * 3)):
+            getattr(handle, name).argtypes = args
+            getattr(handle, name).restype = ctypes.c_int
+        for name in ('sg_linear_workspace_bytes', 'sg_linear_backward_workspace_bytes', 'sg_embedding_backward_workspace_bytes',
+                     'sg_grad_norm_workspace_bytes'):
+            getattr(handle, name).argtypes = [vp]
+            getattr(handle, name).restype = size_t
         handle.sg_conv2d_reduce_rows.argtypes = [vp]
         handle.sg_conv2d_reduce_rows.restype = ctypes.c_int
         handle.sg_conv2d_kernel.argtypes = [vp]

@@ -1,0 +1,780 @@
+// Fully connected layer with its epilogue, and its gradients:
+//   z = x w^T * w_gain + b * b_gain        y = act(z) * gain + residual           x [m, k], w [n, k], y [m, n]
+//   s = dy * act'(z)      dx = s w * (gain w_gain)    dw = s^T x * (gain w_gain)    db = sum over rows of s * (gain b_gain)
+// Three matrix products that differ in which index of each operand is contiguous; one kernel template covers them:
+//   C[i, j] = sum over p of A(i, p) B(j, p),   each operand stored with p contiguous ("rows") or with i / j contiguous ("columns").
+// An operand is never transposed in memory.  Tiles of 128 bytes along p travel to LDS as they lie (16 bytes per lane, straight
+// into LDS where rows are 16-byte aligned), and a fragment of a "columns" operand is read by the transposing LDS read (16-bit)
+// or four rows at a time (float32).  16-bit operands multiply on v_mfma_f32_16x16x32, float32 ones on v_mfma_f32_16x16x4_f32,
+// whose products and sums are plain float32.  All sums are float32; every output is rounded once.
+//
+// The gradient of the activation is s above without the gains: for the piecewise linear activations with slope 1 on one side
+// its 16-bit rounding is exact there, so that folding sqrt(2) into the products' scale keeps it that way.
+#include "sg_common.h"
+#include "sg_column_sums.h"
+
+namespace sg {
+namespace {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+
+constexpr int kStepBytes = 128;                    // of p per LDS tile: 64 16-bit or 32 float32 elements
+constexpr unsigned kOutside = 0x80000000u;         // a buffer offset beyond every descriptor: the load yields zeros
+
+enum { kActLinear = 1, kActRelu, kActLrelu, kActTanh, kActSigmoid, kActElu, kActSelu, kActSoftplus, kActSwish };
+constexpr float kSeluScale = 1.0507009873554804934193349852946f, kSeluAlpha = 1.6732632423543772848170429916717f;
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+
+__device__ __forceinline__ float activate(int act, float alpha, float z) {
+    switch (act) {
+        case kActRelu: return z > 0.f ? z : (z != z ? z : 0.f);
+        case kActLrelu: return z > 0.f ? z : z * alpha;
+        case kActTanh: return tanhf(z);
+        case kActSigmoid: return sigmoid(z);
+        case kActElu: return z > 0.f ? z : expm1f(z);
+        case kActSelu: return kSeluScale * (z > 0.f ? z : kSeluAlpha * expm1f(z));
+        case kActSoftplus: return fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
+        case kActSwish: return z * sigmoid(z);
+        default: return z;
+    }
+}
+
+// act'(z) of the activations that are not piecewise linear with corner at zero alone
+__device__ __forceinline__ float slope_at(int act, float z) {
+    switch (act) {
+        case kActTanh: { const float t = tanhf(z); return 1.f - t * t; }
+        case kActSigmoid: { const float t = sigmoid(z); return t * (1.f - t); }
+        case kActElu: return z > 0.f ? 1.f : expf(z);
+        case kActSelu: return kSeluScale * (z > 0.f ? 1.f : kSeluAlpha * expf(z));
+        case kActSoftplus: return sigmoid(z);
+        case kActSwish: { const float t = sigmoid(z); return t * (1.f + z * (1.f - t)); }
+        default: return 1.f;
+    }
+}
+
+// ---- the matrix product -----------------------------------------------------------------------------------------------------
+
+struct Gemm {
+    const void* a;                       // operand of the rows i
+    const void* b;                       // operand of the columns j
+    int64_t lda, ldb;                    // elements between rows as stored
+    int64_t ni, nj, np;
+    int tiles_i, tiles_j, slices, slice_steps;
+    float* partial;                      // [slices][ni][nj] when slices > 1
+    void* out;                           // [ni][nj]
+    float scale;
+    // epilogue of the forward pass (with_epilogue)
+    int with_epilogue;
+    const void* bias;                    // [nj]
+    const void* residual;                // [ni][ldr]
+    int64_t ldr;
+    float* z;                            // [ni][nj] or NULL: pre-activation values for the backward pass
+    uint8_t* positive;                   // [ni][nj] or NULL: z > 0
+    int act;
+    float alpha, gain, b_gain;
+};
+
+template <class T> struct Io;            // vectors of 1, 2 or 4 consecutive elements as float
+template <class T, int N> struct alignas(N * sizeof(T)) Run { T v[N]; };
+
+// N consecutive results (i, j .. j + N - 1), all inside.
+template <class T, int N>
+__device__ __forceinline__ void finish(const Gemm& g, int64_t i, int64_t j, float (&v)[N]) {
+    const int64_t at = i * g.nj + j;
+    Run<T, N> out;
+    if (!g.with_epilogue) {
+#pragma unroll
+        for (int e = 0; e < N; e++) out.v[e] = Elem<T>::store(v[e] * g.scale);
+        *reinterpret_cast<Run<T, N>*>((T*)g.out + at) = out;
+        return;
+    }
+    Run<T, N> bias, res;
+    if (g.bias) bias = *reinterpret_cast<const Run<T, N>*>((const T*)g.bias + j);
+    if (g.residual) res = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + i * g.ldr + j);
+    Run<float, N> zs;
+    Run<uint8_t, N> pos;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        float z = v[e] * g.scale;
+        if (g.bias) z += Elem<T>::load(bias.v[e]) * g.b_gain;
+        zs.v[e] = z;
+        pos.v[e] = z > 0.f;
+        float y = activate(g.act, g.alpha, z) * g.gain;
+        if (g.residual) y += Elem<T>::load(res.v[e]);
+        out.v[e] = Elem<T>::store(y);
+    }
+    *reinterpret_cast<Run<T, N>*>((T*)g.out + at) = out;
+    if (g.z) *reinterpret_cast<Run<float, N>*>(g.z + at) = zs;
+    if (g.positive) *reinterpret_cast<Run<uint8_t, N>*>(g.positive + at) = pos;
+}
+
+// Whether runs of N elements at multiples of N may be moved as one access: everything finish() touches keeps them aligned.
+template <class T> bool runs_aligned(const Gemm& g, int n) {
+    auto ok = [&](const void* p, size_t bytes) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+    return g.nj % n == 0 && ok(g.out, n * sizeof(T)) && ok(g.bias, n * sizeof(T)) && ok(g.residual, n * sizeof(T)) &&
+           (g.residual == nullptr || g.ldr % n == 0) && ok(g.z, n * 4) && ok(g.positive, n) && ok(g.partial, 16);
+}
+
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)kOutside, 0x00020000);
+}
+
+// One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: SIDE * 8 slots of 16 bytes.
+//   ROWS:  slot (row, c) holds the 16 bytes c ^ ((row >> 1) & 7) of the row: 16 lanes reading one column of 16 rows hit 16
+//          different 16-byte banks.
+//   !ROWS: the tile is [p][side]; 16-bit: the 32-byte block c of line p holds block c ^ swizzle(p), so that the transposing
+//          read of 16 lines hits each 32-byte bank twice, once per half wave; float32: as it lies.
+template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
+    static constexpr int ES = sizeof(T), E = 16 / ES, BK = kStepBytes / ES;
+    static constexpr int BYTES = SIDE * kStepBytes;
+    static constexpr int LOADS = SIDE * 8 / THREADS;               // 16-byte slots per thread
+    static constexpr int LINE = SIDE / E;                          // !ROWS: slots per line
+    static_assert(LOADS >= 1 && LOADS * THREADS == SIDE * 8, "slots divide among the threads");
+
+    static __device__ __forceinline__ int swizzle(int p) {
+        if (ES == 4) return 0;
+        return SIDE >= 128 ? (p & 3) | ((p >> 3) & 1) << 2 : ((p >> 1) & 1) | ((p >> 3) & 1) << 1;
+    }
+    // slot -> (side, p) of its first element within the tile
+    static __device__ __forceinline__ void where(int slot, int& side, int& p) {
+        if (ROWS) {
+            side = slot >> 3;
+            p = ((slot & 7) ^ ((side >> 1) & 7)) * E;
+        } else {
+            p = slot / LINE;
+            side = ((slot % LINE) ^ (swizzle(p) << 1)) * E;
+        }
+    }
+    // straight to LDS.  base: the tile's first element (of this step); left_*: valid extent from there
+    static __device__ __forceinline__ void load_direct(unsigned char* lds, const T* base, int64_t ld, int64_t left_side, int64_t left_p) {
+        const rsrc_t r = make_rsrc(base);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) {
+            int side, p;
+            where(k * THREADS + threadIdx.x, side, p);
+            const unsigned off = (unsigned)((ROWS ? side : p) * (unsigned)ld + (ROWS ? p : side)) * ES;
+            const bool ok = side < left_side && p < left_p;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (k * THREADS + wave * 64) * 16), 16,
+                                                     ok ? off : kOutside, 0, 0, 0);
+        }
+    }
+    // by way of registers: any alignment, any extent
+    struct Regs { uint4 v[LOADS]; };
+    static __device__ __forceinline__ void fetch(Regs& r, const T* base, int64_t ld, int64_t left_side, int64_t left_p) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[E]; };
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) {
+            int side, p;
+            where(k * THREADS + threadIdx.x, side, p);
+            const T* src = base + (ROWS ? side * ld + p : p * ld + side);
+            const bool line = ROWS ? side < left_side : p < left_p;
+            const int64_t in_line = (ROWS ? left_p - p : left_side - side);
+            Pack<T> q;
+            if (line && in_line >= E) {
+                const Loose l = *reinterpret_cast<const Loose*>(src);
+#pragma unroll
+                for (int e = 0; e < E; e++) q.v[e] = l.v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) q.v[e] = line && e < in_line ? src[e] : Elem<T>::store(0.f);
+            }
+            __builtin_memcpy(&r.v[k], &q, 16);
+        }
+    }
+    static __device__ __forceinline__ void commit(unsigned char* lds, const Regs& r) {
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) *reinterpret_cast<uint4*>(lds + (k * THREADS + threadIdx.x) * 16) = r.v[k];
+    }
+};
+
+// Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for K-part kk (two per step: 32 16-bit or 16 float32 elements).
+template <class T, int SIDE, bool ROWS, int COUNT> struct Frags {
+    static constexpr int V = sizeof(T) == 4 && !ROWS ? (COUNT >= 4 ? 4 : COUNT) : 1;   // tiles whose rows interleave
+    uint4 q[COUNT];                                                                   // 8 16-bit values, or 4 float32 (ROWS)
+    float f[sizeof(T) == 4 && !ROWS ? COUNT : 1][4];
+
+    // row within the wave's share of element `r16` (0 .. 15) of tile t
+    static __device__ __forceinline__ int row(int t, int r16) { return (t / V) * 16 * V + r16 * V + t % V; }
+
+    __device__ __forceinline__ void read(const unsigned char* lds, int first, int kk) {
+        const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+        if constexpr (ROWS) {
+            const int at = (first + l16) * kStepBytes + (((kk * 4 + g) ^ ((l16 >> 1) & 7)) << 4);
+#pragma unroll
+            for (int t = 0; t < COUNT; t++) q[t] = *reinterpret_cast<const uint4*>(lds + at + t * 16 * kStepBytes);
+        } else if constexpr (sizeof(T) == 2) {
+            constexpr int LINE = SIDE * 2;
+            const int p = kk * 32 + g * 8 + (l16 >> 2);
+            const int sw = Tile<T, SIDE, false, 64>::swizzle(p);             // (the same for p + 4)
+            const unsigned char* line = lds + p * LINE + (l16 & 3) * 8;
+#pragma unroll
+            for (int t = 0; t < COUNT; t++) {
+                const unsigned char* at = line + (((first >> 4) + t) ^ sw) * 32;
+                typedef __attribute__((address_space(3))) s16x4_t* Lds;
+                const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at);
+                const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 4 * LINE));
+                const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+                q[t] = make_uint4(a.x, a.y, b.x, b.y);
+            }
+        } else {
+            constexpr int LINE = SIDE * 4;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int t = 0; t < COUNT; t += V) {
+                    const unsigned char* at = lds + (kk * 16 + g * 4 + e) * LINE + (first + t * 16 + l16 * V) * 4;
+                    if constexpr (V == 4) {
+                        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(at);
+                        f[t][e] = v.x; f[t + 1][e] = v.y; f[t + 2][e] = v.z; f[t + 3][e] = v.w;
+                    } else if constexpr (V == 2) {
+                        const f32x2_t v = *reinterpret_cast<const f32x2_t*>(at);
+                        f[t][e] = v.x; f[t + 1][e] = v.y;
+                    } else {
+                        f[t][e] = *reinterpret_cast<const float*>(at);
+                    }
+                }
+        }
+    }
+    __device__ __forceinline__ float value(int t, int e) const {
+        if constexpr (ROWS) return __builtin_bit_cast(f32x4_t, q[t])[e];
+        else return f[t][e];
+    }
+};
+
+__device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t c, __hip_bfloat16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t c, __half) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Tile BI x BJ per workgroup of WI x WJ waves.  DIRECT: rows of both operands are whole aligned 16-byte packets.  RUN: elements
+// per store where the layout of the accumulators allows four in a row (1 otherwise).
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, bool DIRECT, int RUN>
+__global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
+    constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
+    using TileA = Tile<T, BI, ROWS_A, THREADS>;
+    using TileB = Tile<T, BJ, ROWS_B, THREADS>;
+    using FragA = Frags<T, BI, ROWS_A, TI>;
+    using FragB = Frags<T, BJ, ROWS_B, TJ>;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * (TileA::BYTES + TileB::BYTES)];
+    constexpr int BUF = TileA::BYTES + TileB::BYTES;
+
+    // Workgroups go round robin over the 8 XCDs: each XCD gets a contiguous share of the tiles, in groups of 8 tile rows so that
+    // the tiles it works on at one time share rows of A and columns of B in its L2.
+    const unsigned tiles = (unsigned)g.tiles_i * g.tiles_j, total = tiles * g.slices;
+    unsigned id = blockIdx.x;
+    {
+        const unsigned per = total / 8, extra = total % 8, xcd = id % 8, k = id / 8;
+        id = xcd * per + (xcd < extra ? xcd : extra) + k;
+    }
+    const unsigned slice = id / tiles, tile = id % tiles;
+    const unsigned group = 8u * g.tiles_j, g0 = tile / group * 8u;
+    const unsigned rows = min((unsigned)g.tiles_i - g0, 8u);
+    const int64_t i0 = (int64_t)(g0 + tile % group % rows) * BI, j0 = (int64_t)(tile % group / rows) * BJ;
+
+    const T* a = (const T*)g.a + (ROWS_A ? i0 * g.lda : i0);
+    const T* b = (const T*)g.b + (ROWS_B ? j0 * g.ldb : j0);
+    const int64_t left_i = g.ni - i0, left_j = g.nj - j0;
+    const int steps_all = (int)((g.np + BK - 1) / BK);
+    const int first = (int)slice * g.slice_steps;
+    const int steps = min(g.slice_steps, steps_all - first);
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    f32x4_t acc[TJ][TI];
+#pragma unroll
+    for (int t = 0; t < TJ; t++)
+#pragma unroll
+        for (int s = 0; s < TI; s++) acc[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    auto at_a = [&](int step) { return a + (ROWS_A ? (int64_t)step * BK : (int64_t)step * BK * g.lda); };
+    auto at_b = [&](int step) { return b + (ROWS_B ? (int64_t)step * BK : (int64_t)step * BK * g.ldb); };
+    auto multiply = [&](const unsigned char* lds) {
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            FragA fa;
+            FragB fb;
+            fa.read(lds, wi, kk);
+            fb.read(lds + TileA::BYTES, wj, kk);
+#pragma unroll
+            for (int t = 0; t < TJ; t++)
+#pragma unroll
+                for (int s = 0; s < TI; s++) {
+                    if constexpr (sizeof(T) == 2) {
+                        acc[t][s] = mfma(fb.q[t], fa.q[s], acc[t][s], T());
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb.value(t, e), fa.value(s, e), acc[t][s], 0, 0, 0);
+                    }
+                }
+        }
+    };
+    // Two LDS buffers: the loads of step n + 1 are under way while step n multiplies; one barrier a step (after it every wave has
+    // read the buffer that is filled next, and every wave's loads into the one that is read next have landed).
+    if constexpr (DIRECT) {
+        auto issue = [&](int n, int buf) {
+            const int step = first + n;
+            TileA::load_direct(smem + buf * BUF, at_a(step), g.lda, left_i, g.np - (int64_t)step * BK);
+            TileB::load_direct(smem + buf * BUF + TileA::BYTES, at_b(step), g.ldb, left_j, g.np - (int64_t)step * BK);
+        };
+        if (steps > 0) issue(0, 0);
+        for (int n = 0; n < steps; n++) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (n + 1 < steps) issue(n + 1, (n + 1) & 1);
+            multiply(smem + (n & 1) * BUF);
+        }
+    } else {
+        typename TileA::Regs ra;
+        typename TileB::Regs rb;
+        auto fetch = [&](int n) {
+            const int step = first + n;
+            TileA::fetch(ra, at_a(step), g.lda, left_i, g.np - (int64_t)step * BK);
+            TileB::fetch(rb, at_b(step), g.ldb, left_j, g.np - (int64_t)step * BK);
+        };
+        auto commit = [&](int buf) {
+            TileA::commit(smem + buf * BUF, ra);
+            TileB::commit(smem + buf * BUF + TileA::BYTES, rb);
+        };
+        if (steps > 0) {
+            fetch(0);
+            commit(0);
+        }
+        for (int n = 0; n < steps; n++) {
+            __syncthreads();
+            if (n + 1 < steps) fetch(n + 1);
+            multiply(smem + (n & 1) * BUF);
+            if (n + 1 < steps) commit((n + 1) & 1);
+        }
+    }
+
+    // acc[t][s][r]: row i = tile s of A at lane % 16, column j = tile t of B at 4 * (lane / 16) + r
+    const int l16 = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
+    auto put = [&](int64_t i, int64_t j, auto& v) {
+        constexpr int N = sizeof(v) / 4;
+        if (g.slices > 1) {
+            float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
+            Run<float, N> w;
+#pragma unroll
+            for (int e = 0; e < N; e++) w.v[e] = v[e];
+            *reinterpret_cast<Run<float, N>*>(out) = w;
+        } else {
+            finish<T, N>(g, i, j, v);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < TI; s++) {
+        const int64_t i = i0 + wi + FragA::row(s, l16);
+        if (i >= g.ni) continue;
+        if constexpr (FragB::V == 1) {                    // the four values of a lane are consecutive columns
+#pragma unroll
+            for (int t = 0; t < TJ; t++) {
+                const int64_t j = j0 + wj + t * 16 + quad * 4;
+                if constexpr (RUN == 4) {
+                    float v[4] = {acc[t][s][0], acc[t][s][1], acc[t][s][2], acc[t][s][3]};
+                    if (j < g.nj) put(i, j, v);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float v[1] = {acc[t][s][r]};
+                        if (j + r < g.nj) put(i, j + r, v);
+                    }
+                }
+            }
+        } else {                                          // V tiles hold consecutive columns
+#pragma unroll
+            for (int t = 0; t < TJ; t += FragB::V)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int64_t j = j0 + wj + FragB::row(t, quad * 4 + r);
+                    if constexpr (RUN == 4) {
+                        float v[FragB::V];
+#pragma unroll
+                        for (int e = 0; e < FragB::V; e++) v[e] = acc[t + e][s][r];
+                        if (j < g.nj) put(i, j, v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < FragB::V; e++) {
+                            float v[1] = {acc[t + e][s][r]};
+                            if (j + e < g.nj) put(i, j + e, v);
+                        }
+                    }
+                }
+        }
+    }
+}
+
+// The slices' partial sums, added in slice order, and the epilogue.
+template <class T, int RUN>
+__global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
+    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * RUN;
+    const int64_t plane = g.ni * g.nj;
+    if (k >= plane) return;
+    float v[RUN];
+#pragma unroll
+    for (int e = 0; e < RUN; e++) v[e] = 0.f;
+    for (int s = 0; s < g.slices; s += 4) {
+        Run<float, RUN> q[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (s + u < g.slices) q[u] = *reinterpret_cast<const Run<float, RUN>*>(g.partial + (int64_t)(s + u) * plane + k);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (s + u < g.slices)
+#pragma unroll
+                for (int e = 0; e < RUN; e++) v[e] += q[u].v[e];
+    }
+    finish<T, RUN>(g, k / g.nj, k % g.nj, v);
+}
+
+// ---- the activation's gradient and column sums ----------------------------------------------------------------------------------
+
+struct SlopeParams {
+    const void* dy;                      // [rows][ld]
+    const void* y;                       // the layer's output, or NULL   (slope by its sign)
+    const uint8_t* positive;             // or NULL
+    const float* z;                      // or NULL
+    void* s;                             // [rows][cols], or NULL: column sums only
+    float* partial;                      // [row blocks][cols]
+    void* sums;                          // [cols], written directly when there is one row block
+    int64_t rows, cols, ld;
+    int rows_per_block;
+    int act;
+    float alpha, sign;                   // sign: of the layer's gain
+    float scale;
+};
+
+// A workgroup: 64 * N columns (N: elements per lane, one 16-byte packet or a single one), rows_per_block rows, the waves taking
+// every fourth row.
+template <class T, int N>
+__global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) {
+    constexpr int UNROLL = 4;
+    __shared__ float part[4][64 * N];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * N;
+    const bool inside = c < p.cols;
+    const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
+    float sum[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) sum[e] = 0.f;
+    for (int64_t r = r0 + wave; r < r1; r += 4 * UNROLL) {
+        Run<T, N> dy[UNROLL], y[UNROLL];
+        Run<uint8_t, N> pos[UNROLL];
+        Run<float, N> z[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const int64_t row = r + 4 * u;
+            if (!inside || row >= r1) continue;
+            dy[u] = *reinterpret_cast<const Run<T, N>*>((const T*)p.dy + row * p.ld + c);
+            const int64_t at = row * p.cols + c;
+            if (p.y) y[u] = *reinterpret_cast<const Run<T, N>*>((const T*)p.y + at);
+            if (p.positive) pos[u] = *reinterpret_cast<const Run<uint8_t, N>*>(p.positive + at);
+            if (p.z) z[u] = *reinterpret_cast<const Run<float, N>*>(p.z + at);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const int64_t row = r + 4 * u;
+            if (!inside || row >= r1) continue;
+            Run<T, N> out;
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                float s = Elem<T>::load(dy[u].v[e]);
+                if (p.y) s = Elem<T>::load(y[u].v[e]) * p.sign > 0.f ? s : s * p.alpha;
+                else if (p.positive) s = pos[u].v[e] ? s : s * p.alpha;
+                else if (p.z) s *= slope_at(p.act, z[u].v[e]);
+                sum[e] += s;
+                out.v[e] = Elem<T>::store(s);
+            }
+            if (p.s) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.cols + c) = out;
+        }
+    }
+    if (p.sums == nullptr) return;
+#pragma unroll
+    for (int e = 0; e < N; e++) part[wave][lane * N + e] = sum[e];
+    __syncthreads();
+    for (int k = threadIdx.x; k < 64 * N; k += 256) {
+        const int64_t col = (int64_t)blockIdx.x * 64 * N + k;
+        if (col >= p.cols) break;
+        const float total = (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
+        if (gridDim.y == 1) ((T*)p.sums)[col] = Elem<T>::store(total * p.scale);
+        else p.partial[(int64_t)blockIdx.y * p.cols + col] = total;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(1024) column_join_kernel(const float* __restrict__ partial, int blocks, int64_t cols, float scale, T* __restrict__ out) {
+    __shared__ float part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    float sum = 0.f;
+    for (int b = wave; b < blocks; b += 16 * 4) {
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = b + 16 * u < blocks && c < cols ? partial[(int64_t)(b + 16 * u) * cols + c] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; u++) sum += v[u];
+    }
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && c < cols) {
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; w++) sum += part[w][lane];
+        out[c] = Elem<T>::store(sum * scale);
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------------
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Rows per workgroup of the slope kernel: 32, doubled up to 256 while more than 2048 workgroups remain (fewer partial sums), or
+// all rows up to 64.
+int slope_rows(int64_t rows, int64_t cols) {
+    if (rows <= 64) return 64;
+    int per = 32;
+    while (per < 256 && (rows + per - 1) / per * ((cols + 255) / 256) > 2048) per *= 2;
+    while ((rows + per - 1) / per > 65535) per *= 2;
+    return per;
+}
+
+int64_t slope_blocks(int64_t rows, int64_t cols) { return rows == 0 ? 0 : (rows + slope_rows(rows, cols) - 1) / slope_rows(rows, cols); }
+
+template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* what) {
+    if (p.cols == 0) return SG_OK;
+    p.rows_per_block = slope_rows(p.rows, p.cols);
+    constexpr int N = Pack<T>::N;
+    const bool packed = p.cols % N == 0 && p.ld % N == 0 && aligned16(p.dy) && aligned16(p.y) && aligned16(p.s) && aligned16(p.z) &&
+                        reinterpret_cast<uintptr_t>(p.positive) % N == 0;
+    const int n = packed ? N : 1;
+    const int64_t bx = (p.cols + 64 * n - 1) / (64 * n), by = p.rows == 0 ? 1 : slope_blocks(p.rows, p.cols);
+    SG_REQUIRE(bx <= INT32_MAX && by <= 65535, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    const dim3 grid((unsigned)bx, (unsigned)by);
+    if (packed) hipLaunchKernelGGL((linear_slope_kernel<T, N>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((linear_slope_kernel<T, 1>), grid, dim3(256), 0, stream, p);
+    if (p.sums && by > 1)
+        hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((p.cols + 63) / 64)), dim3(1024), 0, stream, p.partial, (int)by, p.cols, p.scale, (T*)p.sums);
+    return check_launch(what);
+}
+
+struct Shape {                            // workgroup tile and slices of one product
+    int bi = 0, bj = 0;
+    int tiles_i = 0, tiles_j = 0, slices = 1, slice_steps = 1;
+    size_t partial_bytes = 0;
+};
+
+Shape shape_of(int dtype, int64_t ni, int64_t nj, int64_t np) {
+    Shape s;
+    const int bk = dtype == SG_F32 ? 32 : 64;
+    auto count = [&](int t) { return ((ni + t - 1) / t) * ((nj + t - 1) / t); };
+    int t = 64;
+    if (dtype != SG_F32 && count(256) >= 192) t = 256;
+    else if (count(128) >= 192) t = 128;
+    s.bi = s.bj = t;
+    s.tiles_i = (int)((ni + t - 1) / t);
+    s.tiles_j = (int)((nj + t - 1) / t);
+    const int64_t steps = (np + bk - 1) / bk, tiles = (int64_t)s.tiles_i * s.tiles_j;
+    int64_t slices = 1;
+    if (tiles < 192 && steps > 1) {
+        slices = 512 / tiles;
+        if (slices > steps / 2) slices = steps / 2;
+        if (slices > 64) slices = 64;
+        if (slices < 1) slices = 1;
+    }
+    s.slice_steps = (int)(steps < 1 ? 1 : (steps + slices - 1) / slices);
+    s.slices = (int)(steps < 1 ? 1 : (steps + s.slice_steps - 1) / s.slice_steps);
+    if (s.slices > 1) s.partial_bytes = up256((size_t)s.slices * ni * nj * 4);
+    return s;
+}
+
+template <class T, int BI, int WI, int WJ, bool RA, bool RB>
+void launch_gemm(const Gemm& g, bool direct, bool runs, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices)), block(WI * WJ * 64);
+    if (direct) {
+        if (runs) hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, true, 4>), grid, block, 0, stream, g);
+        else hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, true, 1>), grid, block, 0, stream, g);
+    } else {
+        if (runs) hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, false, 4>), grid, block, 0, stream, g);
+        else hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, false, 1>), grid, block, 0, stream, g);
+    }
+}
+
+template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
+    constexpr int ES = sizeof(T), E = 16 / ES;
+    if (g.ni == 0 || g.nj == 0) return SG_OK;
+    g.tiles_i = s.tiles_i; g.tiles_j = s.tiles_j; g.slices = s.slices; g.slice_steps = s.slice_steps;
+    SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    // offsets within a tile's lines are 32-bit
+    SG_REQUIRE((g.lda + 1) * ES * 256 < (int64_t)kOutside && (g.ldb + 1) * ES * 256 < (int64_t)kOutside, SG_ERR_UNSUPPORTED,
+               "%s: rows of %lld / %lld elements are too long", what, (long long)g.lda, (long long)g.ldb);
+    const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && (RA ? g.np : g.ni) % E == 0 && (RB ? g.np : g.nj) % E == 0;
+    const bool runs = runs_aligned<T>(g, 4);
+    if constexpr (ES == 2) {
+        if (s.bi == 256) launch_gemm<T, 256, 2, 4, RA, RB>(g, direct, runs, stream);
+        else if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, runs, stream);
+        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, runs, stream);
+    } else {
+        if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, runs, stream);
+        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, runs, stream);
+    }
+    if (g.slices > 1) {
+        const int run = runs ? 4 : 1;
+        const int64_t blocks = (g.ni * g.nj / run + 255) / 256;
+        SG_REQUIRE(blocks <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+        if (runs) hipLaunchKernelGGL((linear_join_kernel<T, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+        else hipLaunchKernelGGL((linear_join_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+    }
+    return check_launch(what);
+}
+
+int check(const sg_linear_params* p, const char* what) {
+    SG_REQUIRE(p != nullptr, SG_ERR_NULL_POINTER, "params is NULL");
+    SG_REQUIRE(p->dtype == SG_F32 || p->dtype == SG_F16 || p->dtype == SG_BF16, SG_ERR_UNSUPPORTED, "%s: dtype %d (float32, float16 or bfloat16)", what, p->dtype);
+    SG_REQUIRE(p->act >= kActLinear && p->act <= kActSwish, SG_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, p->act);
+    SG_REQUIRE(p->m >= 0 && p->n >= 0 && p->k >= 0 && p->m <= INT32_MAX && p->n <= INT32_MAX && p->k <= INT32_MAX, SG_ERR_INVALID_ARGUMENT,
+               "%s: sizes %lld, %lld, %lld", what, (long long)p->m, (long long)p->n, (long long)p->k);
+    SG_REQUIRE(p->ldx >= p->k && p->ldw >= p->k && p->ldr >= 0, SG_ERR_INVALID_ARGUMENT, "%s: row strides are smaller than rows", what);
+    SG_REQUIRE(p->m == 0 || p->n == 0 || p->k == 0 || (p->x && p->w), SG_ERR_NULL_POINTER, "%s: x or w is NULL", what);
+    return SG_OK;
+}
+
+bool piecewise(int act) { return act == kActRelu || act == kActLrelu; }
+
+struct BackwardPlan {
+    Shape x, w;
+    size_t s = 0, sums = 0, partial = 0, total = 0;      // offsets: the activation's gradient, row-block sums, slices
+};
+
+BackwardPlan plan_backward(const sg_linear_params& p) {
+    BackwardPlan b;
+    const int es = p.dtype == SG_F32 ? 4 : 2;
+    size_t at = 0;
+    b.s = at;
+    if (p.act != kActLinear) at += up256((size_t)p.m * p.n * es);
+    b.sums = at;
+    at += up256((size_t)slope_blocks(p.m, p.n) * p.n * 4);
+    b.x = shape_of(p.dtype, p.m, p.k, p.n);
+    b.w = shape_of(p.dtype, p.n, p.k, p.m);
+    b.partial = at;
+    at += b.x.partial_bytes > b.w.partial_bytes ? b.x.partial_bytes : b.w.partial_bytes;
+    b.total = at;
+    return b;
+}
+
+}  // namespace
+
+size_t column_sums_workspace_bytes(int64_t rows, int64_t cols) { return up256((size_t)slope_blocks(rows, cols) * cols * 4); }
+
+int column_sums(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ld, float scale, void* out, void* workspace, hipStream_t stream) {
+    SlopeParams p{};
+    p.dy = g; p.partial = (float*)workspace; p.sums = out;
+    p.rows = rows; p.cols = cols; p.ld = ld; p.scale = scale;
+    SG_DISPATCH_DTYPE(dtype, false, return run_slope<T>(p, stream, "column sums"));
+    return SG_OK;
+}
+
+}  // namespace sg
+
+extern "C" size_t sg_linear_workspace_bytes(const sg_linear_params* p) {
+    using namespace sg;
+    if (check(p, "linear") != SG_OK) return 0;
+    return shape_of(p->dtype, p->m, p->n, p->k).partial_bytes;
+}
+
+extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* positive, void* workspace, size_t workspace_bytes, sg_stream_t stream) {
+    using namespace sg;
+    const int rc = check(p, "linear");
+    if (rc != SG_OK) return rc;
+    if (p->m == 0 || p->n == 0) return SG_OK;
+    SG_REQUIRE(y != nullptr, SG_ERR_NULL_POINTER, "linear: y is NULL");
+    SG_REQUIRE(p->residual == nullptr || p->ldr >= p->n, SG_ERR_INVALID_ARGUMENT, "linear: the residual's row stride is smaller than its rows");
+    const Shape s = shape_of(p->dtype, p->m, p->n, p->k);
+    SG_REQUIRE(s.partial_bytes == 0 || (workspace && workspace_bytes >= s.partial_bytes && aligned16(workspace)), SG_ERR_INVALID_ARGUMENT,
+               "linear: needs %zu bytes of aligned workspace", s.partial_bytes);
+    Gemm g{};
+    g.a = p->x; g.lda = p->ldx; g.b = p->w; g.ldb = p->ldw;
+    g.ni = p->m; g.nj = p->n; g.np = p->k;
+    g.partial = (float*)workspace;
+    g.out = y; g.scale = p->w_gain;
+    g.with_epilogue = 1;
+    g.bias = p->b; g.b_gain = p->b_gain;
+    g.residual = p->residual; g.ldr = p->ldr;
+    g.z = z; g.positive = positive;
+    g.act = p->act; g.alpha = p->alpha; g.gain = p->gain;
+    SG_DISPATCH_DTYPE(p->dtype, false, return (run_gemm<T, true, true>(g, s, (hipStream_t)stream, "sg_linear")));
+    return SG_OK;
+}
+
+extern "C" size_t sg_linear_backward_workspace_bytes(const sg_linear_params* p) {
+    using namespace sg;
+    if (check(p, "linear_backward") != SG_OK) return 0;
+    return plan_backward(*p).total;
+}
+
+extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, const void* y, const float* z, const uint8_t* positive, void* dx, void* dw,
+                                  void* db, void* workspace, size_t workspace_bytes, sg_stream_t stream_) {
+    using namespace sg;
+    const int rc = check(p, "linear_backward");
+    if (rc != SG_OK) return rc;
+    hipStream_t stream = (hipStream_t)stream_;
+    const bool any = p->m > 0 && p->n > 0;
+    SG_REQUIRE(!any || dy != nullptr, SG_ERR_NULL_POINTER, "linear_backward: dy is NULL");
+    const int given = (y != nullptr) + (z != nullptr) + (positive != nullptr);
+    SG_REQUIRE(!any || given == (p->act == kActLinear ? 0 : 1), SG_ERR_INVALID_ARGUMENT, "linear_backward: activation %d takes %s of y, z, positive", p->act,
+               p->act == kActLinear ? "none" : "one");
+    SG_REQUIRE(!any || p->act == kActLinear || (z != nullptr) != piecewise(p->act), SG_ERR_INVALID_ARGUMENT,
+               "linear_backward: activation %d takes %s", p->act, piecewise(p->act) ? "y or positive" : "z");
+    const BackwardPlan plan = plan_backward(*p);
+    SG_REQUIRE(plan.total == 0 || (workspace && workspace_bytes >= plan.total && aligned16(workspace)), SG_ERR_INVALID_ARGUMENT,
+               "linear_backward: needs %zu bytes of aligned workspace", plan.total);
+    char* ws = (char*)workspace;
+    const bool own_s = p->act != kActLinear;
+    const void* s = own_s ? (const void*)(ws + plan.s) : dy;
+    if ((own_s && any && (dx || dw)) || db) {
+        SlopeParams q{};
+        q.dy = dy; q.y = y; q.positive = positive; q.z = z;
+        q.s = own_s && (dx || dw) ? ws + plan.s : nullptr;
+        q.partial = (float*)(ws + plan.sums);
+        q.sums = db;
+        q.rows = p->m; q.cols = p->n; q.ld = p->n;
+        q.act = p->act;
+        q.alpha = p->act == kActRelu ? 0.f : p->alpha;
+        q.sign = p->gain < 0.f ? -1.f : 1.f;
+        q.scale = p->gain * p->b_gain;
+        int done = SG_OK;
+        SG_DISPATCH_DTYPE(p->dtype, false, done = run_slope<T>(q, stream, "sg_linear_backward"));
+        if (done != SG_OK) return done;
+    }
+    Gemm g{};
+    g.partial = (float*)(ws + plan.partial);
+    g.scale = p->gain * p->w_gain;
+    if (dx) {                            // [m, k] = s [m, n] w [n, k]
+        Gemm q = g;
+        q.a = s; q.lda = p->n; q.b = p->w; q.ldb = p->ldw;
+        q.ni = p->m; q.nj = p->k; q.np = p->n;
+        q.out = dx;
+        int done = SG_OK;
+        SG_DISPATCH_DTYPE(p->dtype, false, done = (run_gemm<T, true, false>(q, plan.x, stream, "sg_linear_backward")));
+        if (done != SG_OK) return done;
+    }
+    if (dw) {                            // [n, k] = s [m, n]^T x [m, k]
+        Gemm q = g;
+        q.a = s; q.lda = p->n; q.b = p->x; q.ldb = p->ldx;
+        q.ni = p->n; q.nj = p->k; q.np = p->m;
+        q.out = dw;
+        int done = SG_OK;
+        SG_DISPATCH_DTYPE(p->dtype, false, done = (run_gemm<T, false, false>(q, plan.w, stream, "sg_linear_backward")));
+        if (done != SG_OK) return done;
+    }
+    return SG_OK;
+}

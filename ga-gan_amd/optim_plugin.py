@@ -1,5 +1,7 @@
 """Binding of `sg_adam_step` / `sg_lerp_multi` (include/sg_ops.h): the optimizer step of a
-training phase and the generator's moving average, each as one launch per 64 tensors.
+training phase and the generator's moving average, each as one launch per 64 tensors; and of
+`sg_grad_norm` / `sg_scale_grads` / `sg_adam_step_list`: the global norm of a list of gradients, clipping
+by it, and the step with the clip applied as the gradients are read.
 
 `FusedAdam` stands in for the `torch.optim.Adam(params, lr, betas, eps)` the reference's
 loop constructs (training/training_loop.py:303-312) together with the gradient
@@ -39,11 +41,155 @@ def _check(t, what):
         raise RuntimeError(f'{what} must be a dense float32 tensor')
 
 
-def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit=1e5):
+class GradList(ctypes.Structure):
+    _fields_ = [('grads', ctypes.c_void_p), ('numel', ctypes.c_void_p), ('dtype', ctypes.c_void_p), ('count', ctypes.c_int32)]
+
+
+class AdamList(ctypes.Structure):
+    _fields_ = [('param', ctypes.c_void_p), ('grad', ctypes.c_void_p), ('exp_avg', ctypes.c_void_p), ('exp_avg_sq', ctypes.c_void_p),
+                ('numel', ctypes.c_void_p), ('step', ctypes.c_void_p), ('count', ctypes.c_int32), ('lr', ctypes.c_float),
+                ('beta1', ctypes.c_float), ('beta2', ctypes.c_float), ('eps', ctypes.c_float), ('grad_limit', ctypes.c_float),
+                ('grad_scale', ctypes.c_void_p)]
+
+
+_NORM_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+CLIP_EPS = 1e-6        # added to the norm a gradient is divided by, as torch.nn.utils.clip_grad_norm_ does
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _distinct(pointers, numels, what):
+    used = [p for p, n in zip(pointers, numels) if n]
+    if len(set(used)) != len(used):
+        raise RuntimeError(f'{what}: a tensor appears twice')
+
+
+class _Grads:
+    """Host arrays of a list of gradients (kept alive while the library reads them)."""
+
+    def __init__(self, grads, what):
+        self.device = grads[0].device
+        codes = []
+        for g in grads:
+            code = _NORM_DTYPES.get(g.dtype)
+            if code is None:
+                raise RuntimeError(f'{what}: unsupported dtype {g.dtype}')
+            if not g.is_cuda or g.device != self.device:
+                raise RuntimeError(f'{what}: gradients must reside on one CUDA device')
+            if not g.is_contiguous():
+                raise RuntimeError(f'{what}: gradients must be dense')
+            codes.append(code)
+        count = len(grads)
+        self.tensors = grads
+        self.pointers = _pointers(grads)
+        self.numels = [g.numel() for g in grads]
+        self.numel = (ctypes.c_int64 * count)(*self.numels)
+        self.dtype = (ctypes.c_int32 * count)(*codes)
+        self.args = GradList(ctypes.cast(self.pointers, ctypes.c_void_p), ctypes.cast(self.numel, ctypes.c_void_p),
+                             ctypes.cast(self.dtype, ctypes.c_void_p), count)
+
+    def norm(self, grad_limit, max_norm):
+        """float32 [2] on the device: the norm, and min(1, max_norm / (norm + 1e-6))."""
+        handle = _lib.lib()
+        need = handle.sg_grad_norm_workspace_bytes(ctypes.byref(self.args))
+        out = torch.empty([2], dtype=torch.float32, device=self.device)
+        work = torch.empty([max(need, 8)], dtype=torch.uint8, device=self.device)
+        _lib.launch_raw(lambda stream: handle.sg_grad_norm(ctypes.byref(self.args), grad_limit, max_norm, CLIP_EPS, _lib.ptr(out), _lib.ptr(work),
+                                                           need, stream), out, 'sg_grad_norm', 'grad_norm_kernel', _lib.nbytes(*self.tensors))
+        return out
+
+
+def _max_norm(value, what):
+    value = float(value)
+    if not value >= 0:
+        raise RuntimeError(f'{what}: the largest norm must not be negative')
+    return value
+
+
+def grad_norm(grads, grad_limit=None):
+    """sqrt(sum of squares over all elements of all tensors of `grads`) as a float32 scalar on their device (nothing waits for it).
+    float32, float16 and bfloat16 tensors in any mixture and number, dense, on one device; squares are summed in double, in an
+    order that depends on the sizes alone.  `grad_limit`: the norm of the gradients as `adam_step` sanitises them
+    (NaN -> 0, +-Inf -> +-grad_limit); None: as they are.  An empty list has norm zero (a host scalar)."""
+    grads = list(grads)
+    if not grads:
+        return torch.zeros([])
+    if grad_limit is not None and not float(grad_limit) > 0:
+        raise RuntimeError('grad_norm: grad_limit must be positive')
+    return _Grads(grads, 'grad_norm').norm(float(grad_limit or 0), 0.0)[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """Scale the gradients of `parameters` (a tensor or an iterable; those without one are skipped) in place by
+    min(1, max_norm / (norm + 1e-6)) and return their global norm before that: torch.nn.utils.clip_grad_norm_ for the 2-norm, in
+    a launch per 128 tensors and one more, then another pass over the gradients only if they are too long.  A norm that is not
+    finite makes the gradients NaN or zero, as there.  No gradient may overlap another.  `FusedAdam(max_grad_norm=...)` clips
+    without the second pass."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    max_norm = _max_norm(max_norm, 'clip_grad_norm_')
+    params = [p for p in parameters if p.grad is not None]
+    if not params:
+        return torch.zeros([])
+    for p in params:
+        if not p.grad.is_contiguous():
+            p.grad = p.grad.contiguous()
+    grads = _Grads([p.grad for p in params], 'clip_grad_norm_')
+    _distinct(grads.pointers, grads.numels, 'clip_grad_norm_')
+    out = grads.norm(0.0, max_norm)
+    handle = _lib.lib()
+    _lib.launch_raw(lambda stream: handle.sg_scale_grads(ctypes.byref(grads.args), ctypes.c_void_p(out.data_ptr() + 4), stream), out, 'sg_scale_grads',
+                    'grad_scale_kernel', 2 * _lib.nbytes(*grads.tensors))
+    torch.autograd.graph.increment_version(grads.tensors)
+    return out[0]
+
+
+def _check_list(lists, device):
+    params = lists[0][1]
+    for what, tensors in lists:
+        for t, p in zip(tensors, params):
+            if not (t.is_cuda and t.dtype is torch.float32 and t.is_contiguous() and t.device == device) or t.shape != p.shape:
+                _check(t, what)
+                raise RuntimeError(f'adam_step: {what} {tuple(t.shape)} on {t.device} does not match its parameter {tuple(p.shape)} on {device}')
+
+
+def _adam_step_scaled(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, scale):
+    """The update with gradients scaled by the device value `scale` (float32, one element) as they are read."""
+    count = len(params)
+    device = scale.device
+    lists = (('param', params), ('grad', grads), ('exp_avg', exp_avgs), ('exp_avg_sq', exp_avg_sqs))
+    _check_list(lists, device)
+    arrays = [_pointers(tensors) for _, tensors in lists]
+    numels = [p.numel() for p in params]
+    _distinct([p for a in arrays for p in a], numels * 4, 'adam_step')
+    numel = (ctypes.c_int64 * count)(*numels)
+    step = (ctypes.c_int32 * count)(*[int(k) for k in steps])
+    args = AdamList(*[ctypes.cast(a, ctypes.c_void_p) for a in arrays], ctypes.cast(numel, ctypes.c_void_p), ctypes.cast(step, ctypes.c_void_p),
+                    count, lr, beta1, beta2, eps, grad_limit, scale.data_ptr())
+    _lib.launch('sg_adam_step_list', args, scale, 'adam_kernel', 32 * sum(numels))
+    torch.autograd.graph.increment_version(list(params) + list(grads) + list(exp_avgs) + list(exp_avg_sqs))
+
+
+def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit=1e5, max_grad_norm=None):
     """In-place update of `params` (and of the moment estimates; `grads` are sanitised in place).  `steps[i]` is
-    the number of updates tensor i has received including this one."""
+    the number of updates tensor i has received including this one.  With `max_grad_norm` the update uses the sanitised
+    gradients times min(1, max_grad_norm / (their global norm + 1e-6)) and returns that norm (a device scalar); `grads` keep
+    the sanitised, unscaled values."""
     if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps)):
         raise RuntimeError('adam_step: lists differ in length')
+    if max_grad_norm is not None:
+        max_grad_norm = _max_norm(max_grad_norm, 'adam_step')
+        if not params:
+            return torch.zeros([])
+        if not grad_limit > 0:
+            raise RuntimeError('adam_step: grad_limit must be positive')
+        _check_list((('param', params), ('grad', grads)), params[0].device)
+        out = _Grads(list(grads), 'adam_step').norm(grad_limit, max_grad_norm)
+        _adam_step_scaled(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, out[1:])
+        return out[0]
     for i in range(0, len(params), MAX_TENSORS):
         chunk = range(i, min(i + MAX_TENSORS, len(params)))
         table = (AdamTensor * len(chunk))()
@@ -86,10 +232,18 @@ def ema_(dsts, srcs, beta):
 class FusedAdam(torch.optim.Optimizer):
     """Adam without weight decay / amsgrad whose `step()` sanitises the gradients and updates every parameter
     that has one in a single launch per 64 tensors.  State layout (`step`, `exp_avg`, `exp_avg_sq` per parameter)
-    and `state_dict()` follow torch.optim.Adam, so checkpoints of one load into the other."""
+    and `state_dict()` follow torch.optim.Adam, so checkpoints of one load into the other.
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, grad_limit=1e5):
+    `max_grad_norm` clips by the global norm of all the sanitised gradients of a step, over every parameter group: the norm
+    costs one more read of the gradients, the scaling nothing (it happens as the update reads them; `.grad` keeps the
+    sanitised values).  It is a property of the optimizer, not of its groups or its state dict, and may be changed between
+    steps; `last_grad_norm` is the norm of the last step that clipped (a device scalar).  All parameters must then live on
+    one device."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, grad_limit=1e5, max_grad_norm=None):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, grad_limit=grad_limit))
+        self.max_grad_norm = None if max_grad_norm is None else _max_norm(max_grad_norm, 'FusedAdam')
+        self.last_grad_norm = None
 
     def load_state_dict(self, state_dict):
         """As torch.optim.Optimizer.load_state_dict; the step counts are brought back to the host afterwards (a
@@ -106,6 +260,7 @@ class FusedAdam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        work = []
         for group in self.param_groups:
             params, grads, ms, vs, steps = [], [], [], [], []
             for p in group['params']:
@@ -125,6 +280,18 @@ class FusedAdam(torch.optim.Optimizer):
                 vs.append(state['exp_avg_sq'])
                 steps.append(int(state['step']))
             if params:
-                beta1, beta2 = group['betas']
-                adam_step(params, grads, ms, vs, steps, group['lr'], beta1, beta2, group['eps'], group['grad_limit'])
+                work.append((group, (params, grads, ms, vs, steps)))
+        if self.max_grad_norm is None:
+            for group, lists in work:
+                adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'])
+        elif len(work) == 1:
+            group, lists = work[0]
+            self.last_grad_norm = adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], self.max_grad_norm)
+        elif work:
+            if len({group['grad_limit'] for group, _ in work}) > 1:
+                raise RuntimeError('FusedAdam: parameter groups that are clipped together must share grad_limit')
+            out = _Grads([g for _, lists in work for g in lists[1]], 'FusedAdam').norm(work[0][0]['grad_limit'], self.max_grad_norm)
+            for group, lists in work:
+                _adam_step_scaled(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], out[1:])
+            self.last_grad_norm = out[0]
         return loss

@@ -508,6 +508,48 @@ typedef struct sg_adam_params {
 
 int sg_adam_step(const sg_adam_params* p, sg_stream_t stream);
 
+/* The same update over a list of any length (a launch per SG_OPTIM_MAX_TENSORS tensors), given as parallel host arrays, with
+ * the gradients optionally scaled as they enter it: g * *grad_scale, grad_scale a device value such as the second one that
+ * sg_grad_norm writes (clipping by the global norm), or NULL.  What is written back to grad is the sanitised gradient, not
+ * the scaled one.  No tensor may overlap another of the list.  The reference's loop does not clip. */
+typedef struct sg_adam_list {
+    float* const* param;
+    float* const* grad;
+    float* const* exp_avg;
+    float* const* exp_avg_sq;
+    const int64_t* numel;
+    const int32_t* step;
+    int32_t count;
+    float lr, beta1, beta2, eps, grad_limit;
+    const float* grad_scale; /* device, or NULL */
+} sg_adam_list;
+
+int sg_adam_step_list(const sg_adam_list* p, sg_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Global norm of a list of gradients (float32, float16 and bfloat16 mixed as they come), and clipping by it:
+ *   out[0] = norm = sqrt(sum over all tensors and elements of g^2)
+ *   out[1] = min(1, max_norm / (norm + eps))
+ * grad_limit > 0 takes the norm of the gradients as sg_adam_step sanitises them (NaN -> 0, +-Inf -> +-grad_limit);
+ * grad_limit <= 0 takes them as they are, and a NaN or an infinity then shows in both values.  Squares and sums are
+ * double; the result does not depend on scheduling.  `out` is device memory (2 floats), `workspace` device memory of
+ * sg_grad_norm_workspace_bytes(p) bytes, 8-byte aligned, private to the call until the stream has passed it.  The list
+ * is host memory and is consumed before the call returns.
+ * sg_scale_grads multiplies every tensor of the list by the device value *scale in place (a scale of 1 touches nothing);
+ * no tensor may overlap another of the list.
+ * Together they are torch.nn.utils.clip_grad_norm_ without a host read; the reference's loop does not clip. */
+typedef struct sg_grad_list {
+    void* const* grads;
+    const int64_t* numel;
+    const int32_t* dtype; /* sg_dtype of every tensor */
+    int32_t count;
+} sg_grad_list;
+
+size_t sg_grad_norm_workspace_bytes(const sg_grad_list* p);
+int sg_grad_norm(const sg_grad_list* p, float grad_limit, float max_norm, float eps, float* out, void* workspace,
+                 size_t workspace_bytes, sg_stream_t stream);
+int sg_scale_grads(const sg_grad_list* p, const float* scale, sg_stream_t stream);
+
 /* dst = src + beta * (dst - src) over a list of float32 tensors in one launch: the moving average of the generator
  * weights, `p_ema.copy_(p.lerp(p_ema, ema_beta))` with dst = p_ema, src = p (training/training_loop.py:516-521). */
 typedef struct sg_lerp_tensor {
@@ -523,6 +565,66 @@ typedef struct sg_lerp_params {
 } sg_lerp_params;
 
 int sg_lerp_multi(const sg_lerp_params* p, sg_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Fully connected layer with its epilogue:
+ *   z = x w^T * w_gain + b * b_gain        y = act(z) * gain + residual
+ * x [m, k] and w [n, k] with unit stride along k and ldx / ldw elements between rows, b [n] or NULL, residual [m, n] with ldr
+ * elements between rows or NULL, y [m, n] dense; all of `dtype` (SG_F32, SG_F16, SG_BF16), with float32 sums and one rounding.
+ * act counts as in sg_bias_act (1 linear .. 9 swish); alpha is the slope of lrelu.  k == 0 gives z = b * b_gain.
+ * For the backward pass the call also writes, where the pointer is not NULL, z [m, n] (float32) and positive [m, n] (z > 0).
+ * It stands for the `FullyConnectedLayer.forward` of training/networks.py:691-700 (a library product and `bias_act`).
+ *
+ * Backward: with s = dy * act'(z), dy [m, n] dense,
+ *   dx [m, k] = s w * (gain w_gain)     dw [n, k] = s^T x * (gain w_gain)     db [n] = column sums of s * (gain b_gain)
+ * each dense, of `dtype`, and skipped when its pointer is NULL.  The slope comes from exactly one of: y (the layer's output, for
+ * relu / lrelu without a residual and with gain != 0), positive (relu / lrelu), z (every other activation but linear, which
+ * takes none).  p->b and p->residual are not read.  `workspace`: device memory, 16-byte aligned, private to the call until the
+ * stream has passed it.  Sums run in an order that depends on the sizes alone. */
+typedef struct sg_linear_params {
+    const void* x;
+    const void* w;
+    const void* b;
+    const void* residual;
+    int32_t dtype, act;
+    float alpha, gain, w_gain, b_gain;
+    int64_t m, n, k;
+    int64_t ldx, ldw, ldr;
+} sg_linear_params;
+
+size_t sg_linear_workspace_bytes(const sg_linear_params* p);
+int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* positive, void* workspace, size_t workspace_bytes,
+              sg_stream_t stream);
+size_t sg_linear_backward_workspace_bytes(const sg_linear_params* p);
+int sg_linear_backward(const sg_linear_params* p, const void* dy, const void* y, const float* z, const uint8_t* positive,
+                       void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes, sg_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Rows of a table by index, scaled, plus a bias:
+ *   y[t][f] = table[index[t]][f] * w_gain + bias[f] * b_gain
+ * index [tokens] int32 or int64 (index_bytes 4 or 8, device memory); table [v, f] with strides in elements in either order,
+ * bias [f] or NULL, y [tokens, f] dense; all of `dtype` (SG_F32, SG_F16, SG_BF16).  The product and the sum are rounded to
+ * float32 one after the other, so that with float32 the result is bit for bit what a product with one-hot rows gives: it stands
+ * for the label embedding `self.embed(c)` of training/networks.py:732, 748.  An index outside [0, v) yields a row of NaN.
+ *
+ * Backward: p->table is the table's gradient, dense in either order ([v, f] or its transpose), 16-byte aligned, and written whole:
+ *   dtable[v][f] = w_gain * sum over the tokens t with index[t] == v, in order, of dy[t][f]      (zero without tokens)
+ *   dbias[f]     = b_gain * sum over all tokens of dy[t][f]                                       (skipped when NULL)
+ * Sums are float32 in an order that depends on the inputs alone (no atomics).  An index outside the table adds to no row.
+ * `workspace`: device memory, 16-byte aligned, private to the call until the stream has passed it. */
+typedef struct sg_embedding_params {
+    const void* index;
+    const void* table;
+    const void* bias;
+    int32_t dtype, index_bytes;
+    int64_t tokens, v, f, stride_v, stride_f;
+    float w_gain, b_gain;
+} sg_embedding_params;
+
+int sg_embedding(const sg_embedding_params* p, void* y, sg_stream_t stream);
+size_t sg_embedding_backward_workspace_bytes(const sg_embedding_params* p);
+int sg_embedding_backward(const sg_embedding_params* p, const void* dy, void* dbias, void* workspace, size_t workspace_bytes,
+                          sg_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * A batch of training images from a uint8 image set resident in device memory:
