@@ -22,7 +22,7 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kStepBytes = 128;                    // of p per LDS tile: 64 16-bit or 32 float32 elements
 constexpr unsigned kOutside = 0x80000000u;         // a buffer offset beyond every descriptor: the load yields zeros
@@ -32,18 +32,26 @@ constexpr float kSeluScale = 1.0507009873554804934193349852946f, kSeluAlpha = 1.
 
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
 
-__device__ __forceinline__ float activate(int act, float alpha, float z) {
+template <int ACT> __device__ __forceinline__ float activation(float alpha, float z) {
+    if constexpr (ACT == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
+    if constexpr (ACT == kActLrelu) return z > 0.f ? z : z * alpha;
+    if constexpr (ACT == kActTanh) return tanhf(z);
+    if constexpr (ACT == kActSigmoid) return sigmoid(z);
+    if constexpr (ACT == kActElu) return z > 0.f ? z : expm1f(z);
+    if constexpr (ACT == kActSelu) return kSeluScale * (z > 0.f ? z : kSeluAlpha * expm1f(z));
+    if constexpr (ACT == kActSoftplus) return fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
+    if constexpr (ACT == kActSwish) return z * sigmoid(z);
+    return z;
+}
+
+// v = act(v) * gain for N values (one switch for all of them; the elements are a loop, not N copies of nine functions)
+template <int N> __device__ __forceinline__ void activate(int act, float alpha, float gain, float (&v)[N]) {
+#define SG_ACT(A) case A: _Pragma("unroll") for (int e = 0; e < N; e++) v[e] = activation<A>(alpha, v[e]) * gain; break;
     switch (act) {
-        case kActRelu: return z > 0.f ? z : (z != z ? z : 0.f);
-        case kActLrelu: return z > 0.f ? z : z * alpha;
-        case kActTanh: return tanhf(z);
-        case kActSigmoid: return sigmoid(z);
-        case kActElu: return z > 0.f ? z : expm1f(z);
-        case kActSelu: return kSeluScale * (z > 0.f ? z : kSeluAlpha * expm1f(z));
-        case kActSoftplus: return fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
-        case kActSwish: return z * sigmoid(z);
-        default: return z;
+        SG_ACT(kActRelu) SG_ACT(kActLrelu) SG_ACT(kActTanh) SG_ACT(kActSigmoid) SG_ACT(kActElu) SG_ACT(kActSelu) SG_ACT(kActSoftplus) SG_ACT(kActSwish)
+        SG_ACT(kActLinear)
     }
+#undef SG_ACT
 }
 
 // act'(z) of the activations that are not piecewise linear with corner at zero alone
@@ -70,8 +78,7 @@ struct Gemm {
     float* partial;                      // [slices][ni][nj] when slices > 1
     void* out;                           // [ni][nj]
     float scale;
-    // epilogue of the forward pass (with_epilogue)
-    int with_epilogue;
+    // epilogue of the forward pass
     const void* bias;                    // [nj]
     const void* residual;                // [ni][ldr]
     int64_t ldr;
@@ -79,52 +86,70 @@ struct Gemm {
     uint8_t* positive;                   // [ni][nj] or NULL: z > 0
     int act;
     float alpha, gain, b_gain;
+    int whole;                           // rows of everything the epilogue touches are whole aligned 16-byte packets
 };
 
-template <class T> struct Io;            // vectors of 1, 2 or 4 consecutive elements as float
 template <class T, int N> struct alignas(N * sizeof(T)) Run { T v[N]; };
 
-// N consecutive results (i, j .. j + N - 1), all inside.
-template <class T, int N>
+// N consecutive results (i, j .. j + N - 1), all inside; runs of N are aligned wherever they are read and written.
+template <class T, int N, bool FORWARD>
 __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int64_t j, float (&v)[N]) {
     const int64_t at = i * g.nj + j;
     Run<T, N> out;
-    if (!g.with_epilogue) {
 #pragma unroll
-        for (int e = 0; e < N; e++) out.v[e] = Elem<T>::store(v[e] * g.scale);
-        *reinterpret_cast<Run<T, N>*>((T*)g.out + at) = out;
-        return;
-    }
-    Run<T, N> bias, res;
-    if (g.bias) bias = *reinterpret_cast<const Run<T, N>*>((const T*)g.bias + j);
-    if (g.residual) res = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + i * g.ldr + j);
-    Run<float, N> zs;
-    Run<uint8_t, N> pos;
+    for (int e = 0; e < N; e++) v[e] *= g.scale;
+    if constexpr (FORWARD) {
+        Run<T, N> res;
+        if (g.residual) res = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + i * g.ldr + j);
+        if (g.bias) {
+            const Run<T, N> bias = *reinterpret_cast<const Run<T, N>*>((const T*)g.bias + j);
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-        float z = v[e] * g.scale;
-        if (g.bias) z += Elem<T>::load(bias.v[e]) * g.b_gain;
-        zs.v[e] = z;
-        pos.v[e] = z > 0.f;
-        float y = activate(g.act, g.alpha, z) * g.gain;
-        if (g.residual) y += Elem<T>::load(res.v[e]);
-        out.v[e] = Elem<T>::store(y);
+            for (int e = 0; e < N; e++) v[e] += Elem<T>::load(bias.v[e]) * g.b_gain;
+        }
+        if (g.z) {
+            Run<float, N> z;
+#pragma unroll
+            for (int e = 0; e < N; e++) z.v[e] = v[e];
+            *reinterpret_cast<Run<float, N>*>(g.z + at) = z;
+        }
+        if (g.positive) {
+            Run<uint8_t, N> pos;
+#pragma unroll
+            for (int e = 0; e < N; e++) pos.v[e] = v[e] > 0.f;
+            *reinterpret_cast<Run<uint8_t, N>*>(g.positive + at) = pos;
+        }
+        activate(g.act, g.alpha, g.gain, v);
+        if (g.residual)
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] += Elem<T>::load(res.v[e]);
     }
+#pragma unroll
+    for (int e = 0; e < N; e++) out.v[e] = Elem<T>::store(v[e]);
     *reinterpret_cast<Run<T, N>*>((T*)g.out + at) = out;
-    if (g.z) *reinterpret_cast<Run<float, N>*>(g.z + at) = zs;
-    if (g.positive) *reinterpret_cast<Run<uint8_t, N>*>(g.positive + at) = pos;
 }
 
 // Whether runs of N elements at multiples of N may be moved as one access: everything finish() touches keeps them aligned.
-template <class T> bool runs_aligned(const Gemm& g, int n) {
+template <class T> bool runs_aligned(const Gemm& g) {
+    const int n = 16 / (int)sizeof(T);
     auto ok = [&](const void* p, size_t bytes) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % bytes == 0; };
     return g.nj % n == 0 && ok(g.out, n * sizeof(T)) && ok(g.bias, n * sizeof(T)) && ok(g.residual, n * sizeof(T)) &&
-           (g.residual == nullptr || g.ldr % n == 0) && ok(g.z, n * 4) && ok(g.positive, n) && ok(g.partial, 16);
+           (g.residual == nullptr || g.ldr % n == 0) && ok(g.z, 16) && ok(g.positive, n);
 }
 
-__device__ __forceinline__ rsrc_t make_rsrc(const void* p) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)kOutside, 0x00020000);
+// Buffer descriptor of what follows p (offsets below kOutside).  p is the same in every lane of the wave.
+__device__ __forceinline__ i32x4_t descriptor(const void* p) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return i32x4_t{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), (int)kOutside, 0x00020000};
 }
+
+// 16 bytes per lane from `offset` behind the descriptor's address to LDS at lds + 16 * lane; zeros for kOutside.  Written as
+// assembly because of its wait: the compiler holds every LDS read behind all copies into LDS that came before it, those into
+// the other buffer included.  copies_landed() is the wait, and the kernel places it.
+__device__ __forceinline__ void copy_to_lds(i32x4_t from, unsigned offset, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "m0");
+}
+__device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
 // One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: SIDE * 8 slots of 16 bytes.
 //   ROWS:  slot (row, c) holds the 16 bytes c ^ ((row >> 1) & 7) of the row: 16 lanes reading one column of 16 rows hit 16
@@ -152,18 +177,29 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
             side = ((slot % LINE) ^ (swizzle(p) << 1)) * E;
         }
     }
-    // straight to LDS.  base: the tile's first element (of this step); left_*: valid extent from there
-    static __device__ __forceinline__ void load_direct(unsigned char* lds, const T* base, int64_t ld, int64_t left_side, int64_t left_p) {
-        const rsrc_t r = make_rsrc(base);
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // straight to LDS: per thread, the byte offsets of its slots within a step (kOutside where the row or column is)
+    struct Slots { unsigned off[LOADS]; };
+    static __device__ __forceinline__ void plan(Slots& s, int64_t ld, int64_t left_side) {
 #pragma unroll
         for (int k = 0; k < LOADS; k++) {
             int side, p;
             where(k * THREADS + threadIdx.x, side, p);
-            const unsigned off = (unsigned)((ROWS ? side : p) * (unsigned)ld + (ROWS ? p : side)) * ES;
-            const bool ok = side < left_side && p < left_p;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (k * THREADS + wave * 64) * 16), 16,
-                                                     ok ? off : kOutside, 0, 0, 0);
+            s.off[k] = side < left_side ? (unsigned)((ROWS ? side : p) * (unsigned)ld + (ROWS ? p : side)) * ES : kOutside;
+        }
+    }
+    // base: the tile's first element of this step; left_p: extent along p from there
+    static __device__ __forceinline__ void issue(const Slots& s, unsigned lds, const T* base, int64_t left_p) {
+        const i32x4_t from = descriptor(base);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int k = 0; k < LOADS; k++) {
+            unsigned off = s.off[k];
+            if (left_p < BK) {                                     // (the last step only)
+                int side, p;
+                where(k * THREADS + threadIdx.x, side, p);
+                off = p < left_p ? off : kOutside;
+            }
+            copy_to_lds(from, off, lds + (k * THREADS + wave * 64) * 16);
         }
     }
     // by way of registers: any alignment, any extent
@@ -256,9 +292,9 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Tile BI x BJ per workgroup of WI x WJ waves.  DIRECT: rows of both operands are whole aligned 16-byte packets.  RUN: elements
-// per store where the layout of the accumulators allows four in a row (1 otherwise).
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, bool DIRECT, int RUN>
+// Tile BI x BJ per workgroup of WI x WJ waves.  DIRECT: rows of both operands are whole aligned 16-byte packets.  Products of
+// two "rows" operands are the forward pass and carry its epilogue.
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, bool DIRECT>
 __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
     constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
     using TileA = Tile<T, BI, ROWS_A, THREADS>;
@@ -322,16 +358,21 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     // Two LDS buffers: the loads of step n + 1 are under way while step n multiplies; one barrier a step (after it every wave has
     // read the buffer that is filled next, and every wave's loads into the one that is read next have landed).
     if constexpr (DIRECT) {
-        auto issue = [&](int n, int buf) {
+        typename TileA::Slots sa;
+        typename TileB::Slots sb;
+        TileA::plan(sa, g.lda, left_i);
+        TileB::plan(sb, g.ldb, left_j);
+        const unsigned lds = lds_address(smem);
+        auto issue = [&](int n) {
             const int step = first + n;
-            TileA::load_direct(smem + buf * BUF, at_a(step), g.lda, left_i, g.np - (int64_t)step * BK);
-            TileB::load_direct(smem + buf * BUF + TileA::BYTES, at_b(step), g.ldb, left_j, g.np - (int64_t)step * BK);
+            TileA::issue(sa, lds + (n & 1) * BUF, at_a(step), g.np - (int64_t)step * BK);
+            TileB::issue(sb, lds + (n & 1) * BUF + TileA::BYTES, at_b(step), g.np - (int64_t)step * BK);
         };
-        if (steps > 0) issue(0, 0);
+        if (steps > 0) issue(0);
         for (int n = 0; n < steps; n++) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            copies_landed();
             __syncthreads();
-            if (n + 1 < steps) issue(n + 1, (n + 1) & 1);
+            if (n + 1 < steps) issue(n + 1);
             multiply(smem + (n & 1) * BUF);
         }
     } else {
@@ -358,64 +399,81 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         }
     }
 
-    // acc[t][s][r]: row i = tile s of A at lane % 16, column j = tile t of B at 4 * (lane / 16) + r
-    const int l16 = threadIdx.x & 15, quad = (threadIdx.x & 63) >> 4;
-    auto put = [&](int64_t i, int64_t j, auto& v) {
-        constexpr int N = sizeof(v) / 4;
-        if (g.slices > 1) {
-            float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
-            Run<float, N> w;
+    // acc[t][s][r]: row i = tile s of A at lane % 16, column j = tile t of B at 4 * (lane / 16) + r.  Each wave lays its part
+    // down in LDS as rows of four-column chunks (chunk c of row r at c ^ r: the 16 rows a store touches lie in 16 different
+    // 16-byte banks) and takes it up again in runs of consecutive columns: stores of 16 bytes, and one copy of the
+    // epilogue's code.
+    constexpr int COLS = BJ / WJ, CHUNKS = COLS / 4, ROWS_MAX = BUF * 2 / (WI * WJ) / (COLS * 4);
+    constexpr int S_PASS = ROWS_MAX / 16 < TI ? ROWS_MAX / 16 : TI;      // A tiles per pass
+    constexpr int N = 16 / (int)sizeof(T), RUNS = COLS / N;
+    static_assert(S_PASS >= 1 && TI % S_PASS == 0, "the epilogue's passes");
+    const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    float* mine = reinterpret_cast<float*>(smem) + wave * (S_PASS * 16 * COLS);
+    auto chunk_at = [&](int row, int chunk) -> f32x4_t& { return *reinterpret_cast<f32x4_t*>(mine + row * COLS + (chunk ^ (row & (CHUNKS - 1))) * 4); };
+    __syncthreads();                                                     // every wave is done with the tiles
 #pragma unroll
-            for (int e = 0; e < N; e++) w.v[e] = v[e];
-            *reinterpret_cast<Run<float, N>*>(out) = w;
-        } else {
-            finish<T, N>(g, i, j, v);
-        }
-    };
+    for (int s0 = 0; s0 < TI; s0 += S_PASS) {
 #pragma unroll
-    for (int s = 0; s < TI; s++) {
-        const int64_t i = i0 + wi + FragA::row(s, l16);
-        if (i >= g.ni) continue;
-        if constexpr (FragB::V == 1) {                    // the four values of a lane are consecutive columns
+        for (int s = 0; s < S_PASS; s++)
 #pragma unroll
             for (int t = 0; t < TJ; t++) {
-                const int64_t j = j0 + wj + t * 16 + quad * 4;
-                if constexpr (RUN == 4) {
-                    float v[4] = {acc[t][s][0], acc[t][s][1], acc[t][s][2], acc[t][s][3]};
-                    if (j < g.nj) put(i, j, v);
-                } else {
+                const f32x4_t(&c)[TI] = acc[t];
+                const int row = s * 16 + l16;
+                if constexpr (FragB::V == 1) {
+                    chunk_at(row, t * 4 + quad) = c[s0 + s];
+                } else if constexpr (FragB::V == 4) {                    // tiles t .. t + 3 hold consecutive columns
+                    if (t % 4 == 0)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        float v[1] = {acc[t][s][r]};
-                        if (j + r < g.nj) put(i, j + r, v);
-                    }
+                        for (int r = 0; r < 4; r++)
+                            chunk_at(row, t / 4 * 16 + quad * 4 + r) =
+                                f32x4_t{acc[t][s0 + s][r], acc[t + 1][s0 + s][r], acc[t + 2][s0 + s][r], acc[t + 3][s0 + s][r]};
+                } else {
+                    static_assert(FragB::V == 2 || FragB::V == 1 || FragB::V == 4, "interleaved tiles");
+                    if (t % 2 == 0)
+#pragma unroll
+                        for (int r = 0; r < 4; r += 2)
+                            chunk_at(row, t / 2 * 8 + quad * 2 + r / 2) =
+                                f32x4_t{acc[t][s0 + s][r], acc[t + 1][s0 + s][r], acc[t][s0 + s][r + 1], acc[t + 1][s0 + s][r + 1]};
                 }
             }
-        } else {                                          // V tiles hold consecutive columns
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+        for (int k = lane; k < S_PASS * 16 * RUNS; k += 64) {
+            const int row = k / RUNS, run = k % RUNS;
+            const int64_t i = i0 + wi + FragA::row(s0 + row / 16, row % 16), j = j0 + wj + run * N;
+            if (i >= g.ni || j >= g.nj) continue;
+            float v[N];
 #pragma unroll
-            for (int t = 0; t < TJ; t += FragB::V)
+            for (int q = 0; q < N / 4; q++) {
+                const f32x4_t c = chunk_at(row, run * (N / 4) + q);
+                v[4 * q] = c.x; v[4 * q + 1] = c.y; v[4 * q + 2] = c.z; v[4 * q + 3] = c.w;
+            }
+            if (g.slices > 1) {
+                float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
+                if (g.whole) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int64_t j = j0 + wj + FragB::row(t, quad * 4 + r);
-                    if constexpr (RUN == 4) {
-                        float v[FragB::V];
+                    for (int q = 0; q < N / 4; q++) *reinterpret_cast<f32x4_t*>(out + 4 * q) = f32x4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                } else {
 #pragma unroll
-                        for (int e = 0; e < FragB::V; e++) v[e] = acc[t + e][s][r];
-                        if (j < g.nj) put(i, j, v);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < FragB::V; e++) {
-                            float v[1] = {acc[t + e][s][r]};
-                            if (j + e < g.nj) put(i, j + e, v);
-                        }
-                    }
+                    for (int e = 0; e < N; e++)
+                        if (j + e < g.nj) out[e] = v[e];
                 }
+            } else if (g.whole) {
+                finish<T, N, ROWS_A && ROWS_B>(g, i, j, v);
+            } else {
+#pragma unroll 1
+                for (int e = 0; e < N && j + e < g.nj; e++) {
+                    float one[1] = {chunk_at(row, run * (N / 4) + e / 4)[e % 4]};
+                    finish<T, 1, ROWS_A && ROWS_B>(g, i, j + e, one);
+                }
+            }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
 // The slices' partial sums, added in slice order, and the epilogue.
-template <class T, int RUN>
+template <class T, int RUN, bool FORWARD>
 __global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
     const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * RUN;
     const int64_t plane = g.ni * g.nj;
@@ -434,7 +492,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
 #pragma unroll
                 for (int e = 0; e < RUN; e++) v[e] += q[u].v[e];
     }
-    finish<T, RUN>(g, k / g.nj, k % g.nj, v);
+    finish<T, RUN, FORWARD>(g, k / g.nj, k % g.nj, v);
 }
 
 // ---- the activation's gradient and column sums ----------------------------------------------------------------------------------
@@ -598,15 +656,10 @@ Shape shape_of(int dtype, int64_t ni, int64_t nj, int64_t np) {
 }
 
 template <class T, int BI, int WI, int WJ, bool RA, bool RB>
-void launch_gemm(const Gemm& g, bool direct, bool runs, hipStream_t stream) {
+void launch_gemm(const Gemm& g, bool direct, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices)), block(WI * WJ * 64);
-    if (direct) {
-        if (runs) hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, true, 4>), grid, block, 0, stream, g);
-        else hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, true, 1>), grid, block, 0, stream, g);
-    } else {
-        if (runs) hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, false, 4>), grid, block, 0, stream, g);
-        else hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, false, 1>), grid, block, 0, stream, g);
-    }
+    if (direct) hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, true>), grid, block, 0, stream, g);
+    else hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, false>), grid, block, 0, stream, g);
 }
 
 template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
@@ -618,21 +671,21 @@ template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStr
     SG_REQUIRE((g.lda + 1) * ES * 256 < (int64_t)kOutside && (g.ldb + 1) * ES * 256 < (int64_t)kOutside, SG_ERR_UNSUPPORTED,
                "%s: rows of %lld / %lld elements are too long", what, (long long)g.lda, (long long)g.ldb);
     const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && (RA ? g.np : g.ni) % E == 0 && (RB ? g.np : g.nj) % E == 0;
-    const bool runs = runs_aligned<T>(g, 4);
+    g.whole = runs_aligned<T>(g);
     if constexpr (ES == 2) {
-        if (s.bi == 256) launch_gemm<T, 256, 2, 4, RA, RB>(g, direct, runs, stream);
-        else if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, runs, stream);
-        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, runs, stream);
+        if (s.bi == 256) launch_gemm<T, 256, 2, 4, RA, RB>(g, direct, stream);
+        else if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, stream);
+        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, stream);
     } else {
-        if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, runs, stream);
-        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, runs, stream);
+        if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, stream);
+        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, stream);
     }
     if (g.slices > 1) {
-        const int run = runs ? 4 : 1;
+        const int run = g.whole ? 4 : 1;
         const int64_t blocks = (g.ni * g.nj / run + 255) / 256;
         SG_REQUIRE(blocks <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
-        if (runs) hipLaunchKernelGGL((linear_join_kernel<T, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
-        else hipLaunchKernelGGL((linear_join_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+        if (g.whole) hipLaunchKernelGGL((linear_join_kernel<T, 4, RA && RB>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+        else hipLaunchKernelGGL((linear_join_kernel<T, 1, RA && RB>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
     }
     return check_launch(what);
 }
@@ -706,7 +759,6 @@ extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* 
     g.ni = p->m; g.nj = p->n; g.np = p->k;
     g.partial = (float*)workspace;
     g.out = y; g.scale = p->w_gain;
-    g.with_epilogue = 1;
     g.bias = p->b; g.b_gain = p->b_gain;
     g.residual = p->residual; g.ldr = p->ldr;
     g.z = z; g.positive = positive;
