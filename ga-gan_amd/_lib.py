@@ -5,6 +5,7 @@ The shared library is built in-tree by `python -m ga_gan_amd.build` (or
 an ImportError, a failing call is a RuntimeError carrying `sg_last_error()`.
 """
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -127,6 +128,27 @@ def lib():
     return _lib
 
 
+TORCH_PATH = os.path.join(_HERE, '_sg_torch.so')
+_ext = None
+
+
+def ext():
+    """The PyTorch side of the operators that are called from C++ (csrc/sg_torch.cpp), bound to the same library."""
+    global _ext
+    if _ext is None:
+        lib()
+        if not os.path.isfile(TORCH_PATH):
+            raise ImportError(f'{TORCH_PATH} is missing: build it first (python -m ga_gan_amd.build)')
+        spec = importlib.util.spec_from_file_location('_sg_torch', TORCH_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(LIB_PATH)
+        if _profile is not None:
+            module.record(_record)
+        _ext = module
+    return _ext
+
+
 def check(rc, what):
     if rc != 0:
         raise RuntimeError(f'{what} failed ({rc}): {lib().sg_last_error().decode()}')
@@ -157,6 +179,17 @@ def profile_begin():
     The events are recorded on the stream the kernel is enqueued on."""
     global _profile
     _profile = []
+    if _ext is not None:
+        _ext.record(_record)
+
+
+def _record(label, nbytes, flops, call):
+    """A launch from C++, on the current stream of the current device, as an entry of the recording."""
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    call()
+    end.record()
+    _profile.append((label, nbytes, start, end, flops))
 
 
 def profiling():
@@ -168,6 +201,8 @@ def profile_end():
     """Stop recording; returns [(label, bytes, milliseconds, flops)] after synchronising."""
     global _profile
     records, _profile = _profile or [], None
+    if _ext is not None:
+        _ext.record(None)
     torch.cuda.synchronize()
     return [(label, nbytes, start.elapsed_time(end), flops) for label, nbytes, start, end, flops in records]
 

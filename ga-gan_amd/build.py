@@ -1,7 +1,7 @@
 """Build the HIP library in-tree:  python -m ga_gan_amd.build  (hipcc, gfx950 only).
 
 Every csrc/*.hip is compiled to an object of its own (in parallel) and the objects are linked into
-libsgops.so.  Staleness is decided by content, not by time stamps: each object carries a stamp with the
+libsgops.so; csrc/sg_torch.cpp (host code: the operators' PyTorch side) is compiled into _sg_torch.so.  Staleness is decided by content, not by time stamps: each object carries a stamp with the
 digest of its source, of every header and of the compiler flags, the way the reference keys its plugin build
 directory by a digest of the op's sources (torch_utils/custom_ops.py:88-104).  The whole build runs under an
 exclusive file lock, so that several ranks importing a stale tree at once build it once and the others wait
@@ -18,6 +18,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 OUT = os.path.join(HERE, 'libsgops.so')
+TORCH_OUT = os.path.join(HERE, '_sg_torch.so')
+TORCH_SRC = os.path.join(HERE, 'csrc', 'sg_torch.cpp')
 OBJ_DIR = os.path.join(HERE, 'build')
 # Without packed float32 arithmetic: the compiler forms v_pk_{add,mul,fma}_f32 from ordinary scalar code, and some of their operand
 # forms have given wrong results on MI355X now and then.  (The host pass warns that it does not know the feature.)
@@ -63,9 +65,26 @@ def _plan():
     return items, hashlib.md5(''.join(i[3] for i in items).encode()).hexdigest()
 
 
+def _torch_plan():
+    """(compiler command, wanted digest) of the PyTorch side."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    flags = ['-O2', '-std=c++17', '-fPIC', '-shared', '-Wall', '-Wno-unknown-pragmas', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+             f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}']
+    include = [os.path.join(ROOT, 'include'), *cpp_extension.include_paths(), '/opt/rocm/include', sysconfig.get_paths()['include']]
+    # (torch's headers as system headers: their warnings are not this file's)
+    cmd = [os.environ.get('CXX', 'g++'), *flags, *[a for d in include for a in (('-I' if d.startswith(ROOT) else '-isystem'), d)], TORCH_SRC,
+           '-L', lib, '-ltorch', '-ltorch_cpu', '-ltorch_python', '-ltorch_hip', '-lc10', '-lc10_hip', '-ldl']
+    return cmd, _digest([TORCH_SRC] + headers(), ' '.join(flags) + torch.__version__)
+
+
 def is_stale():
     _, want = _plan()
-    return not os.path.isfile(OUT) or _read(os.path.join(OBJ_DIR, 'libsgops.md5')) != want
+    _, torch_want = _torch_plan()
+    return (not os.path.isfile(OUT) or _read(os.path.join(OBJ_DIR, 'libsgops.md5')) != want
+            or not os.path.isfile(TORCH_OUT) or _read(os.path.join(OBJ_DIR, '_sg_torch.md5')) != torch_want)
 
 
 def build(force=False, verbose=True, jobs=None):
@@ -92,9 +111,26 @@ def build(force=False, verbose=True, jobs=None):
                 with open(stamp, 'w') as f:
                     f.write(digest)
 
-            jobs = jobs or min(len(todo) or 1, int(os.environ.get('MAX_JOBS', 0)) or os.cpu_count() or 1, 16)
+            torch_cmd, torch_want = _torch_plan()
+            torch_stamp = os.path.join(OBJ_DIR, '_sg_torch.md5')
+
+            def compile_torch():
+                if not force and os.path.isfile(TORCH_OUT) and _read(torch_stamp) == torch_want:
+                    return
+                tmp = TORCH_OUT + f'.tmp{os.getpid()}'
+                cmd = [*torch_cmd, '-o', tmp]
+                if verbose:
+                    print(' '.join(cmd), flush=True)
+                subprocess.run(cmd, check=True)
+                os.replace(tmp, TORCH_OUT)
+                with open(torch_stamp, 'w') as f:
+                    f.write(torch_want)
+
+            jobs = jobs or min(len(todo) + 1, int(os.environ.get('MAX_JOBS', 0)) or os.cpu_count() or 1, 16)
             with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
+                glue = pool.submit(compile_torch)
                 list(pool.map(compile_one, todo))
+                glue.result()
             tmp = OUT + f'.tmp{os.getpid()}'
             cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', *[i[1] for i in items], '-o', tmp]
             if verbose:

@@ -41,64 +41,7 @@ def _check(t, what):
         raise RuntimeError(f'{what} must be a dense float32 tensor')
 
 
-class GradList(ctypes.Structure):
-    _fields_ = [('grads', ctypes.c_void_p), ('numel', ctypes.c_void_p), ('dtype', ctypes.c_void_p), ('count', ctypes.c_int32)]
-
-
-class AdamList(ctypes.Structure):
-    _fields_ = [('param', ctypes.c_void_p), ('grad', ctypes.c_void_p), ('exp_avg', ctypes.c_void_p), ('exp_avg_sq', ctypes.c_void_p),
-                ('numel', ctypes.c_void_p), ('step', ctypes.c_void_p), ('count', ctypes.c_int32), ('lr', ctypes.c_float),
-                ('beta1', ctypes.c_float), ('beta2', ctypes.c_float), ('eps', ctypes.c_float), ('grad_limit', ctypes.c_float),
-                ('grad_scale', ctypes.c_void_p)]
-
-
-_NORM_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 CLIP_EPS = 1e-6        # added to the norm a gradient is divided by, as torch.nn.utils.clip_grad_norm_ does
-
-
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
-
-
-def _distinct(pointers, numels, what):
-    used = [p for p, n in zip(pointers, numels) if n]
-    if len(set(used)) != len(used):
-        raise RuntimeError(f'{what}: a tensor appears twice')
-
-
-class _Grads:
-    """Host arrays of a list of gradients (kept alive while the library reads them)."""
-
-    def __init__(self, grads, what):
-        self.device = grads[0].device
-        codes = []
-        for g in grads:
-            code = _NORM_DTYPES.get(g.dtype)
-            if code is None:
-                raise RuntimeError(f'{what}: unsupported dtype {g.dtype}')
-            if not g.is_cuda or g.device != self.device:
-                raise RuntimeError(f'{what}: gradients must reside on one CUDA device')
-            if not g.is_contiguous():
-                raise RuntimeError(f'{what}: gradients must be dense')
-            codes.append(code)
-        count = len(grads)
-        self.tensors = grads
-        self.pointers = _pointers(grads)
-        self.numels = [g.numel() for g in grads]
-        self.numel = (ctypes.c_int64 * count)(*self.numels)
-        self.dtype = (ctypes.c_int32 * count)(*codes)
-        self.args = GradList(ctypes.cast(self.pointers, ctypes.c_void_p), ctypes.cast(self.numel, ctypes.c_void_p),
-                             ctypes.cast(self.dtype, ctypes.c_void_p), count)
-
-    def norm(self, grad_limit, max_norm):
-        """float32 [2] on the device: the norm, and min(1, max_norm / (norm + 1e-6))."""
-        handle = _lib.lib()
-        need = handle.sg_grad_norm_workspace_bytes(ctypes.byref(self.args))
-        out = torch.empty([2], dtype=torch.float32, device=self.device)
-        work = torch.empty([max(need, 8)], dtype=torch.uint8, device=self.device)
-        _lib.launch_raw(lambda stream: handle.sg_grad_norm(ctypes.byref(self.args), grad_limit, max_norm, CLIP_EPS, _lib.ptr(out), _lib.ptr(work),
-                                                           need, stream), out, 'sg_grad_norm', 'grad_norm_kernel', _lib.nbytes(*self.tensors))
-        return out
 
 
 def _max_norm(value, what):
@@ -118,7 +61,7 @@ def grad_norm(grads, grad_limit=None):
         return torch.zeros([])
     if grad_limit is not None and not float(grad_limit) > 0:
         raise RuntimeError('grad_norm: grad_limit must be positive')
-    return _Grads(grads, 'grad_norm').norm(float(grad_limit or 0), 0.0)[0]
+    return _lib.ext().grad_norm(grads, float(grad_limit or 0), 0.0, CLIP_EPS)[0]
 
 
 @torch.no_grad()
@@ -137,40 +80,7 @@ def clip_grad_norm_(parameters, max_norm):
     for p in params:
         if not p.grad.is_contiguous():
             p.grad = p.grad.contiguous()
-    grads = _Grads([p.grad for p in params], 'clip_grad_norm_')
-    _distinct(grads.pointers, grads.numels, 'clip_grad_norm_')
-    out = grads.norm(0.0, max_norm)
-    handle = _lib.lib()
-    _lib.launch_raw(lambda stream: handle.sg_scale_grads(ctypes.byref(grads.args), ctypes.c_void_p(out.data_ptr() + 4), stream), out, 'sg_scale_grads',
-                    'grad_scale_kernel', 2 * _lib.nbytes(*grads.tensors))
-    torch.autograd.graph.increment_version(grads.tensors)
-    return out[0]
-
-
-def _check_list(lists, device):
-    params = lists[0][1]
-    for what, tensors in lists:
-        for t, p in zip(tensors, params):
-            if not (t.is_cuda and t.dtype is torch.float32 and t.is_contiguous() and t.device == device) or t.shape != p.shape:
-                _check(t, what)
-                raise RuntimeError(f'adam_step: {what} {tuple(t.shape)} on {t.device} does not match its parameter {tuple(p.shape)} on {device}')
-
-
-def _adam_step_scaled(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, scale):
-    """The update with gradients scaled by the device value `scale` (float32, one element) as they are read."""
-    count = len(params)
-    device = scale.device
-    lists = (('param', params), ('grad', grads), ('exp_avg', exp_avgs), ('exp_avg_sq', exp_avg_sqs))
-    _check_list(lists, device)
-    arrays = [_pointers(tensors) for _, tensors in lists]
-    numels = [p.numel() for p in params]
-    _distinct([p for a in arrays for p in a], numels * 4, 'adam_step')
-    numel = (ctypes.c_int64 * count)(*numels)
-    step = (ctypes.c_int32 * count)(*[int(k) for k in steps])
-    args = AdamList(*[ctypes.cast(a, ctypes.c_void_p) for a in arrays], ctypes.cast(numel, ctypes.c_void_p), ctypes.cast(step, ctypes.c_void_p),
-                    count, lr, beta1, beta2, eps, grad_limit, scale.data_ptr())
-    _lib.launch('sg_adam_step_list', args, scale, 'adam_kernel', 32 * sum(numels))
-    torch.autograd.graph.increment_version(list(params) + list(grads) + list(exp_avgs) + list(exp_avg_sqs))
+    return _lib.ext().clip_grads([p.grad for p in params], max_norm, CLIP_EPS)
 
 
 def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit=1e5, max_grad_norm=None):
@@ -186,10 +96,7 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps
             return torch.zeros([])
         if not grad_limit > 0:
             raise RuntimeError('adam_step: grad_limit must be positive')
-        _check_list((('param', params), ('grad', grads)), params[0].device)
-        out = _Grads(list(grads), 'adam_step').norm(grad_limit, max_grad_norm)
-        _adam_step_scaled(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, out[1:])
-        return out[0]
+        return _lib.ext().adam_step_clipped(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, max_grad_norm, CLIP_EPS)
     for i in range(0, len(params), MAX_TENSORS):
         chunk = range(i, min(i + MAX_TENSORS, len(params)))
         table = (AdamTensor * len(chunk))()
@@ -290,8 +197,9 @@ class FusedAdam(torch.optim.Optimizer):
         elif work:
             if len({group['grad_limit'] for group, _ in work}) > 1:
                 raise RuntimeError('FusedAdam: parameter groups that are clipped together must share grad_limit')
-            out = _Grads([g for _, lists in work for g in lists[1]], 'FusedAdam').norm(work[0][0]['grad_limit'], self.max_grad_norm)
+            ext = _lib.ext()
+            out = ext.grad_norm([g for _, lists in work for g in lists[1]], work[0][0]['grad_limit'], self.max_grad_norm, CLIP_EPS)
             for group, lists in work:
-                _adam_step_scaled(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], out[1:])
+                ext.adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], out[1:])
             self.last_grad_norm = out[0]
         return loss
