@@ -102,4 +102,13 @@ __host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_c
         default: return ::sg::fail(SG_ERR_INVALID_ARGUMENT, "unknown dtype %d", (int)(dtype)); \
     }
 
+// The same for kernels without a float64 form (none is instantiated).
+#define SG_DISPATCH_16_32(dtype, ...)                                              \
+    switch (dtype) {                                                               \
+        case SG_F32: { using T = float; __VA_ARGS__; break; }                      \
+        case SG_F16: { using T = __half; __VA_ARGS__; break; }                     \
+        case SG_BF16: { using T = __hip_bfloat16; __VA_ARGS__; break; }            \
+        default: return ::sg::fail(SG_ERR_UNSUPPORTED, "dtype %d is not supported here", (int)(dtype)); \
+    }
+
 }  // namespace sg

@@ -559,7 +559,7 @@ extern "C" int sg_embedding(const sg_embedding_params* p, void* y, sg_stream_t s
     int64_t blocks = (items + 256 * kFwdUnroll - 1) / (256 * kFwdUnroll);
     if (items <= 256 * 256 * kFwdUnroll) blocks = (items + 255) / 256;                // few items: one per lane, on as many CUs as there are
     if (blocks > 1 << 20) blocks = 1 << 20;
-    SG_DISPATCH_DTYPE(p->dtype, false, {
+    SG_DISPATCH_16_32(p->dtype, {
         if (packed) hipLaunchKernelGGL((embedding_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, e);
         else hipLaunchKernelGGL((embedding_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, e);
     });
@@ -597,7 +597,7 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
         const int64_t tiles_v = (p->v + kOwnTile - 1) / kOwnTile, tiles_f = (p->f + kOwnTile - 1) / kOwnTile;
         SG_REQUIRE((tiles_v + 1) * tiles_f <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "embedding_backward: table too large");
         const GradParams q{index, dy, dtable, dbias, p->tokens, p->v, p->f, p->stride_v, p->stride_f, p->w_gain, p->b_gain, rows ? 1 : 0};
-        SG_DISPATCH_DTYPE(p->dtype, false,
+        SG_DISPATCH_16_32(p->dtype,
             hipLaunchKernelGGL((embedding_grad_owner_kernel<T>), dim3((unsigned)((tiles_v + (dbias ? 1 : 0)) * tiles_f)), dim3(256), 0, stream, q,
                                (int)tiles_v, (int)tiles_f));
         return check_launch("sg_embedding_backward");
@@ -637,7 +637,7 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
     const int64_t items = (int64_t)g.spans * tiles;
     const int tiles64 = (int)((p->f + 63) / 64);
     SG_REQUIRE((items + 3) / 4 <= INT32_MAX && (int64_t)g.spans * tiles64 <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "embedding_backward: too many elements");
-    SG_DISPATCH_DTYPE(p->dtype, false, {
+    SG_DISPATCH_16_32(p->dtype, {
         if (packed) hipLaunchKernelGGL((embedding_grad_runs_kernel<T, Pack<T>::N>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
         else hipLaunchKernelGGL((embedding_grad_runs_kernel<T, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
         hipLaunchKernelGGL((embedding_grad_join_kernel<T>), dim3((unsigned)(g.spans * tiles64)), dim3(512), 0, stream, r, tiles64);

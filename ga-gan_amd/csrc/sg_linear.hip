@@ -13,6 +13,8 @@
 #include "sg_common.h"
 #include "sg_column_sums.h"
 
+#include <type_traits>
+
 namespace sg {
 namespace {
 
@@ -142,77 +144,75 @@ __device__ __forceinline__ i32x4_t descriptor(const void* p) {
     return i32x4_t{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), (int)kOutside, 0x00020000};
 }
 
-// 16 bytes per lane from `offset` behind the descriptor's address to LDS at lds + 16 * lane; zeros for kOutside.  Written as
+// 16 bytes per lane from `offset + more` behind the descriptor's address to LDS at lds + 16 * lane; zeros for kOutside.  Written as
 // assembly because of its wait: the compiler holds every LDS read behind all copies into LDS that came before it, those into
 // the other buffer included.  copies_landed() is the wait, and the kernel places it.
-__device__ __forceinline__ void copy_to_lds(i32x4_t from, unsigned offset, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "m0");
+__device__ __forceinline__ void copy_to_lds(i32x4_t from, unsigned offset, unsigned more, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(from), "s"(more) : "m0");
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
-// One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: SIDE * 8 slots of 16 bytes.
+// One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: SIDE * 8 slots of 16 bytes, slot k * THREADS + t filled by
+// thread t.
 //   ROWS:  slot (row, c) holds the 16 bytes c ^ ((row >> 1) & 7) of the row: 16 lanes reading one column of 16 rows hit 16
 //          different 16-byte banks.
-//   !ROWS: the tile is [p][side]; 16-bit: the 32-byte block c of line p holds block c ^ swizzle(p), so that the transposing
-//          read of 16 lines hits each 32-byte bank twice, once per half wave; float32: as it lies.
+//   !ROWS: lines of SIDE elements at one p.  16-bit: the 32-byte block c of line q holds block c ^ swizzle(q), so that the
+//          transposing read of 16 lines hits each 32-byte bank twice, once per half wave; float32: as it lies.  Line q holds
+//          p = p_of(q): where a thread fills every 8th line (256 columns), bits 2 and 3 trade places, so that a thread's slots
+//          share one swizzle.
+// Either way a thread's slots are one address and constant distances apart.
 template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
     static constexpr int ES = sizeof(T), E = 16 / ES, BK = kStepBytes / ES;
     static constexpr int BYTES = SIDE * kStepBytes;
     static constexpr int LOADS = SIDE * 8 / THREADS;               // 16-byte slots per thread
-    static constexpr int LINE = SIDE / E;                          // !ROWS: slots per line
+    static constexpr int LINE = ROWS ? 8 : SIDE / E;               // slots per row or line
+    static constexpr int APART = THREADS / LINE;                   // rows or lines from one slot of a thread to its next
+    static constexpr bool SWAP = !ROWS && ES == 2 && APART == 8;
     static_assert(LOADS >= 1 && LOADS * THREADS == SIDE * 8, "slots divide among the threads");
+    static_assert(ROWS ? APART % 16 == 0 : ES == 4 || APART % 16 == 0 || SWAP, "a thread's slots share one swizzle");
 
-    static __device__ __forceinline__ int swizzle(int p) {
+    static __device__ __forceinline__ constexpr int p_of(int q) { return SWAP ? (q & ~12) | (q & 4) << 1 | (q & 8) >> 1 : q; }
+    static __device__ __forceinline__ int swizzle(int q) {
         if (ES == 4) return 0;
-        return SIDE >= 128 ? (p & 3) | ((p >> 3) & 1) << 2 : ((p >> 1) & 1) | ((p >> 3) & 1) << 1;
+        if (SWAP) return q & 7;
+        return SIDE >= 128 ? (q & 3) | ((q >> 3) & 1) << 2 : ((q >> 1) & 1) | ((q >> 3) & 1) << 1;
     }
-    // slot -> (side, p) of its first element within the tile
-    static __device__ __forceinline__ void where(int slot, int& side, int& p) {
+    // the slots of a thread: its first one as (side, p) within the tile
+    struct Slots { int side, p; unsigned off; };
+    static __device__ __forceinline__ Slots plan(int64_t ld) {
+        Slots s;
+        const int line = threadIdx.x / LINE, c = threadIdx.x % LINE;
         if (ROWS) {
-            side = slot >> 3;
-            p = ((slot & 7) ^ ((side >> 1) & 7)) * E;
+            s.side = line;
+            s.p = (c ^ ((line >> 1) & 7)) * E;
         } else {
-            p = slot / LINE;
-            side = ((slot % LINE) ^ (swizzle(p) << 1)) * E;
+            s.p = p_of(line);
+            s.side = (c ^ (swizzle(line) << 1)) * E;
         }
+        s.off = (unsigned)((ROWS ? s.side : s.p) * (unsigned)ld + (ROWS ? s.p : s.side)) * ES;
+        return s;
     }
-    // straight to LDS: per thread, the byte offsets of its slots within a step (kOutside where the row or column is)
-    struct Slots { unsigned off[LOADS]; };
-    static __device__ __forceinline__ void plan(Slots& s, int64_t ld, int64_t left_side) {
-#pragma unroll
-        for (int k = 0; k < LOADS; k++) {
-            int side, p;
-            where(k * THREADS + threadIdx.x, side, p);
-            s.off[k] = side < left_side ? (unsigned)((ROWS ? side : p) * (unsigned)ld + (ROWS ? p : side)) * ES : kOutside;
-        }
+    // distance of slot k from the first, along side (ROWS) or p (!ROWS)
+    static __device__ __forceinline__ constexpr int apart(int k) { return ROWS ? k * APART : p_of(k * APART); }
+    static __device__ __forceinline__ bool inside(const Slots& s, int k, int left_side, int left_p) {
+        return ROWS ? s.side < left_side - apart(k) && s.p < left_p : s.side < left_side && s.p < left_p - apart(k);
     }
-    // base: the tile's first element of this step; left_p: extent along p from there
-    static __device__ __forceinline__ void issue(const Slots& s, unsigned lds, const T* base, int64_t left_p) {
-        const i32x4_t from = descriptor(base);
+    // slot k straight to LDS.  from: the tile's first element of this step; left_*: extent from there (at most 2^30)
+    static __device__ __forceinline__ void copy(const Slots& s, int k, i32x4_t from, unsigned ld, unsigned lds, int left_side, int left_p) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-        for (int k = 0; k < LOADS; k++) {
-            unsigned off = s.off[k];
-            if (left_p < BK) {                                     // (the last step only)
-                int side, p;
-                where(k * THREADS + threadIdx.x, side, p);
-                off = p < left_p ? off : kOutside;
-            }
-            copy_to_lds(from, off, lds + (k * THREADS + wave * 64) * 16);
-        }
+        copy_to_lds(from, inside(s, k, left_side, left_p) ? s.off : kOutside, (unsigned)apart(k) * ld * ES, lds + (k * THREADS + wave * 64) * 16);
     }
     // by way of registers: any alignment, any extent
     struct Regs { uint4 v[LOADS]; };
-    static __device__ __forceinline__ void fetch(Regs& r, const T* base, int64_t ld, int64_t left_side, int64_t left_p) {
+    static __device__ __forceinline__ void fetch(Regs& r, const Slots& s, const T* base, int64_t ld, int left_side, int left_p) {
         struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[E]; };
+        const T* first = base + (ROWS ? s.side * ld + s.p : s.p * ld + s.side);
 #pragma unroll
         for (int k = 0; k < LOADS; k++) {
-            int side, p;
-            where(k * THREADS + threadIdx.x, side, p);
-            const T* src = base + (ROWS ? side * ld + p : p * ld + side);
-            const bool line = ROWS ? side < left_side : p < left_p;
-            const int64_t in_line = (ROWS ? left_p - p : left_side - side);
+            const T* src = first + apart(k) * ld;
+            const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
+            const int in_line = ROWS ? left_p - s.p : left_side - s.side;
             Pack<T> q;
             if (line && in_line >= E) {
                 const Loose l = *reinterpret_cast<const Loose*>(src);
@@ -232,7 +232,7 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
 };
 
 // Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for K-part kk (two per step: 32 16-bit or 16 float32 elements).
-template <class T, int SIDE, bool ROWS, int COUNT> struct Frags {
+template <class T, int SIDE, bool ROWS, int THREADS, int COUNT> struct Frags {
     static constexpr int V = sizeof(T) == 4 && !ROWS ? (COUNT >= 4 ? 4 : COUNT) : 1;   // tiles whose rows interleave
     uint4 q[COUNT];                                                                   // 8 16-bit values, or 4 float32 (ROWS)
     float f[sizeof(T) == 4 && !ROWS ? COUNT : 1][4];
@@ -240,32 +240,27 @@ template <class T, int SIDE, bool ROWS, int COUNT> struct Frags {
     // row within the wave's share of element `r16` (0 .. 15) of tile t
     static __device__ __forceinline__ int row(int t, int r16) { return (t / V) * 16 * V + r16 * V + t % V; }
 
-    __device__ __forceinline__ void read(const unsigned char* lds, int first, int kk) {
+    // tile t (with V > 1: tiles t .. t + V - 1, for t a multiple of V)
+    __device__ __forceinline__ void read(const unsigned char* lds, int first, int kk, int t) {
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
         if constexpr (ROWS) {
             const int at = (first + l16) * kStepBytes + (((kk * 4 + g) ^ ((l16 >> 1) & 7)) << 4);
-#pragma unroll
-            for (int t = 0; t < COUNT; t++) q[t] = *reinterpret_cast<const uint4*>(lds + at + t * 16 * kStepBytes);
+            q[t] = *reinterpret_cast<const uint4*>(lds + at + t * 16 * kStepBytes);
         } else if constexpr (sizeof(T) == 2) {
             constexpr int LINE = SIDE * 2;
-            const int p = kk * 32 + g * 8 + (l16 >> 2);
-            const int sw = Tile<T, SIDE, false, 64>::swizzle(p);             // (the same for p + 4)
-            const unsigned char* line = lds + p * LINE + (l16 & 3) * 8;
-#pragma unroll
-            for (int t = 0; t < COUNT; t++) {
-                const unsigned char* at = line + (((first >> 4) + t) ^ sw) * 32;
-                typedef __attribute__((address_space(3))) s16x4_t* Lds;
-                const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at);
-                const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 4 * LINE));
-                const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
-                q[t] = make_uint4(a.x, a.y, b.x, b.y);
-            }
+            using Lines = Tile<T, SIDE, false, THREADS>;
+            const int q0 = Lines::p_of(kk * 32 + g * 8 + (l16 >> 2));        // (its own inverse)
+            const unsigned char* at = lds + q0 * LINE + (l16 & 3) * 8 + (((first >> 4) + t) ^ Lines::swizzle(q0)) * 32;
+            typedef __attribute__((address_space(3))) s16x4_t* Lds;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at);
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + Lines::p_of(4) * LINE));
+            const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+            q[t] = make_uint4(a.x, a.y, b.x, b.y);
         } else {
             constexpr int LINE = SIDE * 4;
+            if (t % V == 0)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int t = 0; t < COUNT; t += V) {
+                for (int e = 0; e < 4; e++) {
                     const unsigned char* at = lds + (kk * 16 + g * 4 + e) * LINE + (first + t * 16 + l16 * V) * 4;
                     if constexpr (V == 4) {
                         const f32x4_t v = *reinterpret_cast<const f32x4_t*>(at);
@@ -278,6 +273,10 @@ template <class T, int SIDE, bool ROWS, int COUNT> struct Frags {
                     }
                 }
         }
+    }
+    __device__ __forceinline__ void read(const unsigned char* lds, int first, int kk) {
+#pragma unroll
+        for (int t = 0; t < COUNT; t++) read(lds, first, kk, t);
     }
     __device__ __forceinline__ float value(int t, int e) const {
         if constexpr (ROWS) return __builtin_bit_cast(f32x4_t, q[t])[e];
@@ -299,8 +298,8 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
     using TileA = Tile<T, BI, ROWS_A, THREADS>;
     using TileB = Tile<T, BJ, ROWS_B, THREADS>;
-    using FragA = Frags<T, BI, ROWS_A, TI>;
-    using FragB = Frags<T, BJ, ROWS_B, TJ>;
+    using FragA = Frags<T, BI, ROWS_A, THREADS, TI>;
+    using FragB = Frags<T, BJ, ROWS_B, THREADS, TJ>;
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * (TileA::BYTES + TileB::BYTES)];
     constexpr int BUF = TileA::BYTES + TileB::BYTES;
 
@@ -319,7 +318,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
 
     const T* a = (const T*)g.a + (ROWS_A ? i0 * g.lda : i0);
     const T* b = (const T*)g.b + (ROWS_B ? j0 * g.ldb : j0);
-    const int64_t left_i = g.ni - i0, left_j = g.nj - j0;
+    const int left_i = (int)min(g.ni - i0, (int64_t)BI), left_j = (int)min(g.nj - j0, (int64_t)BJ);
     const int steps_all = (int)((g.np + BK - 1) / BK);
     const int first = (int)slice * g.slice_steps;
     const int steps = min(g.slice_steps, steps_all - first);
@@ -332,56 +331,106 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
 #pragma unroll
         for (int s = 0; s < TI; s++) acc[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+    auto left_p = [&](int step) { return (int)min(g.np - (int64_t)step * BK, (int64_t)BK); };
+    const typename TileA::Slots sa = TileA::plan(g.lda);
+    const typename TileB::Slots sb = TileB::plan(g.ldb);
     auto at_a = [&](int step) { return a + (ROWS_A ? (int64_t)step * BK : (int64_t)step * BK * g.lda); };
     auto at_b = [&](int step) { return b + (ROWS_B ? (int64_t)step * BK : (int64_t)step * BK * g.ldb); };
-    auto multiply = [&](const unsigned char* lds) {
+    // column tile t of the wave's part
+    auto multiply_tile = [&](const FragA& fa, const FragB& fb, int t) {
 #pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            FragA fa;
-            FragB fb;
-            fa.read(lds, wi, kk);
-            fb.read(lds + TileA::BYTES, wj, kk);
+        for (int s = 0; s < TI; s++) {
+            if constexpr (sizeof(T) == 2) {
+                acc[t][s] = mfma(fb.q[t], fa.q[s], acc[t][s], T());
+            } else {
 #pragma unroll
-            for (int t = 0; t < TJ; t++)
-#pragma unroll
-                for (int s = 0; s < TI; s++) {
-                    if constexpr (sizeof(T) == 2) {
-                        acc[t][s] = mfma(fb.q[t], fa.q[s], acc[t][s], T());
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb.value(t, e), fa.value(s, e), acc[t][s], 0, 0, 0);
-                    }
-                }
+                for (int e = 0; e < 4; e++) acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb.value(t, e), fa.value(s, e), acc[t][s], 0, 0, 0);
+            }
         }
     };
-    // Two LDS buffers: the loads of step n + 1 are under way while step n multiplies; one barrier a step (after it every wave has
-    // read the buffer that is filled next, and every wave's loads into the one that is read next have landed).
     if constexpr (DIRECT) {
-        typename TileA::Slots sa;
-        typename TileB::Slots sb;
-        TileA::plan(sa, g.lda, left_i);
-        TileB::plan(sb, g.ldb, left_j);
+        // Two LDS buffers and two sets of fragments.  A step is two halves: the first multiplies the fragments of its first
+        // K-part while those of the second are read; then, behind the one barrier of a step, the second is multiplied while the
+        // first fragments of the next step are read and the copies of the step after it start into the buffer that has just
+        // been read for the last time.  So the matrix unit has operands in registers at the barrier, and a copy has a whole
+        // step to land.
         const unsigned lds = lds_address(smem);
-        auto issue = [&](int n) {
-            const int step = first + n;
-            TileA::issue(sa, lds + (n & 1) * BUF, at_a(step), g.np - (int64_t)step * BK);
-            TileB::issue(sb, lds + (n & 1) * BUF + TileA::BYTES, at_b(step), g.np - (int64_t)step * BK);
+        constexpr int PARTS = TI > TJ ? TI : TJ;
+        FragA fa[2];
+        FragB fb[2];
+        // share `part` of PARTS of the copies of step n
+        auto copy_part = [&](i32x4_t from_a, i32x4_t from_b, int n, int part) {
+            const int left = left_p(first + n);
+            const unsigned to = lds + (n & 1) * BUF;
+#pragma unroll
+            for (int k = 0; k < TileA::LOADS; k++)
+                if (k * PARTS / TileA::LOADS == part) TileA::copy(sa, k, from_a, (unsigned)g.lda, to, left_i, left);
+#pragma unroll
+            for (int k = 0; k < TileB::LOADS; k++)
+                if (k * PARTS / TileB::LOADS == part) TileB::copy(sb, k, from_b, (unsigned)g.ldb, to + TileA::BYTES, left_j, left);
         };
-        if (steps > 0) issue(0);
-        for (int n = 0; n < steps; n++) {
+        auto copy_all = [&](int n) {
+            const i32x4_t from_a = descriptor(at_a(first + n)), from_b = descriptor(at_b(first + n));
+#pragma unroll
+            for (int part = 0; part < PARTS; part++) copy_part(from_a, from_b, n, part);
+        };
+        // share `part` of the reads of a half: spread over its first three quarters, so that the last of them are back in time
+        constexpr int READ_PARTS = PARTS >= 4 ? PARTS * 3 / 4 : PARTS;
+        auto read_part = [&](int set, const unsigned char* from, int kk, int part) {
+#pragma unroll
+            for (int t = 0; t < TI; t++)
+                if (t * READ_PARTS / TI == part) fa[set].read(from, wi, kk, t);
+#pragma unroll
+            for (int t = 0; t < TJ; t++)
+                if (t * READ_PARTS / TJ == part) fb[set].read(from + TileA::BYTES, wj, kk, t);
+        };
+        auto step = [&](int n, auto copies, auto more) {           // copies: step n + 2 exists; more: step n + 1 does
+            const unsigned char* now = smem + (n & 1) * BUF;
+            const unsigned char* next = smem + (~n & 1) * BUF;
+#pragma unroll
+            for (int t = 0; t < PARTS; t++) {
+                read_part(1, now, 1, t);
+                if (t < TJ) multiply_tile(fa[0], fb[0], t);
+                __builtin_amdgcn_sched_barrier(0);        // (or the reads gather behind the products)
+            }
+            if constexpr (more) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            i32x4_t from_a{}, from_b{};
+            if constexpr (copies) {
+                from_a = descriptor(at_a(first + n + 2));
+                from_b = descriptor(at_b(first + n + 2));
+            }
+#pragma unroll
+            for (int t = 0; t < PARTS; t++) {
+                if constexpr (copies) copy_part(from_a, from_b, n + 2, t);
+                if constexpr (more) read_part(0, next, 0, t);
+                if (t < TJ) multiply_tile(fa[1], fb[1], t);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        constexpr auto yes = std::true_type{};
+        constexpr auto no = std::false_type{};
+        if (steps > 0) {
+            copy_all(0);
             copies_landed();
             __syncthreads();
-            if (n + 1 < steps) issue(n + 1);
-            multiply(smem + (n & 1) * BUF);
+            if (steps > 1) copy_all(1);
+            fa[0].read(smem, wi, 0);
+            fb[0].read(smem + TileA::BYTES, wj, 0);
+            int n = 0;
+            for (; n + 2 < steps; n++) step(n, yes, yes);
+            if (n + 1 < steps) step(n++, no, yes);
+            step(n, no, no);
         }
     } else {
+        // Two LDS buffers: the loads of step n + 1 are under way while step n multiplies; one barrier a step.
         typename TileA::Regs ra;
         typename TileB::Regs rb;
         auto fetch = [&](int n) {
             const int step = first + n;
-            TileA::fetch(ra, at_a(step), g.lda, left_i, g.np - (int64_t)step * BK);
-            TileB::fetch(rb, at_b(step), g.ldb, left_j, g.np - (int64_t)step * BK);
+            TileA::fetch(ra, sa, at_a(step), g.lda, left_i, left_p(step));
+            TileB::fetch(rb, sb, at_b(step), g.ldb, left_j, left_p(step));
         };
         auto commit = [&](int buf) {
             TileA::commit(smem + buf * BUF, ra);
@@ -394,7 +443,15 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         for (int n = 0; n < steps; n++) {
             __syncthreads();
             if (n + 1 < steps) fetch(n + 1);
-            multiply(smem + (n & 1) * BUF);
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                FragA fa;
+                FragB fb;
+                fa.read(smem + (n & 1) * BUF, wi, kk);
+                fb.read(smem + (n & 1) * BUF + TileA::BYTES, wj, kk);
+#pragma unroll
+                for (int t = 0; t < TJ; t++) multiply_tile(fa, fb, t);
+            }
             if (n + 1 < steps) commit((n + 1) & 1);
         }
     }
@@ -673,7 +730,7 @@ template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStr
     const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && (RA ? g.np : g.ni) % E == 0 && (RB ? g.np : g.nj) % E == 0;
     g.whole = runs_aligned<T>(g);
     if constexpr (ES == 2) {
-        if (s.bi == 256) launch_gemm<T, 256, 2, 4, RA, RB>(g, direct, stream);
+        if (s.bi == 256) launch_gemm<T, 256, 2, 2, RA, RB>(g, direct, stream);
         else if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, stream);
         else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, stream);
     } else {
@@ -732,7 +789,7 @@ int column_sums(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ld
     SlopeParams p{};
     p.dy = g; p.partial = (float*)workspace; p.sums = out;
     p.rows = rows; p.cols = cols; p.ld = ld; p.scale = scale;
-    SG_DISPATCH_DTYPE(dtype, false, return run_slope<T>(p, stream, "column sums"));
+    SG_DISPATCH_16_32(dtype, return run_slope<T>(p, stream, "column sums"));
     return SG_OK;
 }
 
@@ -763,7 +820,7 @@ extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* 
     g.residual = p->residual; g.ldr = p->ldr;
     g.z = z; g.positive = positive;
     g.act = p->act; g.alpha = p->alpha; g.gain = p->gain;
-    SG_DISPATCH_DTYPE(p->dtype, false, return (run_gemm<T, true, true>(g, s, (hipStream_t)stream, "sg_linear")));
+    SG_DISPATCH_16_32(p->dtype, return (run_gemm<T, true, true>(g, s, (hipStream_t)stream, "sg_linear")));
     return SG_OK;
 }
 
@@ -804,7 +861,7 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         q.sign = p->gain < 0.f ? -1.f : 1.f;
         q.scale = p->gain * p->b_gain;
         int done = SG_OK;
-        SG_DISPATCH_DTYPE(p->dtype, false, done = run_slope<T>(q, stream, "sg_linear_backward"));
+        SG_DISPATCH_16_32(p->dtype, done = run_slope<T>(q, stream, "sg_linear_backward"));
         if (done != SG_OK) return done;
     }
     Gemm g{};
@@ -816,7 +873,7 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         q.ni = p->m; q.nj = p->k; q.np = p->n;
         q.out = dx;
         int done = SG_OK;
-        SG_DISPATCH_DTYPE(p->dtype, false, done = (run_gemm<T, true, false>(q, plan.x, stream, "sg_linear_backward")));
+        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, true, false>(q, plan.x, stream, "sg_linear_backward")));
         if (done != SG_OK) return done;
     }
     if (dw) {                            // [n, k] = s [m, n]^T x [m, k]
@@ -825,7 +882,7 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         q.ni = p->n; q.nj = p->k; q.np = p->m;
         q.out = dw;
         int done = SG_OK;
-        SG_DISPATCH_DTYPE(p->dtype, false, done = (run_gemm<T, false, false>(q, plan.w, stream, "sg_linear_backward")));
+        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, false, false>(q, plan.w, stream, "sg_linear_backward")));
         if (done != SG_OK) return done;
     }
     return SG_OK;
