@@ -32,23 +32,44 @@ constexpr unsigned kOutside = 0x80000000u;         // a buffer offset beyond eve
 enum { kActLinear = 1, kActRelu, kActLrelu, kActTanh, kActSigmoid, kActElu, kActSelu, kActSoftplus, kActSwish };
 constexpr float kSeluScale = 1.0507009873554804934193349852946f, kSeluAlpha = 1.6732632423543772848170429916717f;
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+// exp and friends: the library's for float32 outputs; for 16-bit ones the hardware's exp2, log2 and reciprocal (1 ulp each, the
+// argument's rounding adds |z| * 2^-24), which a 16-bit result does not see, with a series where a difference would cancel.
+// An epilogue of ~35 instructions per element (expf, a division) takes 17 us of a 256 x 256 tile's 60 otherwise.
+template <bool FAST> struct Math {
+    static __device__ __forceinline__ float exp(float z) { return FAST ? __builtin_amdgcn_exp2f(z * 1.44269504088896341f) : expf(z); }
+    static __device__ __forceinline__ float sigmoid(float z) { return FAST ? __builtin_amdgcn_rcpf(1.f + exp(-z)) : 1.f / (1.f + expf(-z)); }
+    static __device__ __forceinline__ float tanh(float z) {
+        if (!FAST) return tanhf(z);
+        const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + exp(2.f * z));
+        return fabsf(z) < 0.02f ? z - z * z * z * (1.f / 3.f) : t;
+    }
+    static __device__ __forceinline__ float expm1(float z) {
+        if (!FAST) return expm1f(z);
+        return fabsf(z) < 0.01f ? z + z * z * (0.5f + z * (1.f / 6.f)) : exp(z) - 1.f;
+    }
+    static __device__ __forceinline__ float softplus(float z) {
+        if (!FAST) return fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
+        const float t = exp(-fabsf(z));
+        return fmaxf(z, 0.f) + (t < 0.001f ? t - 0.5f * t * t : __builtin_amdgcn_logf(1.f + t) * 0.693147180559945309f);
+    }
+};
 
-template <int ACT> __device__ __forceinline__ float activation(float alpha, float z) {
+template <int ACT, bool FAST> __device__ __forceinline__ float activation(float alpha, float z) {
+    using M = Math<FAST>;
     if constexpr (ACT == kActRelu) return z > 0.f ? z : (z != z ? z : 0.f);
     if constexpr (ACT == kActLrelu) return z > 0.f ? z : z * alpha;
-    if constexpr (ACT == kActTanh) return tanhf(z);
-    if constexpr (ACT == kActSigmoid) return sigmoid(z);
-    if constexpr (ACT == kActElu) return z > 0.f ? z : expm1f(z);
-    if constexpr (ACT == kActSelu) return kSeluScale * (z > 0.f ? z : kSeluAlpha * expm1f(z));
-    if constexpr (ACT == kActSoftplus) return fmaxf(z, 0.f) + log1pf(expf(-fabsf(z)));
-    if constexpr (ACT == kActSwish) return z * sigmoid(z);
+    if constexpr (ACT == kActTanh) return M::tanh(z);
+    if constexpr (ACT == kActSigmoid) return M::sigmoid(z);
+    if constexpr (ACT == kActElu) return z > 0.f ? z : M::expm1(z);
+    if constexpr (ACT == kActSelu) return kSeluScale * (z > 0.f ? z : kSeluAlpha * M::expm1(z));
+    if constexpr (ACT == kActSoftplus) return M::softplus(z);
+    if constexpr (ACT == kActSwish) return z * M::sigmoid(z);
     return z;
 }
 
 // v = act(v) * gain for N values (one switch for all of them; the elements are a loop, not N copies of nine functions)
-template <int N> __device__ __forceinline__ void activate(int act, float alpha, float gain, float (&v)[N]) {
-#define SG_ACT(A) case A: _Pragma("unroll") for (int e = 0; e < N; e++) v[e] = activation<A>(alpha, v[e]) * gain; break;
+template <bool FAST, int N> __device__ __forceinline__ void activate(int act, float alpha, float gain, float (&v)[N]) {
+#define SG_ACT(A) case A: _Pragma("unroll") for (int e = 0; e < N; e++) v[e] = activation<A, FAST>(alpha, v[e]) * gain; break;
     switch (act) {
         SG_ACT(kActRelu) SG_ACT(kActLrelu) SG_ACT(kActTanh) SG_ACT(kActSigmoid) SG_ACT(kActElu) SG_ACT(kActSelu) SG_ACT(kActSoftplus) SG_ACT(kActSwish)
         SG_ACT(kActLinear)
@@ -57,17 +78,22 @@ template <int N> __device__ __forceinline__ void activate(int act, float alpha, 
 }
 
 // act'(z) of the activations that are not piecewise linear with corner at zero alone
-__device__ __forceinline__ float slope_at(int act, float z) {
+template <bool FAST> __device__ __forceinline__ float slope_at(int act, float z) {
+    using M = Math<FAST>;
     switch (act) {
-        case kActTanh: { const float t = tanhf(z); return 1.f - t * t; }
-        case kActSigmoid: { const float t = sigmoid(z); return t * (1.f - t); }
-        case kActElu: return z > 0.f ? 1.f : expf(z);
-        case kActSelu: return kSeluScale * (z > 0.f ? 1.f : kSeluAlpha * expf(z));
-        case kActSoftplus: return sigmoid(z);
-        case kActSwish: { const float t = sigmoid(z); return t * (1.f + z * (1.f - t)); }
+        case kActTanh: { const float t = M::tanh(z); return 1.f - t * t; }
+        case kActSigmoid: { const float t = M::sigmoid(z); return t * (1.f - t); }
+        case kActElu: return z > 0.f ? 1.f : M::exp(z);
+        case kActSelu: return kSeluScale * (z > 0.f ? 1.f : kSeluAlpha * M::exp(z));
+        case kActSoftplus: return M::sigmoid(z);
+        case kActSwish: { const float t = M::sigmoid(z); return t * (1.f + z * (1.f - t)); }
         default: return 1.f;
     }
 }
+
+// Rounding to T, to nearest even (bfloat16: the hardware's conversion).
+template <class T> __device__ __forceinline__ T rounded(float v) { return Elem<T>::store(v); }
+template <> __device__ __forceinline__ __hip_bfloat16 rounded<__hip_bfloat16>(float v) { return __builtin_bit_cast(__hip_bfloat16, (__bf16)v); }
 
 // ---- the matrix product -----------------------------------------------------------------------------------------------------
 
@@ -93,21 +119,26 @@ struct Gemm {
 
 template <class T, int N> struct alignas(N * sizeof(T)) Run { T v[N]; };
 
+template <class T, int N> __device__ __forceinline__ Run<T, N> bias_run(const Gemm& g, int64_t j) {
+    return g.bias ? *reinterpret_cast<const Run<T, N>*>((const T*)g.bias + j) : Run<T, N>{};
+}
+
 // N consecutive results (i, j .. j + N - 1), all inside; runs of N are aligned wherever they are read and written.
 template <class T, int N, bool FORWARD>
 __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int64_t j, float (&v)[N]) {
+    Run<T, N> bias{}, res{};
+    if constexpr (FORWARD) {
+        bias = bias_run<T, N>(g, j);
+        if (g.residual) res = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + i * g.ldr + j);
+    }
     const int64_t at = i * g.nj + j;
     Run<T, N> out;
 #pragma unroll
     for (int e = 0; e < N; e++) v[e] *= g.scale;
     if constexpr (FORWARD) {
-        Run<T, N> res;
-        if (g.residual) res = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + i * g.ldr + j);
-        if (g.bias) {
-            const Run<T, N> bias = *reinterpret_cast<const Run<T, N>*>((const T*)g.bias + j);
+        if (g.bias)
 #pragma unroll
             for (int e = 0; e < N; e++) v[e] += Elem<T>::load(bias.v[e]) * g.b_gain;
-        }
         if (g.z) {
             Run<float, N> z;
 #pragma unroll
@@ -120,13 +151,13 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int64_t j, floa
             for (int e = 0; e < N; e++) pos.v[e] = v[e] > 0.f;
             *reinterpret_cast<Run<uint8_t, N>*>(g.positive + at) = pos;
         }
-        activate(g.act, g.alpha, g.gain, v);
+        activate<sizeof(T) == 2>(g.act, g.alpha, g.gain, v);
         if (g.residual)
 #pragma unroll
             for (int e = 0; e < N; e++) v[e] += Elem<T>::load(res.v[e]);
     }
 #pragma unroll
-    for (int e = 0; e < N; e++) out.v[e] = Elem<T>::store(v[e]);
+    for (int e = 0; e < N; e++) out.v[e] = rounded<T>(v[e]);
     *reinterpret_cast<Run<T, N>*>((T*)g.out + at) = out;
 }
 
@@ -295,6 +326,7 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
 // two "rows" operands are the forward pass and carry its epilogue.
 template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, bool DIRECT>
 __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
+    constexpr bool FORWARD = ROWS_A && ROWS_B;
     constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
     using TileA = Tile<T, BI, ROWS_A, THREADS>;
     using TileB = Tile<T, BJ, ROWS_B, THREADS>;
@@ -494,34 +526,107 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                 }
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-        for (int k = lane; k < S_PASS * 16 * RUNS; k += 64) {
-            const int row = k / RUNS, run = k % RUNS;
-            const int64_t i = i0 + wi + FragA::row(s0 + row / 16, row % 16), j = j0 + wj + run * N;
-            if (i >= g.ni || j >= g.nj) continue;
-            float v[N];
+        // 64 / RUNS rows at a time; a lane keeps its columns.
+        constexpr int ROUND = 64 / RUNS, ROUNDS = S_PASS * 16 / ROUND;
+        static_assert(ROUND * RUNS == 64 && ROUNDS * ROUND == S_PASS * 16, "whole rounds");
+        const int run = lane % RUNS, row0 = lane / RUNS;
+        const int64_t j = j0 + wj + run * N;
+        auto row_of = [&](int round) { const int row = round * ROUND + row0; return i0 + wi + FragA::row(s0 + row / 16, row % 16); };
+        auto take = [&](int round, float* v) {
 #pragma unroll
             for (int q = 0; q < N / 4; q++) {
-                const f32x4_t c = chunk_at(row, run * (N / 4) + q);
+                const f32x4_t c = chunk_at(round * ROUND + row0, run * (N / 4) + q);
                 v[4 * q] = c.x; v[4 * q + 1] = c.y; v[4 * q + 2] = c.z; v[4 * q + 3] = c.w;
             }
-            if (g.slices > 1) {
-                float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
-                if (g.whole) {
+        };
+        // Tiles that lie inside whole rows: no branch around a load or a store.  (Both count in vmcnt; behind a branch the compiler
+        // cannot count, and a wait for the prefetched residual becomes one for every store as well: 28 us a tile instead of 8.)
+        if (g.slices == 1 && g.whole && left_i == BI && left_j == BJ) {
+            constexpr int U = ROUNDS % 2 == 0 ? 2 : 1;
+            auto rounds = [&](auto has_residual) {
+                float bias[N] = {};
+                Run<T, N> next[U];
+                if constexpr (FORWARD) {
+                    const Run<T, N> raw = bias_run<T, N>(g, j);
 #pragma unroll
-                    for (int q = 0; q < N / 4; q++) *reinterpret_cast<f32x4_t*>(out + 4 * q) = f32x4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-                } else {
+                    for (int e = 0; e < N; e++) bias[e] = Elem<T>::load(raw.v[e]) * g.b_gain;
+                    if constexpr (has_residual)
 #pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (j + e < g.nj) out[e] = v[e];
+                        for (int u = 0; u < U; u++) next[u] = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + row_of(u) * g.ldr + j);
                 }
-            } else if (g.whole) {
-                finish<T, N, ROWS_A && ROWS_B>(g, i, j, v);
-            } else {
 #pragma unroll 1
-                for (int e = 0; e < N && j + e < g.nj; e++) {
-                    float one[1] = {chunk_at(row, run * (N / 4) + e / 4)[e % 4]};
-                    finish<T, 1, ROWS_A && ROWS_B>(g, i, j + e, one);
+                for (int round = 0; round < ROUNDS; round += U) {
+                    Run<T, N> now[U];
+                    if constexpr (has_residual) {
+                        const int ahead = min(round + U, ROUNDS - U);
+#pragma unroll
+                        for (int u = 0; u < U; u++) {
+                            now[u] = next[u];
+                            next[u] = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + row_of(ahead + u) * g.ldr + j);
+                        }
+                    }
+                    float v[U * N];
+#pragma unroll
+                    for (int u = 0; u < U; u++) take(round + u, v + u * N);
+#pragma unroll
+                    for (int e = 0; e < U * N; e++) v[e] = v[e] * g.scale + bias[e % N];
+                    if constexpr (FORWARD) {
+                        if (g.z)
+#pragma unroll
+                            for (int u = 0; u < U; u++)
+#pragma unroll
+                                for (int q = 0; q < N; q += 4)
+                                    *reinterpret_cast<f32x4_t*>(g.z + row_of(round + u) * g.nj + j + q) =
+                                        f32x4_t{v[u * N + q], v[u * N + q + 1], v[u * N + q + 2], v[u * N + q + 3]};
+                        if (g.positive)
+#pragma unroll
+                            for (int u = 0; u < U; u++) {
+                                Run<uint8_t, N> pos;
+#pragma unroll
+                                for (int e = 0; e < N; e++) pos.v[e] = v[u * N + e] > 0.f;
+                                *reinterpret_cast<Run<uint8_t, N>*>(g.positive + row_of(round + u) * g.nj + j) = pos;
+                            }
+                        activate<sizeof(T) == 2>(g.act, g.alpha, g.gain, v);
+                        if constexpr (has_residual)
+#pragma unroll
+                            for (int e = 0; e < U * N; e++) v[e] += Elem<T>::load(now[e / N].v[e % N]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        Run<T, N> out;
+#pragma unroll
+                        for (int e = 0; e < N; e++) out.v[e] = rounded<T>(v[u * N + e]);
+                        *reinterpret_cast<Run<T, N>*>((T*)g.out + row_of(round + u) * g.nj + j) = out;
+                    }
+                }
+            };
+            if (FORWARD && g.residual) rounds(std::true_type{});
+            else rounds(std::false_type{});
+        } else {
+#pragma unroll 1
+            for (int round = 0; round < ROUNDS; round++) {
+                const int64_t i = row_of(round);
+                if (i >= g.ni || j >= g.nj) continue;
+                float v[N];
+                take(round, v);
+                if (g.slices > 1) {
+                    float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
+                    if (g.whole) {
+#pragma unroll
+                        for (int q = 0; q < N; q += 4) *reinterpret_cast<f32x4_t*>(out + q) = f32x4_t{v[q], v[q + 1], v[q + 2], v[q + 3]};
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < N; e++)
+                            if (j + e < g.nj) out[e] = v[e];
+                    }
+                } else if (g.whole) {
+                    finish<T, N, FORWARD>(g, i, j, v);
+                } else {
+#pragma unroll 1
+                    for (int e = 0; e < N && j + e < g.nj; e++) {
+                        float one[1] = {chunk_at(round * ROUND + row0, run * (N / 4) + e / 4)[e % 4]};
+                        finish<T, 1, FORWARD>(g, i, j + e, one);
+                    }
                 }
             }
         }
@@ -606,9 +711,9 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
                 float s = Elem<T>::load(dy[u].v[e]);
                 if (p.y) s = Elem<T>::load(y[u].v[e]) * p.sign > 0.f ? s : s * p.alpha;
                 else if (p.positive) s = pos[u].v[e] ? s : s * p.alpha;
-                else if (p.z) s *= slope_at(p.act, z[u].v[e]);
+                else if (p.z) s *= slope_at<sizeof(T) == 2>(p.act, z[u].v[e]);
                 sum[e] += s;
-                out.v[e] = Elem<T>::store(s);
+                out.v[e] = rounded<T>(s);
             }
             if (p.s) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.cols + c) = out;
         }
