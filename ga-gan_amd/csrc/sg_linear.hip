@@ -13,6 +13,7 @@
 #include "sg_common.h"
 #include "sg_column_sums.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace sg {
@@ -235,25 +236,41 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
         copy_to_lds(from, inside(s, k, left_side, left_p) ? s.off : kOutside, (unsigned)apart(k) * ld * ES, lds + (k * THREADS + wave * 64) * 16);
     }
     // by way of registers: any alignment, any extent
+    // A slot that the end of its row cuts is read from the row's last 16 bytes and shifted into place, so that every slot is
+    // one load without a branch around it (extent_c: elements from the tile's first one to the end of its rows, along the
+    // contiguous index, of row_c in all).  Rows shorter than 16 bytes are read element by element.
     struct Regs { uint4 v[LOADS]; };
-    static __device__ __forceinline__ void fetch(Regs& r, const Slots& s, const T* base, int64_t ld, int left_side, int left_p) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[E]; };
-        const T* first = base + (ROWS ? s.side * ld + s.p : s.p * ld + s.side);
+    static __device__ __forceinline__ void fetch(Regs& r, const Slots& s, const T* base, int64_t ld, int left_side, int left_p, int64_t extent_c, int64_t row_c) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Loose { uint4 v; };
+        const int c = ROWS ? s.p : s.side;                             // the slot's place along the contiguous index
+        if (row_c >= E) {
+            const int cut = c + E > extent_c ? (int)min(c + E - extent_c, (int64_t)E) : 0;
+            const int64_t back = cut == E ? extent_c - E : c - cut;        // (a slot wholly outside reads what is inside)
 #pragma unroll
-        for (int k = 0; k < LOADS; k++) {
-            const T* src = first + apart(k) * ld;
-            const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
-            const int in_line = ROWS ? left_p - s.p : left_side - s.side;
-            Pack<T> q;
-            if (line && in_line >= E) {
-                const Loose l = *reinterpret_cast<const Loose*>(src);
-#pragma unroll
-                for (int e = 0; e < E; e++) q.v[e] = l.v[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) q.v[e] = line && e < in_line ? src[e] : Elem<T>::store(0.f);
+            for (int k = 0; k < LOADS; k++) {
+                const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
+                const int l = line ? (ROWS ? s.side : s.p) + apart(k) : 0;
+                r.v[k] = reinterpret_cast<const Loose*>(base + l * ld + back)->v;
             }
-            __builtin_memcpy(&r.v[k], &q, 16);
+#pragma unroll
+            for (int k = 0; k < LOADS; k++) {
+                const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
+                if (cut) {
+                    const unsigned __int128 q = __builtin_bit_cast(unsigned __int128, r.v[k]);
+                    r.v[k] = cut == E ? make_uint4(0, 0, 0, 0) : __builtin_bit_cast(uint4, q >> (cut * ES * 8));
+                }
+                if (!line) r.v[k] = make_uint4(0, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < LOADS; k++) {
+                const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
+                const T* src = base + ((ROWS ? s.side : s.p) + apart(k)) * ld + c;
+                Pack<T> q;
+#pragma unroll 1
+                for (int e = 0; e < E; e++) q.v[e] = line && c + e < extent_c ? src[e] : Elem<T>::store(0.f);
+                __builtin_memcpy(&r.v[k], &q, 16);
+            }
         }
     }
     static __device__ __forceinline__ void commit(unsigned char* lds, const Regs& r) {
@@ -461,8 +478,9 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         typename TileB::Regs rb;
         auto fetch = [&](int n) {
             const int step = first + n;
-            TileA::fetch(ra, sa, at_a(step), g.lda, left_i, left_p(step));
-            TileB::fetch(rb, sb, at_b(step), g.ldb, left_j, left_p(step));
+            const int64_t rest_p = g.np - (int64_t)step * BK;
+            TileA::fetch(ra, sa, at_a(step), g.lda, left_i, left_p(step), ROWS_A ? rest_p : g.ni - i0, ROWS_A ? g.np : g.ni);
+            TileB::fetch(rb, sb, at_b(step), g.ldb, left_j, left_p(step), ROWS_B ? rest_p : g.nj - j0, ROWS_B ? g.np : g.nj);
         };
         auto commit = [&](int buf) {
             TileA::commit(smem + buf * BUF, ra);
@@ -634,6 +652,80 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     }
 }
 
+// Few rows (at most 32) and a short sum: the tile kernel would spend most of its products on rows that are not there, and need
+// slices and a second launch to use more than a few CUs.  Here eight waves share the sum of 16 (ROWS_B) or 32 columns: operands go
+// from global memory to fragments, 64 bytes of p per wave and turn (the eight waves' turns lie side by side), the waves' sums are
+// added in wave order.  Rows of both operands are whole aligned packets.  TI: row tiles.
+template <class T, int TI, bool ROWS_B>
+__global__ void __launch_bounds__(512) linear_thin_kernel(const Gemm g) {
+    constexpr int WAVES = 8, TJ = ROWS_B ? 1 : 2, COLS = 16 * TJ, E = 16 / (int)sizeof(T), UNIT = 4 * E, UNROLL = 4;
+    static_assert(ROWS_B || sizeof(T) == 4, "16-bit columns need the transposing read");
+    __shared__ __attribute__((aligned(16))) float part[WAVES][TI * 16][COLS + 4];
+    const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t j0 = (int64_t)blockIdx.x * COLS;
+    const T* a = (const T*)g.a;
+    const T* b = (const T*)g.b;
+    const int64_t units = (g.np + UNIT - 1) / UNIT;
+    f32x4_t acc[TJ][TI];
+#pragma unroll
+    for (int t = 0; t < TJ; t++)
+#pragma unroll
+        for (int s = 0; s < TI; s++) acc[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int64_t u0 = wave; u0 < units; u0 += WAVES * UNROLL) {
+        uint4 fa[UNROLL][TI], fb[UNROLL];
+        float fc[UNROLL][TJ][4];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const int64_t p = (u0 + u * WAVES) * UNIT + quad * E;
+            const bool in = p < g.np;
+#pragma unroll
+            for (int s = 0; s < TI; s++) fa[u][s] = load16_or_zero(in && s * 16 + l16 < g.ni, a + (s * 16 + l16) * g.lda + p);
+            if constexpr (ROWS_B) {
+                fb[u] = load16_or_zero(in && j0 + l16 < g.nj, b + (j0 + l16) * g.ldb + p);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {              // two columns a lane
+                    const uint2 v = load8_or_zero(p + e < g.np && j0 + 2 * l16 < g.nj, b + (p + e) * g.ldb + j0 + 2 * l16);
+                    fc[u][0][e] = __uint_as_float(v.x);
+                    fc[u][1][e] = __uint_as_float(v.y);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+            for (int t = 0; t < TJ; t++)
+#pragma unroll
+                for (int s = 0; s < TI; s++) {
+                    if constexpr (sizeof(T) == 2) {
+                        acc[t][s] = mfma(fb[u], fa[u][s], acc[t][s], T());
+                    } else {
+                        const f32x4_t va = __builtin_bit_cast(f32x4_t, fa[u][s]);
+                        const f32x4_t vb = ROWS_B ? __builtin_bit_cast(f32x4_t, fb[u]) : f32x4_t{fc[u][t][0], fc[u][t][1], fc[u][t][2], fc[u][t][3]};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(vb[e], va[e], acc[t][s], 0, 0, 0);
+                    }
+                }
+    }
+    // row s * 16 + l16, columns quad * 4 + r (two tiles: interleaved)
+#pragma unroll
+    for (int s = 0; s < TI; s++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < TJ; t++) part[wave][s * 16 + l16][(quad * 4 + r) * TJ + t] = acc[t][s][r];
+    __syncthreads();
+    for (int k = threadIdx.x; k < TI * 16 * COLS; k += 512) {
+        const int i = k / COLS, c = k % COLS;
+        if (i >= g.ni || j0 + c >= g.nj) continue;
+        float v[1] = {0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) v[0] += part[w][i][c];
+        finish<T, 1, ROWS_B>(g, i, j0 + c, v);
+    }
+}
+
 // The slices' partial sums, added in slice order, and the epilogue.
 template <class T, int RUN, bool FORWARD>
 __global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
@@ -788,59 +880,94 @@ template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* 
 }
 
 struct Shape {                            // workgroup tile and slices of one product
-    int bi = 0, bj = 0;
+    bool thin = false;
+    int tile = 0;
     int tiles_i = 0, tiles_j = 0, slices = 1, slice_steps = 1;
     size_t partial_bytes = 0;
 };
 
-Shape shape_of(int dtype, int64_t ni, int64_t nj, int64_t np) {
-    Shape s;
-    const int bk = dtype == SG_F32 ? 32 : 64;
-    auto count = [&](int t) { return ((ni + t - 1) / t) * ((nj + t - 1) / t); };
-    int t = 64;
-    if (dtype != SG_F32 && count(256) >= 192) t = 256;
-    else if (count(128) >= 192) t = 128;
-    s.bi = s.bj = t;
-    s.tiles_i = (int)((ni + t - 1) / t);
-    s.tiles_j = (int)((nj + t - 1) / t);
-    const int64_t steps = (np + bk - 1) / bk, tiles = (int64_t)s.tiles_i * s.tiles_j;
-    int64_t slices = 1;
-    if (tiles < 192 && steps > 1) {
-        slices = 512 / tiles;
-        if (slices > steps / 2) slices = steps / 2;
-        if (slices > 64) slices = 64;
-        if (slices < 1) slices = 1;
-    }
-    s.slice_steps = (int)(steps < 1 ? 1 : (steps + slices - 1) / slices);
-    s.slices = (int)(steps < 1 ? 1 : (steps + s.slice_steps - 1) / s.slice_steps);
-    if (s.slices > 1) s.partial_bytes = up256((size_t)s.slices * ni * nj * 4);
-    return s;
+// Whether linear_thin_kernel covers a product: few rows, a sum of at most 16 turns of its eight waves, packets.
+bool thin_fits(int dtype, bool rows_b, int64_t ni, int64_t nj, int64_t np) {
+    const int e = dtype == SG_F32 ? 4 : 8;
+    return ni <= 32 && np <= 16 * 8 * 4 * e && np % e == 0 && (rows_b || (dtype == SG_F32 && nj % 2 == 0));
 }
 
-template <class T, int BI, int WI, int WJ, bool RA, bool RB>
-void launch_gemm(const Gemm& g, bool direct, hipStream_t stream) {
-    const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices)), block(WI * WJ * 64);
-    if (direct) hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, true>), grid, block, 0, stream, g);
-    else hipLaunchKernelGGL((linear_gemm_kernel<T, BI, BI, WI, WJ, RA, RB, false>), grid, block, 0, stream, g);
+// The tile and the number of slices with the least predicted time.  Measured on MI355X, us per step (128 bytes along p) of a
+// workgroup that has a CU to itself / of each of several that share one, by the number of "columns" operands:
+//   16-bit  64 x 64: 0.25 / 0.18, 0.28 / 0.18, 0.31 / 0.20     128 x 128: 0.69 / 0.45, 0.69 / 0.47, 0.82 / 0.59     256 x 256: 1.8, 1.63, 1.61
+//   float32 64 x 64: 0.62 / 0.50, whichever                     (a 128 x 128 tile takes four times that: not built)
+// 3 us for a launch and its ends; slices cost a second launch and a round trip of their float32 sums at 6 TB/s.
+// 1024^3 in bfloat16: 64 x 64 tiles 6.9 us, 128 x 128 11.5; 4096^3: 256 x 256 106, 128 x 128 122, 64 x 64 190; a weight gradient of
+// 2048 x 2048 over 8192 rows: 256 x 256 in four slices 76, 128 x 128 106.
+Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
+    struct Kind { int tile; double alone[3], shared[3]; };
+    static const Kind kinds[] = {{64, {0.25, 0.28, 0.31}, {0.18, 0.18, 0.20}}, {128, {0.69, 0.69, 0.82}, {0.45, 0.47, 0.59}}, {256, {1.8, 1.63, 1.61}, {1.8, 1.63, 1.61}}};
+    static const Kind kinds32[] = {{64, {0.62, 0.62, 0.62}, {0.50, 0.50, 0.50}}};
+    Shape best;
+    best.thin = columns < 2 && thin_fits(dtype, columns == 0, ni, nj, np);
+    const int bk = dtype == SG_F32 ? 32 : 64;
+    const int64_t steps = np <= 0 ? 1 : (np + bk - 1) / bk;
+    double best_us = 0;
+    for (int k = 0; k < (dtype == SG_F32 ? 1 : 3); k++) {
+        const Kind& kind = dtype == SG_F32 ? kinds32[k] : kinds[k];
+        const int64_t ti = (ni + kind.tile - 1) / kind.tile, tj = (nj + kind.tile - 1) / kind.tile;
+        for (int64_t slices = 1; slices <= 64 && (slices == 1 || 2 * slices <= steps); slices = slices < 4 ? slices + 1 : slices * 3 / 2) {
+            const int64_t each = (steps + slices - 1) / slices, used = (steps + each - 1) / each;
+            const int64_t per_cu = (ti * tj * used + 255) / 256;
+            const double step = std::max(kind.alone[columns], kind.shared[columns] * (double)per_cu);
+            const double us = 3 + (double)each * step + (used > 1 ? 4 + (double)used * ni * nj * 8 / 6e6 : 0);
+            if (best.tile == 0 || us < best_us) {
+                best_us = us;
+                best.tile = kind.tile;
+                best.tiles_i = (int)ti;
+                best.tiles_j = (int)tj;
+                best.slices = (int)used;
+                best.slice_steps = (int)each;
+            }
+        }
+    }
+    if (best.slices > 1) best.partial_bytes = up256((size_t)best.slices * ni * nj * 4);
+    return best;
+}
+
+template <class T, int TILE, bool RA, bool RB, bool DIRECT> void launch_gemm(const Gemm& g, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices));
+    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, DIRECT>), grid, dim3(256), 0, stream, g);
 }
 
 template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
     constexpr int ES = sizeof(T), E = 16 / ES;
     if (g.ni == 0 || g.nj == 0) return SG_OK;
     g.tiles_i = s.tiles_i; g.tiles_j = s.tiles_j; g.slices = s.slices; g.slice_steps = s.slice_steps;
-    SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
     // offsets within a tile's lines are 32-bit
     SG_REQUIRE((g.lda + 1) * ES * 256 < (int64_t)kOutside && (g.ldb + 1) * ES * 256 < (int64_t)kOutside, SG_ERR_UNSUPPORTED,
                "%s: rows of %lld / %lld elements are too long", what, (long long)g.lda, (long long)g.ldb);
     const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && (RA ? g.np : g.ni) % E == 0 && (RB ? g.np : g.nj) % E == 0;
     g.whole = runs_aligned<T>(g);
+    if constexpr (RA && (RB || ES == 4)) {
+        if (s.thin && aligned16(g.a) && g.lda % E == 0 && (RB ? aligned16(g.b) && g.ldb % E == 0 : reinterpret_cast<uintptr_t>(g.b) % 8 == 0 && g.ldb % 2 == 0)) {
+            const int cols = RB ? 16 : 32;
+            const dim3 grid((unsigned)((g.nj + cols - 1) / cols));
+            if (g.ni <= 16) hipLaunchKernelGGL((linear_thin_kernel<T, 1, RB>), grid, dim3(512), 0, stream, g);
+            else hipLaunchKernelGGL((linear_thin_kernel<T, 2, RB>), grid, dim3(512), 0, stream, g);
+            return check_launch(what);
+        }
+    }
+    int tile = s.tile;
+    if (tile == 256 && !direct) {          // no registers to spare there for operands that need them on their way to LDS
+        tile = 128;
+        g.tiles_i = (int)((g.ni + 127) / 128);
+        g.tiles_j = (int)((g.nj + 127) / 128);
+    }
+    SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
     if constexpr (ES == 2) {
-        if (s.bi == 256) launch_gemm<T, 256, 2, 2, RA, RB>(g, direct, stream);
-        else if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, stream);
-        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, stream);
-    } else {
-        if (s.bi == 128) launch_gemm<T, 128, 2, 2, RA, RB>(g, direct, stream);
-        else launch_gemm<T, 64, 2, 2, RA, RB>(g, direct, stream);
+        if (tile == 256) launch_gemm<T, 256, RA, RB, true>(g, stream);
+        else if (tile == 128 && direct) launch_gemm<T, 128, RA, RB, true>(g, stream);
+        else if (tile == 128) launch_gemm<T, 128, RA, RB, false>(g, stream);
+    }
+    if (tile == 64) {
+        if (direct) launch_gemm<T, 64, RA, RB, true>(g, stream);
+        else launch_gemm<T, 64, RA, RB, false>(g, stream);
     }
     if (g.slices > 1) {
         const int run = g.whole ? 4 : 1;
@@ -878,8 +1005,8 @@ BackwardPlan plan_backward(const sg_linear_params& p) {
     if (p.act != kActLinear) at += up256((size_t)p.m * p.n * es);
     b.sums = at;
     at += up256((size_t)slope_blocks(p.m, p.n) * p.n * 4);
-    b.x = shape_of(p.dtype, p.m, p.k, p.n);
-    b.w = shape_of(p.dtype, p.n, p.k, p.m);
+    b.x = shape_of(p.dtype, 1, p.m, p.k, p.n);
+    b.w = shape_of(p.dtype, 2, p.n, p.k, p.m);
     b.partial = at;
     at += b.x.partial_bytes > b.w.partial_bytes ? b.x.partial_bytes : b.w.partial_bytes;
     b.total = at;
@@ -903,7 +1030,7 @@ int column_sums(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ld
 extern "C" size_t sg_linear_workspace_bytes(const sg_linear_params* p) {
     using namespace sg;
     if (check(p, "linear") != SG_OK) return 0;
-    return shape_of(p->dtype, p->m, p->n, p->k).partial_bytes;
+    return shape_of(p->dtype, 0, p->m, p->n, p->k).partial_bytes;
 }
 
 extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* positive, void* workspace, size_t workspace_bytes, sg_stream_t stream) {
@@ -913,7 +1040,7 @@ extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* 
     if (p->m == 0 || p->n == 0) return SG_OK;
     SG_REQUIRE(y != nullptr, SG_ERR_NULL_POINTER, "linear: y is NULL");
     SG_REQUIRE(p->residual == nullptr || p->ldr >= p->n, SG_ERR_INVALID_ARGUMENT, "linear: the residual's row stride is smaller than its rows");
-    const Shape s = shape_of(p->dtype, p->m, p->n, p->k);
+    const Shape s = shape_of(p->dtype, 0, p->m, p->n, p->k);
     SG_REQUIRE(s.partial_bytes == 0 || (workspace && workspace_bytes >= s.partial_bytes && aligned16(workspace)), SG_ERR_INVALID_ARGUMENT,
                "linear: needs %zu bytes of aligned workspace", s.partial_bytes);
     Gemm g{};
