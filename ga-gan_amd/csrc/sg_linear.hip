@@ -236,46 +236,54 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
         copy_to_lds(from, inside(s, k, left_side, left_p) ? s.off : kOutside, (unsigned)apart(k) * ld * ES, lds + (k * THREADS + wave * 64) * 16);
     }
     // by way of registers: any alignment, any extent
-    // A slot that the end of its row cuts is read from the row's last 16 bytes and shifted into place, so that every slot is
-    // one load without a branch around it (extent_c: elements from the tile's first one to the end of its rows, along the
-    // contiguous index, of row_c in all).  Rows shorter than 16 bytes are read element by element.
+    // A slot that the end of its row cuts is read from the row's last 16 bytes and shifted into place when it is written to LDS, so
+    // that every slot is one load without a branch around it and nothing waits for a load before then.  (extent_c: elements from
+    // the tile's first one to the end of its rows, along the contiguous index.)  Rows shorter than 16 bytes are read element by
+    // element (SHORT).
     struct Regs { uint4 v[LOADS]; };
-    static __device__ __forceinline__ void fetch(Regs& r, const Slots& s, const T* base, int64_t ld, int left_side, int left_p, int64_t extent_c, int64_t row_c) {
+    static __device__ __forceinline__ bool line_inside(const Slots& s, int k, int left_side, int left_p) {
+        return ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
+    }
+    // elements of the slot beyond the end of its row
+    static __device__ __forceinline__ int cut_of(const Slots& s, int64_t extent_c) {
+        const int c = ROWS ? s.p : s.side;
+        return c + E > extent_c ? (int)min(c + E - extent_c, (int64_t)E) : 0;
+    }
+    template <bool SHORT>
+    static __device__ __forceinline__ void fetch(Regs& r, const Slots& s, const T* base, int64_t ld, int left_side, int left_p, int64_t extent_c) {
         struct __attribute__((packed, aligned(sizeof(T)))) Loose { uint4 v; };
-        const int c = ROWS ? s.p : s.side;                             // the slot's place along the contiguous index
-        if (row_c >= E) {
-            const int cut = c + E > extent_c ? (int)min(c + E - extent_c, (int64_t)E) : 0;
-            const int64_t back = cut == E ? extent_c - E : c - cut;        // (a slot wholly outside reads what is inside)
+        const int c = ROWS ? s.p : s.side, cut = cut_of(s, extent_c);
+        const int64_t back = SHORT ? 0 : cut == E ? extent_c - E : c - cut;        // (a slot wholly outside reads what is inside)
 #pragma unroll
-            for (int k = 0; k < LOADS; k++) {
-                const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
-                const int l = line ? (ROWS ? s.side : s.p) + apart(k) : 0;
-                r.v[k] = reinterpret_cast<const Loose*>(base + l * ld + back)->v;
-            }
-#pragma unroll
-            for (int k = 0; k < LOADS; k++) {
-                const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
-                if (cut) {
-                    const unsigned __int128 q = __builtin_bit_cast(unsigned __int128, r.v[k]);
-                    r.v[k] = cut == E ? make_uint4(0, 0, 0, 0) : __builtin_bit_cast(uint4, q >> (cut * ES * 8));
-                }
-                if (!line) r.v[k] = make_uint4(0, 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < LOADS; k++) {
-                const bool line = ROWS ? s.side < left_side - apart(k) : s.p < left_p - apart(k);
-                const T* src = base + ((ROWS ? s.side : s.p) + apart(k)) * ld + c;
+        for (int k = 0; k < LOADS; k++) {
+            const T* line = base + (line_inside(s, k, left_side, left_p) ? (ROWS ? s.side : s.p) + apart(k) : 0) * ld;
+            if constexpr (SHORT) {
                 Pack<T> q;
-#pragma unroll 1
-                for (int e = 0; e < E; e++) q.v[e] = line && c + e < extent_c ? src[e] : Elem<T>::store(0.f);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const T v = line[c + e < extent_c ? c + e : 0];
+                    q.v[e] = c + e < extent_c ? v : Elem<T>::store(0.f);
+                }
                 __builtin_memcpy(&r.v[k], &q, 16);
+            } else {
+                r.v[k] = reinterpret_cast<const Loose*>(line + back)->v;
             }
         }
     }
-    static __device__ __forceinline__ void commit(unsigned char* lds, const Regs& r) {
+    template <bool SHORT>
+    static __device__ __forceinline__ void commit(unsigned char* lds, const Regs& r, const Slots& s, int left_side, int left_p, int64_t extent_c) {
+        const int cut = cut_of(s, extent_c);
 #pragma unroll
-        for (int k = 0; k < LOADS; k++) *reinterpret_cast<uint4*>(lds + (k * THREADS + threadIdx.x) * 16) = r.v[k];
+        for (int k = 0; k < LOADS; k++) {
+            uint4 q = r.v[k];
+            if (!SHORT) {                                              // up by `cut` elements, zeros behind them
+                if (ES == 2 && (cut & 1)) q = make_uint4(q.x >> 16 | q.y << 16, q.y >> 16 | q.z << 16, q.z >> 16 | q.w << 16, q.w >> 16);
+                if (cut & (4 / ES)) q = make_uint4(q.y, q.z, q.w, 0);
+                if (cut & (8 / ES)) q = make_uint4(q.z, q.w, 0, 0);
+            }
+            const bool zero = cut == E || left_side <= 0 || !line_inside(s, k, left_side, left_p);
+            *reinterpret_cast<uint4*>(lds + (k * THREADS + threadIdx.x) * 16) = zero ? make_uint4(0, 0, 0, 0) : q;
+        }
     }
 };
 
@@ -339,9 +347,12 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Tile BI x BJ per workgroup of WI x WJ waves.  DIRECT: rows of both operands are whole aligned 16-byte packets.  Products of
+// Tile BI x BJ per workgroup of WI x WJ waves.  How operands travel: kDirect, rows of both are whole aligned 16-byte packets;
+// kLoose, rows start anywhere and end anywhere; kShort, rows of one of them are shorter than 16 bytes.  Products of
 // two "rows" operands are the forward pass and carry its epilogue.
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, bool DIRECT>
+enum { kDirect, kLoose, kShort };
+
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
 __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
     constexpr bool FORWARD = ROWS_A && ROWS_B;
     constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
@@ -397,7 +408,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
             }
         }
     };
-    if constexpr (DIRECT) {
+    if constexpr (MODE == kDirect) {
         // Two LDS buffers and two sets of fragments.  A step is two halves: the first multiplies the fragments of its first
         // K-part while those of the second are read; then, behind the one barrier of a step, the second is multiplied while the
         // first fragments of the next step are read and the copies of the step after it start into the buffer that has just
@@ -473,36 +484,47 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
             step(n, no, no);
         }
     } else {
-        // Two LDS buffers: the loads of step n + 1 are under way while step n multiplies; one barrier a step.
-        typename TileA::Regs ra;
-        typename TileB::Regs rb;
-        auto fetch = [&](int n) {
-            const int step = first + n;
-            const int64_t rest_p = g.np - (int64_t)step * BK;
-            TileA::fetch(ra, sa, at_a(step), g.lda, left_i, left_p(step), ROWS_A ? rest_p : g.ni - i0, ROWS_A ? g.np : g.ni);
-            TileB::fetch(rb, sb, at_b(step), g.ldb, left_j, left_p(step), ROWS_B ? rest_p : g.nj - j0, ROWS_B ? g.np : g.nj);
+        // Two LDS buffers and two sets of registers: a step's loads have the two steps before it to arrive; one barrier a step.
+        // Steps go in pairs and every step loads, the last ones their own data again (behind a branch the compiler would wait
+        // for the newest loads where it needs those of the step before); what lies behind the last step is written as zeros.
+        typename TileA::Regs ra[2];
+        typename TileB::Regs rb[2];
+        auto rest = [&](int n) { return g.np - (int64_t)(first + n) * BK; };
+        auto fetch = [&](int n, int set) {
+            n = min(n, steps - 1);
+            const int left = left_p(first + n);
+            TileA::template fetch<MODE == kShort>(ra[set], sa, at_a(first + n), g.lda, left_i, left, ROWS_A ? rest(n) : g.ni - i0);
+            TileB::template fetch<MODE == kShort>(rb[set], sb, at_b(first + n), g.ldb, left_j, left, ROWS_B ? rest(n) : g.nj - j0);
         };
-        auto commit = [&](int buf) {
-            TileA::commit(smem + buf * BUF, ra);
-            TileB::commit(smem + buf * BUF + TileA::BYTES, rb);
+        auto commit = [&](int n, int set) {
+            const int li = n < steps ? left_i : 0, lj = n < steps ? left_j : 0;
+            n = min(n, steps - 1);
+            const int left = left_p(first + n);
+            TileA::template commit<MODE == kShort>(smem + set * BUF, ra[set], sa, li, left, ROWS_A ? rest(n) : g.ni - i0);
+            TileB::template commit<MODE == kShort>(smem + set * BUF + TileA::BYTES, rb[set], sb, lj, left, ROWS_B ? rest(n) : g.nj - j0);
         };
-        if (steps > 0) {
-            fetch(0);
-            commit(0);
-        }
-        for (int n = 0; n < steps; n++) {
+        auto step = [&](int n, int set) {                          // set = n & 1
             __syncthreads();
-            if (n + 1 < steps) fetch(n + 1);
+            fetch(n + 2, set);
 #pragma unroll
             for (int kk = 0; kk < 2; kk++) {
                 FragA fa;
                 FragB fb;
-                fa.read(smem + (n & 1) * BUF, wi, kk);
-                fb.read(smem + (n & 1) * BUF + TileA::BYTES, wj, kk);
+                fa.read(smem + set * BUF, wi, kk);
+                fb.read(smem + set * BUF + TileA::BYTES, wj, kk);
 #pragma unroll
                 for (int t = 0; t < TJ; t++) multiply_tile(fa, fb, t);
             }
-            if (n + 1 < steps) commit((n + 1) & 1);
+            commit(n + 1, set ^ 1);
+        };
+        if (steps > 0) {
+            fetch(0, 0);
+            fetch(1, 1);
+            commit(0, 0);
+            for (int n = 0; n < steps; n += 2) {
+                step(n, 0);
+                step(n + 1, 1);
+            }
         }
     }
 
@@ -557,11 +579,15 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                 v[4 * q] = c.x; v[4 * q + 1] = c.y; v[4 * q + 2] = c.z; v[4 * q + 3] = c.w;
             }
         };
-        // Tiles that lie inside whole rows: no branch around a load or a store.  (Both count in vmcnt; behind a branch the compiler
-        // cannot count, and a wait for the prefetched residual becomes one for every store as well: 28 us a tile instead of 8.)
-        if (g.slices == 1 && g.whole && left_i == BI && left_j == BJ) {
+        // Rows of whole packets.  Inside the matrix there is no branch around a load or a store: both count in vmcnt, behind a branch
+        // the compiler cannot count, and a wait for the prefetched residual becomes one for every store as well (28 us a 256 x 256
+        // tile instead of 8).
+        if (g.slices == 1 && g.whole) {
             constexpr int U = ROUNDS % 2 == 0 ? 2 : 1;
-            auto rounds = [&](auto has_residual) {
+            auto rounds = [&](auto has_residual, auto edge) {
+                if (edge && j >= g.nj) return;
+                auto there = [&](int64_t i) { return edge ? i < g.ni : true; };
+                auto clamped = [&](int64_t i) { return edge ? min(i, g.ni - 1) : i; };
                 float bias[N] = {};
                 Run<T, N> next[U];
                 if constexpr (FORWARD) {
@@ -570,7 +596,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                     for (int e = 0; e < N; e++) bias[e] = Elem<T>::load(raw.v[e]) * g.b_gain;
                     if constexpr (has_residual)
 #pragma unroll
-                        for (int u = 0; u < U; u++) next[u] = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + row_of(u) * g.ldr + j);
+                        for (int u = 0; u < U; u++) next[u] = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + clamped(row_of(u)) * g.ldr + j);
                 }
 #pragma unroll 1
                 for (int round = 0; round < ROUNDS; round += U) {
@@ -580,7 +606,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
 #pragma unroll
                         for (int u = 0; u < U; u++) {
                             now[u] = next[u];
-                            next[u] = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + row_of(ahead + u) * g.ldr + j);
+                            next[u] = *reinterpret_cast<const Run<T, N>*>((const T*)g.residual + clamped(row_of(ahead + u)) * g.ldr + j);
                         }
                     }
                     float v[U * N];
@@ -594,7 +620,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                             for (int u = 0; u < U; u++)
 #pragma unroll
                                 for (int q = 0; q < N; q += 4)
-                                    *reinterpret_cast<f32x4_t*>(g.z + row_of(round + u) * g.nj + j + q) =
+                                    if (there(row_of(round + u))) *reinterpret_cast<f32x4_t*>(g.z + row_of(round + u) * g.nj + j + q) =
                                         f32x4_t{v[u * N + q], v[u * N + q + 1], v[u * N + q + 2], v[u * N + q + 3]};
                         if (g.positive)
 #pragma unroll
@@ -602,7 +628,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                                 Run<uint8_t, N> pos;
 #pragma unroll
                                 for (int e = 0; e < N; e++) pos.v[e] = v[u * N + e] > 0.f;
-                                *reinterpret_cast<Run<uint8_t, N>*>(g.positive + row_of(round + u) * g.nj + j) = pos;
+                                if (there(row_of(round + u))) *reinterpret_cast<Run<uint8_t, N>*>(g.positive + row_of(round + u) * g.nj + j) = pos;
                             }
                         activate<sizeof(T) == 2>(g.act, g.alpha, g.gain, v);
                         if constexpr (has_residual)
@@ -614,12 +640,58 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                         Run<T, N> out;
 #pragma unroll
                         for (int e = 0; e < N; e++) out.v[e] = rounded<T>(v[u * N + e]);
-                        *reinterpret_cast<Run<T, N>*>((T*)g.out + row_of(round + u) * g.nj + j) = out;
+                        if (there(row_of(round + u))) *reinterpret_cast<Run<T, N>*>((T*)g.out + row_of(round + u) * g.nj + j) = out;
                     }
                 }
             };
-            if (FORWARD && g.residual) rounds(std::true_type{});
-            else rounds(std::false_type{});
+            using Yes = std::true_type;
+            using No = std::false_type;
+            const bool edge = left_i < BI || left_j < BJ;
+            if (FORWARD && g.residual) edge ? rounds(Yes{}, Yes{}) : rounds(Yes{}, No{});
+            else edge ? rounds(No{}, Yes{}) : rounds(No{}, No{});
+        } else if (g.slices == 1) {
+            // Rows that start anywhere: a lane takes single elements, neighbouring lanes neighbouring columns.
+            constexpr int SETS = COLS > 64 ? COLS / 64 : 1, STRIDE = COLS > 64 ? 1 : 64 / COLS, U = 8;     // columns per lane; rows per round
+            static_assert(S_PASS * 16 % (STRIDE * U) == 0, "whole rounds");
+#pragma unroll 1
+            for (int set = 0; set < SETS; set++) {
+                const int col = set * 64 + (COLS > 64 ? lane : lane % COLS);
+                const int64_t jj = j0 + wj + col;
+                if (jj >= g.nj) continue;
+                const float bias = FORWARD && g.bias ? Elem<T>::load(((const T*)g.bias)[jj]) * g.b_gain : 0.f;
+#pragma unroll 1
+                for (int r0 = COLS > 64 ? 0 : lane / COLS; r0 < S_PASS * 16; r0 += STRIDE * U) {
+                    float v[U], res[U];
+                    int64_t at[U];
+                    bool there[U];
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const int row = r0 + u * STRIDE;
+                        const int64_t i = i0 + wi + FragA::row(s0 + row / 16, row % 16);
+                        there[u] = i < g.ni;
+                        at[u] = i * g.nj + jj;
+                        v[u] = chunk_at(row, col / 4)[col % 4] * g.scale + bias;
+                        if (FORWARD && g.residual) res[u] = Elem<T>::load(((const T*)g.residual)[(there[u] ? i : 0) * g.ldr + jj]);
+                    }
+                    if constexpr (FORWARD) {
+                        if (g.z)
+#pragma unroll
+                            for (int u = 0; u < U; u++)
+                                if (there[u]) g.z[at[u]] = v[u];
+                        if (g.positive)
+#pragma unroll
+                            for (int u = 0; u < U; u++)
+                                if (there[u]) g.positive[at[u]] = v[u] > 0.f;
+                        activate<sizeof(T) == 2>(g.act, g.alpha, g.gain, v);
+                        if (g.residual)
+#pragma unroll
+                            for (int u = 0; u < U; u++) v[u] += res[u];
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        if (there[u]) ((T*)g.out)[at[u]] = rounded<T>(v[u]);
+                }
+            }
         } else {
 #pragma unroll 1
             for (int round = 0; round < ROUNDS; round++) {
@@ -627,24 +699,14 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                 if (i >= g.ni || j >= g.nj) continue;
                 float v[N];
                 take(round, v);
-                if (g.slices > 1) {
-                    float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
-                    if (g.whole) {
+                float* out = g.partial + ((int64_t)slice * g.ni + i) * g.nj + j;
+                if (g.whole) {
 #pragma unroll
-                        for (int q = 0; q < N; q += 4) *reinterpret_cast<f32x4_t*>(out + q) = f32x4_t{v[q], v[q + 1], v[q + 2], v[q + 3]};
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < N; e++)
-                            if (j + e < g.nj) out[e] = v[e];
-                    }
-                } else if (g.whole) {
-                    finish<T, N, FORWARD>(g, i, j, v);
+                    for (int q = 0; q < N; q += 4) *reinterpret_cast<f32x4_t*>(out + q) = f32x4_t{v[q], v[q + 1], v[q + 2], v[q + 3]};
                 } else {
-#pragma unroll 1
-                    for (int e = 0; e < N && j + e < g.nj; e++) {
-                        float one[1] = {chunk_at(round * ROUND + row0, run * (N / 4) + e / 4)[e % 4]};
-                        finish<T, 1, FORWARD>(g, i, j + e, one);
-                    }
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (j + e < g.nj) out[e] = v[e];
                 }
             }
         }
@@ -930,9 +992,9 @@ Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
     return best;
 }
 
-template <class T, int TILE, bool RA, bool RB, bool DIRECT> void launch_gemm(const Gemm& g, hipStream_t stream) {
+template <class T, int TILE, bool RA, bool RB, int MODE> void launch_gemm(const Gemm& g, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices));
-    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, DIRECT>), grid, dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, MODE>), grid, dim3(256), 0, stream, g);
 }
 
 template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
@@ -959,15 +1021,22 @@ template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStr
         g.tiles_i = (int)((g.ni + 127) / 128);
         g.tiles_j = (int)((g.nj + 127) / 128);
     }
+    const bool is_short = (RA ? g.np : g.ni) < E || (RB ? g.np : g.nj) < E;
+    if (tile == 128 && is_short) {
+        tile = 64;
+        g.tiles_i = (int)((g.ni + 63) / 64);
+        g.tiles_j = (int)((g.nj + 63) / 64);
+    }
     SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
     if constexpr (ES == 2) {
-        if (tile == 256) launch_gemm<T, 256, RA, RB, true>(g, stream);
-        else if (tile == 128 && direct) launch_gemm<T, 128, RA, RB, true>(g, stream);
-        else if (tile == 128) launch_gemm<T, 128, RA, RB, false>(g, stream);
+        if (tile == 256) launch_gemm<T, 256, RA, RB, kDirect>(g, stream);
+        else if (tile == 128 && direct) launch_gemm<T, 128, RA, RB, kDirect>(g, stream);
+        else if (tile == 128) launch_gemm<T, 128, RA, RB, kLoose>(g, stream);
     }
     if (tile == 64) {
-        if (direct) launch_gemm<T, 64, RA, RB, true>(g, stream);
-        else launch_gemm<T, 64, RA, RB, false>(g, stream);
+        if (direct) launch_gemm<T, 64, RA, RB, kDirect>(g, stream);
+        else if (is_short) launch_gemm<T, 64, RA, RB, kShort>(g, stream);
+        else launch_gemm<T, 64, RA, RB, kLoose>(g, stream);
     }
     if (g.slices > 1) {
         const int run = g.whole ? 4 : 1;
