@@ -97,6 +97,11 @@ def differentiable_twice():
         _twice = old
 
 
+def composite_wanted():
+    """True inside differentiable_twice()."""
+    return _twice
+
+
 def _noise_plane(noise, dtype):
     return None if noise is None else noise.to(torch.float32).contiguous()
 

@@ -28,9 +28,11 @@ from ..torch_utils import misc
 from ..torch_utils import persistence
 from ..torch_utils.ops import bias_act
 from ..torch_utils.ops import conv2d_resample
+from ..torch_utils.ops import embedding
 from ..torch_utils.ops import fma
 from ..torch_utils.ops import styles as styles_op
 from ..torch_utils.ops import fused_layer
+from ..torch_utils.ops import linear
 from ..torch_utils.ops import minibatch_std
 from ..torch_utils.ops import upfirdn2d
 
@@ -449,6 +451,12 @@ def _modulated_layer(x, weight, styles, noise, noise_strength, bias, up, padding
                                   bias=bias, act=act, gain=gain, clamp=clamp, also_input=also_input)
 
 
+# Evaluate fully connected layers (mapping network, discriminator head) as one kernel that reads the parameters as they are
+# stored (torch_utils/ops/linear.py) instead of a library product of scaled copies followed by bias_act.  Off by default: the
+# sums run in another order, so results differ from the library's in the last bits of float32.
+FUSE_DENSE = os.environ.get('SG_FUSE_DENSE', '0') != '0'
+
+
 # ----------------------------------------------------------------------------
 
 @persistence.records_init
@@ -462,6 +470,9 @@ class FullyConnectedLayer(torch.nn.Module):
         self.bias_gain = lr_multiplier
 
     def forward(self, x):
+        if FUSE_DENSE and x.is_cuda and x.dtype == self.weight.dtype and not fused_layer.composite_wanted() \
+                and getattr(self, 'affine_weights_domain_modulation_parametrization', None) is None:
+            return linear.linear(x, self.weight, self.bias, act=self.activation, w_gain=self.weight_gain, b_gain=self.bias_gain)
         if getattr(self, 'affine_weights_domain_modulation_parametrization', None) is None:
             w = _prepared(self, self.weight, self.weight_gain, x.dtype, 'w')
         else:
@@ -568,15 +579,24 @@ class MappingNetwork(torch.nn.Module):
         if num_ws is not None and w_avg_beta is not None:
             self.register_buffer('w_avg', torch.zeros([w_dim]))
 
+    def _embedded(self, c):
+        """The label embedding of c [N, c_dim] (one-hot or any other weights of the classes), or of class numbers c [N] (int32 or
+        int64): the same layer as a lookup in its weight, bit for bit what the one-hot rows of those classes give."""
+        if c.dim() == 1 and c.dtype in (torch.int32, torch.int64) and c.is_cuda:
+            layer = self.embed
+            return embedding.embedding(c, layer.weight.t(), layer.bias, w_gain=layer.weight_gain, b_gain=layer.bias_gain)
+        misc.assert_shape(c, [None, self.c_dim])
+        return self.embed(c.to(torch.float32))
+
     def forward(self, z, c, truncation_psi=1, truncation_cutoff=None, skip_w_avg_update=False):
+        """c: [N, c_dim], or class numbers [N] (see _embedded); [N, 0] or anything without conditioning."""
         x = None
         with torch.autograd.profiler.record_function('input'):
             if self.z_dim > 0:
                 misc.assert_shape(z, [None, self.z_dim])
                 x = normalize_2nd_moment(z.to(torch.float32))
             if self.c_dim > 0:
-                misc.assert_shape(c, [None, self.c_dim])
-                y = normalize_2nd_moment(self.embed(c.to(torch.float32)))
+                y = normalize_2nd_moment(self._embedded(c))
                 x = torch.cat([x, y], dim=1) if x is not None else y
         for idx in range(self.num_layers):
             x = getattr(self, f'fc{idx}')(x)

@@ -104,8 +104,9 @@ FULL = dict(generator_requires_grad_parts=['all'], use_domain_modulation=False, 
 def setup_training_options(cfg='paper256', resolution=256, batch_size=None, num_gpus=1, batch_gpu=None,
                            generator_requires_grad_parts=('all',), use_domain_modulation=False,
                            domain_modulation_parametrization=None, glrate=None, dlrate=None, gamma=None, fp32=False,
-                           mbstd=None, c_dim=0, freezed=None):
-    """Keyword arguments for `Trainer` the way the reference's `train.py` derives them from its flags."""
+                           mbstd=None, c_dim=0, freezed=None, max_grad_norm=None):
+    """Keyword arguments for `Trainer` the way the reference's `train.py` derives them from its flags.  `max_grad_norm` (not one
+    of its flags): both optimizers clip by the global norm of the gradients of each step."""
     spec = dict(CFG_SPECS[cfg])
     batch_size = spec['mb'] if batch_size is None else batch_size
     batch_gpu = batch_size // num_gpus if batch_gpu is None else batch_gpu
@@ -123,9 +124,10 @@ def setup_training_options(cfg='paper256', resolution=256, batch_size=None, num_
                     epilogue_kwargs=dict(mbstd_group_size=min(spec['mbstd'] if mbstd is None else mbstd, batch_gpu)))
     lr_g = spec['lrate'] if glrate is None else glrate
     lr_d = spec['lrate'] if dlrate is None else dlrate
+    clip = {} if max_grad_norm is None else dict(max_grad_norm=max_grad_norm)
     return dict(
         G_kwargs=G_kwargs, D_kwargs=D_kwargs,
-        G_opt_kwargs=dict(lr=lr_g, betas=[0, 0.99], eps=1e-8), D_opt_kwargs=dict(lr=lr_d, betas=[0, 0.99], eps=1e-8),
+        G_opt_kwargs=dict(lr=lr_g, betas=[0, 0.99], eps=1e-8, **clip), D_opt_kwargs=dict(lr=lr_d, betas=[0, 0.99], eps=1e-8, **clip),
         loss_kwargs=dict(r1_gamma=spec['gamma'] if gamma is None else gamma),
         batch_size=batch_size, batch_gpu=batch_gpu, num_gpus=num_gpus, ema_kimg=spec['ema'], ema_rampup=spec['ramp'],
         requires_grad_parts={'Gboth': parts, 'Gmain': parts, 'Greg': parts, 'Dboth': ['all'], 'Dmain': ['all'], 'Dreg': ['all']})
@@ -513,7 +515,8 @@ class Trainer:
     # -- one iteration ----------------------------------------------------------
     def step(self, real_img, real_c, gen_z=None, gen_c=None):
         """real_img: this rank's share, uint8 [n, C, H, W] (or float already in [-1, 1]).  gen_z / gen_c: latents and
-        labels of the generated images, [phases * n, ...] (one run of n per phase).  The reference draws every
+        labels of the generated images, [phases * n, ...] (one run of n per phase).  Labels are rows [n, c_dim] or class
+        numbers [n] (int32 or int64; real_c and gen_c alike).  The reference draws every
         generated label from a random item of the dataset (training_loop.py:364-366); a caller with a label table
         passes such draws as gen_c.  Without gen_c the labels of this real batch are resampled with replacement,
         independently for every phase."""
@@ -531,7 +534,7 @@ class Trainer:
             all_gen_z = [z.split(self.batch_gpu) for z in gen_z.split(n_rank)]
             if gen_c is None:
                 gen_c = real_c.to(self.device)
-                if gen_c.shape[1] > 0:
+                if gen_c.dim() == 1 or gen_c.shape[1] > 0:
                     gen_c = gen_c[torch.randint(gen_c.shape[0], [len(self.phases) * n_rank], device=self.device)]
                 else:
                     gen_c = gen_c.new_zeros([len(self.phases) * n_rank, 0])
