@@ -350,6 +350,24 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
 // Tile BI x BJ per workgroup of WI x WJ waves.  How operands travel: kDirect, rows of both are whole aligned 16-byte packets;
 // kLoose, rows start anywhere and end anywhere; kShort, rows of one of them are shorter than 16 bytes.  Products of
 // two "rows" operands are the forward pass and carry its epilogue.
+// c += a b, written as assembly for the one thing the builtin does not say: c is read and written in place, in accumulation
+// registers.  (With 256 of them a lane the register allocator otherwise moves accumulators about, up to 448 moves in a step of 128
+// products: 400 us instead of 240 for 8192 x 4096 -> 4096.)  Products of one accumulator are at least a tile row apart, and settle()
+// is the wait before anything else reads them.
+__device__ __forceinline__ void mfma_in_place(f32x4_t& c, const uint4& a, const uint4& b, __hip_bfloat16) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(bf16x8_t, a)), "v"(__builtin_bit_cast(bf16x8_t, b)));
+}
+__device__ __forceinline__ void mfma_in_place(f32x4_t& c, const uint4& a, const uint4& b, __half) {
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(f16x8_t, a)), "v"(__builtin_bit_cast(f16x8_t, b)));
+}
+template <int M, int N> __device__ __forceinline__ void settle(f32x4_t (&acc)[M][N]) {
+    asm volatile("s_nop 15\n\ts_nop 15");               // more than the passes of a 16 x 16 x 32 product
+#pragma unroll
+    for (int t = 0; t < M; t++)
+#pragma unroll
+        for (int s = 0; s < N; s++) asm volatile("" : "+a"(acc[t][s]));
+}
+
 enum { kDirect, kLoose, kShort };
 
 template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
@@ -401,7 +419,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
 #pragma unroll
         for (int s = 0; s < TI; s++) {
             if constexpr (sizeof(T) == 2) {
-                acc[t][s] = mfma(fb.q[t], fa.q[s], acc[t][s], T());
+                mfma_in_place(acc[t][s], fb.q[t], fa.q[s], T());
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb.value(t, e), fa.value(s, e), acc[t][s], 0, 0, 0);
@@ -418,9 +436,9 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         constexpr int PARTS = TI > TJ ? TI : TJ;
         FragA fa[2];
         FragB fb[2];
-        // share `part` of PARTS of the copies of step n
+        // share `part` of PARTS of the copies of step n (of one behind the last step: zeros, which nothing reads)
         auto copy_part = [&](i32x4_t from_a, i32x4_t from_b, int n, int part) {
-            const int left = left_p(first + n);
+            const int left = n < steps ? left_p(first + n) : 0;
             const unsigned to = lds + (n & 1) * BUF;
 #pragma unroll
             for (int k = 0; k < TileA::LOADS; k++)
@@ -444,7 +462,17 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
             for (int t = 0; t < TJ; t++)
                 if (t * READ_PARTS / TJ == part) fb[set].read(from + TileA::BYTES, wj, kk, t);
         };
-        auto step = [&](int n, auto copies, auto more) {           // copies: step n + 2 exists; more: step n + 1 does
+        if (steps > 0) {
+            copy_all(0);
+            copies_landed();
+            __syncthreads();
+            copy_all(1);
+            fa[0].read(smem, wi, 0);
+            fb[0].read(smem + TileA::BYTES, wj, 0);
+        }
+        // One body for every step: the last two read and copy what does not exist.
+#pragma unroll 1
+        for (int n = 0; n < steps; n++) {
             const unsigned char* now = smem + (n & 1) * BUF;
             const unsigned char* next = smem + (~n & 1) * BUF;
 #pragma unroll
@@ -453,36 +481,17 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
                 if (t < TJ) multiply_tile(fa[0], fb[0], t);
                 __builtin_amdgcn_sched_barrier(0);        // (or the reads gather behind the products)
             }
-            if constexpr (more) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            }
-            i32x4_t from_a{}, from_b{};
-            if constexpr (copies) {
-                from_a = descriptor(at_a(first + n + 2));
-                from_b = descriptor(at_b(first + n + 2));
-            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const i32x4_t from_a = descriptor(at_a(first + n + 2)), from_b = descriptor(at_b(first + n + 2));
 #pragma unroll
             for (int t = 0; t < PARTS; t++) {
-                if constexpr (copies) copy_part(from_a, from_b, n + 2, t);
-                if constexpr (more) read_part(0, next, 0, t);
+                copy_part(from_a, from_b, n + 2, t);
+                read_part(0, next, 0, t);
                 if (t < TJ) multiply_tile(fa[1], fb[1], t);
                 __builtin_amdgcn_sched_barrier(0);
             }
-        };
-        constexpr auto yes = std::true_type{};
-        constexpr auto no = std::false_type{};
-        if (steps > 0) {
-            copy_all(0);
-            copies_landed();
-            __syncthreads();
-            if (steps > 1) copy_all(1);
-            fa[0].read(smem, wi, 0);
-            fb[0].read(smem + TileA::BYTES, wj, 0);
-            int n = 0;
-            for (; n + 2 < steps; n++) step(n, yes, yes);
-            if (n + 1 < steps) step(n++, no, yes);
-            step(n, no, no);
         }
+        copies_landed();                                  // (the epilogue writes where they go)
     } else {
         // Two LDS buffers and two sets of registers: a step's loads have the two steps before it to arrive; one barrier a step.
         // Steps go in pairs and every step loads, the last ones their own data again (behind a branch the compiler would wait
@@ -528,6 +537,8 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         }
     }
 
+    if constexpr (sizeof(T) == 2) settle(acc);
+
     // acc[t][s][r]: row i = tile s of A at lane % 16, column j = tile t of B at 4 * (lane / 16) + r.  Each wave lays its part
     // down in LDS as rows of four-column chunks (chunk c of row r at c ^ r: the 16 rows a store touches lie in 16 different
     // 16-byte banks) and takes it up again in runs of consecutive columns: stores of 16 bytes, and one copy of the
@@ -540,31 +551,33 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     float* mine = reinterpret_cast<float*>(smem) + wave * (S_PASS * 16 * COLS);
     auto chunk_at = [&](int row, int chunk) -> f32x4_t& { return *reinterpret_cast<f32x4_t*>(mine + row * COLS + (chunk ^ (row & (CHUNKS - 1))) * 4); };
     __syncthreads();                                                     // every wave is done with the tiles
+    auto lay_down = [&](int s, int row) {                                 // A tile s, constant, as the region's rows from `row` on
 #pragma unroll
+        for (int t = 0; t < TJ; t++) {
+            if constexpr (FragB::V == 1) {
+                chunk_at(row, t * 4 + quad) = acc[t][s];
+            } else if constexpr (FragB::V == 4) {                        // tiles t .. t + 3 hold consecutive columns
+                if (t % 4 == 0)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        chunk_at(row, t / 4 * 16 + quad * 4 + r) = f32x4_t{acc[t][s][r], acc[t + 1][s][r], acc[t + 2][s][r], acc[t + 3][s][r]};
+            } else {
+                static_assert(FragB::V == 2 || FragB::V == 1 || FragB::V == 4, "interleaved tiles");
+                if (t % 2 == 0)
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2)
+                        chunk_at(row, t / 2 * 8 + quad * 2 + r / 2) = f32x4_t{acc[t][s][r], acc[t + 1][s][r], acc[t][s][r + 1], acc[t + 1][s][r + 1]};
+            }
+        }
+    };
+    // (one copy of the code behind lay_down for all passes; accumulators are picked by constants, or they would move to memory)
+#pragma unroll 1
     for (int s0 = 0; s0 < TI; s0 += S_PASS) {
 #pragma unroll
-        for (int s = 0; s < S_PASS; s++)
+        for (int pass = 0; pass < TI / S_PASS; pass++)
+            if (s0 == pass * S_PASS)
 #pragma unroll
-            for (int t = 0; t < TJ; t++) {
-                const f32x4_t(&c)[TI] = acc[t];
-                const int row = s * 16 + l16;
-                if constexpr (FragB::V == 1) {
-                    chunk_at(row, t * 4 + quad) = c[s0 + s];
-                } else if constexpr (FragB::V == 4) {                    // tiles t .. t + 3 hold consecutive columns
-                    if (t % 4 == 0)
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            chunk_at(row, t / 4 * 16 + quad * 4 + r) =
-                                f32x4_t{acc[t][s0 + s][r], acc[t + 1][s0 + s][r], acc[t + 2][s0 + s][r], acc[t + 3][s0 + s][r]};
-                } else {
-                    static_assert(FragB::V == 2 || FragB::V == 1 || FragB::V == 4, "interleaved tiles");
-                    if (t % 2 == 0)
-#pragma unroll
-                        for (int r = 0; r < 4; r += 2)
-                            chunk_at(row, t / 2 * 8 + quad * 2 + r / 2) =
-                                f32x4_t{acc[t][s0 + s][r], acc[t + 1][s0 + s][r], acc[t][s0 + s][r + 1], acc[t + 1][s0 + s][r + 1]};
-                }
-            }
+                for (int s = 0; s < S_PASS; s++) lay_down(pass * S_PASS + s, s * 16 + l16);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         // 64 / RUNS rows at a time; a lane keeps its columns.
         constexpr int ROUND = 64 / RUNS, ROUNDS = S_PASS * 16 / ROUND;
@@ -955,16 +968,18 @@ bool thin_fits(int dtype, bool rows_b, int64_t ni, int64_t nj, int64_t np) {
 }
 
 // The tile and the number of slices with the least predicted time.  Measured on MI355X, us per step (128 bytes along p) of a
-// workgroup that has a CU to itself / of each of several that share one, by the number of "columns" operands:
-//   16-bit  64 x 64: 0.25 / 0.18, 0.28 / 0.18, 0.31 / 0.20     128 x 128: 0.69 / 0.45, 0.69 / 0.47, 0.82 / 0.59     256 x 256: 1.8, 1.63, 1.61
-//   float32 64 x 64: 0.62 / 0.50, whichever                     (a 128 x 128 tile takes four times that: not built)
-// 3 us for a launch and its ends; slices cost a second launch and a round trip of their float32 sums at 6 TB/s.
-// 1024^3 in bfloat16: 64 x 64 tiles 6.9 us, 128 x 128 11.5; 4096^3: 256 x 256 106, 128 x 128 122, 64 x 64 190; a weight gradient of
-// 2048 x 2048 over 8192 rows: 256 x 256 in four slices 76, 128 x 128 106.
+// workgroup that has a CU to itself / of each of several that share one, by the number of "columns" operands, and us for the ends
+// of a tile (first copies, epilogue) that nothing overlaps:
+//   16-bit  64 x 64: 0.27 / 0.18, 0.29 / 0.18, 0.31 / 0.20, 0.4     128 x 128: 0.75 / 0.48, 0.75 / 0.50, 0.82 / 0.52, 1.2     256 x 256: 1.62 each, 5
+//   float32 64 x 64: 0.62 / 0.50, whichever, 0.4                 (a 128 x 128 tile takes four times that: not built)
+// 3 us for a launch; slices cost a second launch and a round trip of their float32 sums at 6 TB/s.
+// 1024^3 in bfloat16: 64 x 64 tiles 7 us, 128 x 128 12; 4096^3: 256 x 256 109 us (1257 TFLOP/s), 128 x 128 125, 64 x 64 182; a weight
+// gradient of 2048 x 2048 over 8192 rows: 256 x 256 in four slices 76, 128 x 128 97.
 Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
-    struct Kind { int tile; double alone[3], shared[3]; };
-    static const Kind kinds[] = {{64, {0.25, 0.28, 0.31}, {0.18, 0.18, 0.20}}, {128, {0.69, 0.69, 0.82}, {0.45, 0.47, 0.59}}, {256, {1.8, 1.63, 1.61}, {1.8, 1.63, 1.61}}};
-    static const Kind kinds32[] = {{64, {0.62, 0.62, 0.62}, {0.50, 0.50, 0.50}}};
+    struct Kind { int tile; double alone[3], shared[3], ends; };
+    static const Kind kinds[] = {{64, {0.27, 0.29, 0.31}, {0.18, 0.18, 0.20}, 0.4}, {128, {0.75, 0.75, 0.82}, {0.48, 0.50, 0.52}, 1.2},
+                                 {256, {1.62, 1.62, 1.62}, {1.62, 1.62, 1.62}, 5.0}};
+    static const Kind kinds32[] = {{64, {0.62, 0.62, 0.62}, {0.50, 0.50, 0.50}, 0.4}};
     Shape best;
     best.thin = columns < 2 && thin_fits(dtype, columns == 0, ni, nj, np);
     const int bk = dtype == SG_F32 ? 32 : 64;
@@ -977,7 +992,7 @@ Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
             const int64_t each = (steps + slices - 1) / slices, used = (steps + each - 1) / each;
             const int64_t per_cu = (ti * tj * used + 255) / 256;
             const double step = std::max(kind.alone[columns], kind.shared[columns] * (double)per_cu);
-            const double us = 3 + (double)each * step + (used > 1 ? 4 + (double)used * ni * nj * 8 / 6e6 : 0);
+            const double us = 3 + (double)each * step + kind.ends * (double)per_cu + (used > 1 ? 4 + (double)used * ni * nj * 8 / 6e6 : 0);
             if (best.tile == 0 || us < best_us) {
                 best_us = us;
                 best.tile = kind.tile;
