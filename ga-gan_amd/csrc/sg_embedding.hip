@@ -302,53 +302,54 @@ __global__ void __launch_bounds__(256) sort_count_kernel(IndexView index, const 
 }
 
 // Second half: every token to its place.  A place is (tokens of smaller digits) + (equal digits of earlier blocks, of earlier
-// rounds and waves of this block, of earlier lanes).
-__global__ void __launch_bounds__(256) sort_place_kernel(IndexView index, const unsigned* __restrict__ keys, const unsigned* __restrict__ ids,
-                                                         int64_t tokens, int64_t v, int shift, int64_t share, const int* __restrict__ counts,
-                                                         unsigned* __restrict__ keys_out, unsigned* __restrict__ ids_out) {
-    constexpr int ITEMS = 4, WAVES = 4, ROUND = ITEMS * 256;
+// rounds and waves of this block, of earlier lanes).  Sixteen waves: the table of counts is read by four threads a digit.
+__global__ void __launch_bounds__(1024) sort_place_kernel(IndexView index, const unsigned* __restrict__ keys, const unsigned* __restrict__ ids,
+                                                          int64_t tokens, int64_t v, int shift, int64_t share, const int* __restrict__ counts,
+                                                          unsigned* __restrict__ keys_out, unsigned* __restrict__ ids_out) {
+    constexpr int WAVES = 16, ROUND = 1024;
     __shared__ int count[WAVES][256];
     __shared__ int scratch[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, digit_of_thread = threadIdx.x & 255, quarter = threadIdx.x >> 8;
     const int blocks = gridDim.x;
     int earlier = 0, total = 0;
 #pragma unroll 8
-    for (int b = 0; b < blocks; b++) {
-        const int c = counts[b * 256 + threadIdx.x];
+    for (int b = quarter; b < blocks; b += 4) {
+        const int c = counts[b * 256 + digit_of_thread];
         earlier += b < (int)blockIdx.x ? c : 0;
         total += c;
     }
-    int next = scan256(total, scratch) + earlier;         // place of the block's next token with digit threadIdx.x
+    count[quarter][digit_of_thread] = total;
+    count[4 + quarter][digit_of_thread] = earlier;
+    __syncthreads();
+    if (threadIdx.x < 256) {
+        total = count[0][threadIdx.x] + count[1][threadIdx.x] + count[2][threadIdx.x] + count[3][threadIdx.x];
+        earlier = count[4][threadIdx.x] + count[5][threadIdx.x] + count[6][threadIdx.x] + count[7][threadIdx.x];
+    }
+    int next = scan256(threadIdx.x < 256 ? total : 0, scratch) + earlier;     // threads 0 .. 255: place of the block's next token with that digit
     const int64_t first = (int64_t)blockIdx.x * share, last = first + share < tokens ? first + share : tokens;
     for (int64_t at0 = first; at0 < last; at0 += ROUND) {
-        for (int w = 0; w < WAVES; w++) count[w][threadIdx.x] = 0;
+        for (int i = threadIdx.x; i < WAVES * 256; i += 1024) (&count[0][0])[i] = 0;
         __syncthreads();
-        unsigned key[ITEMS], id[ITEMS], digit[ITEMS];
-        bool valid[ITEMS];
-        int rank[ITEMS];
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int64_t at = at0 + (wave * ITEMS + i) * 64 + lane;
-            valid[i] = at < last;
-            key[i] = valid[i] ? (keys ? keys[at] : key_of(index.at(at), v)) : 0;
-            id[i] = valid[i] ? (ids ? ids[at] : (unsigned)at) : 0;
-            digit[i] = (key[i] >> shift) & 255;
-        }
-        wave_ranks<ITEMS>(digit, valid, count[wave], rank);
+        const int64_t at = at0 + threadIdx.x;
+        const bool valid[1] = {at < last};
+        const unsigned key = valid[0] ? (keys ? keys[at] : key_of(index.at(at), v)) : 0;
+        const unsigned id = valid[0] ? (ids ? ids[at] : (unsigned)at) : 0;
+        const unsigned digit[1] = {(key >> shift) & 255};
+        int rank[1];
+        wave_ranks<1>(digit, valid, count[wave], rank);
         __syncthreads();
-        for (int w = 0; w < WAVES; w++) {
-            const int c = count[w][threadIdx.x];
-            count[w][threadIdx.x] = next;
-            next += c;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++)
-            if (valid[i]) {
-                const int to = count[wave][digit[i]] + rank[i];
-                keys_out[to] = key[i];
-                ids_out[to] = id[i];
+        if (threadIdx.x < 256)
+            for (int w = 0; w < WAVES; w++) {
+                const int c = count[w][threadIdx.x];
+                count[w][threadIdx.x] = next;
+                next += c;
             }
+        __syncthreads();
+        if (valid[0]) {
+            const int to = count[wave][digit[0]] + rank[0];
+            keys_out[to] = key;
+            ids_out[to] = id;
+        }
         __syncthreads();
     }
 }
@@ -442,50 +443,81 @@ __global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const RunParam
     flush(key == key_after);
 }
 
-// Runs that cross spans: the workgroup of the span a run begins in adds the later spans' partial sums to its own, the waves
-// taking consecutive shares, and the shares are added in wave order.
-template <class T>
-__global__ void __launch_bounds__(512) embedding_grad_join_kernel(const RunParams p, int tiles64) {
+// Runs that cross spans: the workgroup of the span a run begins in adds the later spans' partial sums to its own.  A wave takes 64 * N
+// features; where that leaves waves over, 2, 4 or 8 of them take consecutive shares of the spans, which are added in their order.
+template <class T, int N>
+__global__ void __launch_bounds__(512) embedding_grad_join_kernel(const RunParams p) {
     constexpr int WAVES = 8;
-    __shared__ float part[WAVES][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int span = blockIdx.x / tiles64, tile = blockIdx.x % tiles64;
+    __shared__ float part[WAVES][64 * N];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int span = blockIdx.x;
     const int64_t p0 = (int64_t)span * p.span, end = p0 + p.span;
     if (end >= p.tokens) return;                                       // the last span: nothing goes on
     const unsigned key = p.keys[end - 1];
     if (key >= (unsigned)p.v || p.keys[end] != key) return;            // the run ends here
     if (p.keys[p0] == key && p0 > 0 && p.keys[p0 - 1] == key) return;  // it began earlier
     // the last span the run reaches: the largest j for which position (span + j) * p.span still holds the key (sorted, so
-    // 64 probes at a time find it in three rounds up to 2^18 spans)
+    // 64 probes at a time find it in three rounds up to 2^18 spans; most runs end within the first 64)
     int reach = 1;
-    for (int step = 4096; step >= 1; step /= 64)
+    auto probe = [&](int step) {
         for (;;) {
             const int64_t at = (int64_t)(span + reach + (int64_t)step * (lane + 1)) * p.span;
             const uint64_t in = __ballot(at < p.tokens && p.keys[at < p.tokens ? at : 0] == key);
             const int more = in == ~0ull ? 64 : __ffsll((unsigned long long)~in) - 1;
             reach += step * more;
-            if (more < 64) break;
+            if (more < 64) return more;
         }
-    const int64_t f = (int64_t)tile * 64 + lane;
-    const bool inside = f < p.f;
-    const int each = (reach + WAVES - 1) / WAVES;
-    const int a = wave * each, b = a + each < reach ? a + each : reach;
-    const float* src = p.partial + (int64_t)(span + 1) * 2 * p.f + (inside ? f : 0);
-    float sum = wave == 0 ? p.partial[((int64_t)span * 2 + 1) * p.f + (inside ? f : 0)] : 0.f;
-    for (int i = a; i < b; i += 8) {
-        float g[8];
-#pragma unroll
-        for (int u = 0; u < 8; u++) g[u] = i + u < b ? src[(int64_t)(i + u) * 2 * p.f] : 0.f;
-#pragma unroll
-        for (int u = 0; u < 8; u++) sum += g[u];
+    };
+    const int64_t far = (int64_t)(span + reach + 64) * p.span;
+    if (far < p.tokens && p.keys[far] == key) {
+        probe(4096);
+        probe(64);
     }
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave == 0 && inside) {
-        sum = 0.f;
+    probe(1);
+    const int tiles = (int)((p.f + 64 * N - 1) / (64 * N));
+    const int shares = tiles >= 8 ? 1 : tiles >= 4 ? 2 : tiles >= 2 ? 4 : 8;
+    const int mine = wave % shares, each = (reach + shares - 1) / shares;
+    const int a = mine * each, b = a + each < reach ? a + each : reach;
+    for (int tile0 = 0; tile0 < tiles; tile0 += WAVES / shares) {       // (the same number of turns for every wave)
+        const int64_t f = ((int64_t)(tile0 + wave / shares) * 64 + lane) * N;
+        const bool inside = f < p.f;
+        const float* src = p.partial + (int64_t)(span + 1) * 2 * p.f + (inside ? f : 0);
+        const float* own = p.partial + ((int64_t)span * 2 + 1) * p.f + (inside ? f : 0);
+        float sum[N];
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) sum += part[w][lane];
-        ((T*)p.dtable)[(int64_t)key * p.stride_v + f * p.stride_f] = Elem<T>::store(sum * p.w_gain);
+        for (int j = 0; j < N; j++) sum[j] = mine == 0 ? own[j] : 0.f;
+        for (int i = a; i < b; i += 4) {
+            float g[4][N];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int j = 0; j < N; j++) g[u][j] = src[(int64_t)(i + u < b ? i + u : a) * 2 * p.f + j];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int j = 0; j < N; j++) sum[j] += i + u < b ? g[u][j] : 0.f;
+        }
+        if (shares > 1) {
+#pragma unroll
+            for (int j = 0; j < N; j++) part[wave][j * 64 + lane] = sum[j];
+            __syncthreads();
+            if (mine == 0)
+                for (int w = 1; w < shares; w++)
+#pragma unroll
+                    for (int j = 0; j < N; j++) sum[j] += part[wave + w][j * 64 + lane];
+            __syncthreads();
+        }
+        if (mine == 0 && inside) {
+            T* out = (T*)p.dtable + (int64_t)key * p.stride_v + f * p.stride_f;
+            if constexpr (N > 1) {
+                Pack<T> q;
+#pragma unroll
+                for (int j = 0; j < N; j++) q.v[j] = Elem<T>::store(sum[j] * p.w_gain);
+                store_pack(out, q);
+            } else {
+                *out = Elem<T>::store(sum[0] * p.w_gain);
+            }
+        }
     }
 }
 
@@ -622,7 +654,7 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
             unsigned** out = pass & 1 ? b : a;
             hipLaunchKernelGGL(sort_count_kernel, dim3(g.sort_blocks + (pass == 0 ? (unsigned)zero_blocks : 0)), dim3(256), 0, stream, index, k_in,
                                p->tokens, p->v, 8 * pass, g.share, g.sort_blocks, counts, dtable, zero_bytes);
-            hipLaunchKernelGGL(sort_place_kernel, dim3(g.sort_blocks), dim3(256), 0, stream, index, k_in, i_in, p->tokens, p->v, 8 * pass, g.share,
+            hipLaunchKernelGGL(sort_place_kernel, dim3(g.sort_blocks), dim3(1024), 0, stream, index, k_in, i_in, p->tokens, p->v, 8 * pass, g.share,
                                counts, out[0], out[1]);
             const int done = check_launch("sg_embedding_backward");
             if (done != SG_OK) return done;
@@ -635,12 +667,15 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
     const int tiles = (int)((p->f + 64 * n - 1) / (64 * n));
     const RunParams r{keys, perm, dy, dtable, (float*)(ws + g.partial), p->tokens, p->v, p->f, p->stride_v, p->stride_f, p->w_gain, g.span, g.spans, tiles};
     const int64_t items = (int64_t)g.spans * tiles;
-    const int tiles64 = (int)((p->f + 63) / 64);
-    SG_REQUIRE((items + 3) / 4 <= INT32_MAX && (int64_t)g.spans * tiles64 <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "embedding_backward: too many elements");
+    SG_REQUIRE((items + 3) / 4 <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "embedding_backward: too many elements");
     SG_DISPATCH_16_32(p->dtype, {
-        if (packed) hipLaunchKernelGGL((embedding_grad_runs_kernel<T, Pack<T>::N>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
-        else hipLaunchKernelGGL((embedding_grad_runs_kernel<T, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
-        hipLaunchKernelGGL((embedding_grad_join_kernel<T>), dim3((unsigned)(g.spans * tiles64)), dim3(512), 0, stream, r, tiles64);
+        if (packed) {
+            hipLaunchKernelGGL((embedding_grad_runs_kernel<T, Pack<T>::N>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
+            hipLaunchKernelGGL((embedding_grad_join_kernel<T, Pack<T>::N>), dim3((unsigned)g.spans), dim3(512), 0, stream, r);
+        } else {
+            hipLaunchKernelGGL((embedding_grad_runs_kernel<T, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
+            hipLaunchKernelGGL((embedding_grad_join_kernel<T, 1>), dim3((unsigned)g.spans), dim3(512), 0, stream, r);
+        }
     });
     const int done = check_launch("sg_embedding_backward");
     if (done != SG_OK || dbias == nullptr) return done;

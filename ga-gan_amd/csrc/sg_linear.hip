@@ -810,16 +810,15 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
     float v[RUN];
 #pragma unroll
     for (int e = 0; e < RUN; e++) v[e] = 0.f;
-    for (int s = 0; s < g.slices; s += 4) {
-        Run<float, RUN> q[4];
+    constexpr int AHEAD = 8;              // loads under way (slices behind the last read it again and count as nothing)
+    for (int s = 0; s < g.slices; s += AHEAD) {
+        Run<float, RUN> q[AHEAD];
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (s + u < g.slices) q[u] = *reinterpret_cast<const Run<float, RUN>*>(g.partial + (int64_t)(s + u) * plane + k);
+        for (int u = 0; u < AHEAD; u++) q[u] = *reinterpret_cast<const Run<float, RUN>*>(g.partial + (int64_t)min(s + u, g.slices - 1) * plane + k);
 #pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (s + u < g.slices)
+        for (int u = 0; u < AHEAD; u++)
 #pragma unroll
-                for (int e = 0; e < RUN; e++) v[e] += q[u].v[e];
+            for (int e = 0; e < RUN; e++) v[e] += s + u < g.slices ? q[u].v[e] : 0.f;
     }
     finish<T, RUN, FORWARD>(g, k / g.nj, k % g.nj, v);
 }
@@ -842,47 +841,49 @@ struct SlopeParams {
 };
 
 // A workgroup: 64 * N columns (N: elements per lane, one 16-byte packet or a single one), rows_per_block rows, the waves taking
-// every fourth row.
-template <class T, int N>
+// every fourth row, UNROLL of them requested at a time (rows behind the last read it again and count as nothing).  BY: where the
+// slope comes from.
+enum { kByNothing, kByY, kByPositive, kByZ };
+
+template <class T, int N, int BY>
 __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) {
-    constexpr int UNROLL = 4;
+    constexpr int UNROLL = BY == kByZ && N == 8 ? 4 : 8;
     __shared__ float part[4][64 * N];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * N;
-    const bool inside = c < p.cols;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
     float sum[N];
 #pragma unroll
     for (int e = 0; e < N; e++) sum[e] = 0.f;
-    for (int64_t r = r0 + wave; r < r1; r += 4 * UNROLL) {
-        Run<T, N> dy[UNROLL], y[UNROLL];
-        Run<uint8_t, N> pos[UNROLL];
-        Run<float, N> z[UNROLL];
+    if (c < p.cols) {
+        for (int64_t r = r0 + wave; r < r1; r += 4 * UNROLL) {
+            Run<T, N> dy[UNROLL], y[UNROLL];
+            Run<uint8_t, N> pos[UNROLL];
+            Run<float, N> z[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const int64_t row = r + 4 * u;
-            if (!inside || row >= r1) continue;
-            dy[u] = *reinterpret_cast<const Run<T, N>*>((const T*)p.dy + row * p.ld + c);
-            const int64_t at = row * p.cols + c;
-            if (p.y) y[u] = *reinterpret_cast<const Run<T, N>*>((const T*)p.y + at);
-            if (p.positive) pos[u] = *reinterpret_cast<const Run<uint8_t, N>*>(p.positive + at);
-            if (p.z) z[u] = *reinterpret_cast<const Run<float, N>*>(p.z + at);
-        }
-#pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const int64_t row = r + 4 * u;
-            if (!inside || row >= r1) continue;
-            Run<T, N> out;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                float s = Elem<T>::load(dy[u].v[e]);
-                if (p.y) s = Elem<T>::load(y[u].v[e]) * p.sign > 0.f ? s : s * p.alpha;
-                else if (p.positive) s = pos[u].v[e] ? s : s * p.alpha;
-                else if (p.z) s *= slope_at<sizeof(T) == 2>(p.act, z[u].v[e]);
-                sum[e] += s;
-                out.v[e] = rounded<T>(s);
+            for (int u = 0; u < UNROLL; u++) {
+                const int64_t row = min(r + 4 * u, r1 - 1), at = row * p.cols + c;
+                dy[u] = *reinterpret_cast<const Run<T, N>*>((const T*)p.dy + row * p.ld + c);
+                if constexpr (BY == kByY) y[u] = *reinterpret_cast<const Run<T, N>*>((const T*)p.y + at);
+                if constexpr (BY == kByPositive) pos[u] = *reinterpret_cast<const Run<uint8_t, N>*>(p.positive + at);
+                if constexpr (BY == kByZ) z[u] = *reinterpret_cast<const Run<float, N>*>(p.z + at);
             }
-            if (p.s) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.cols + c) = out;
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const int64_t row = r + 4 * u;
+                const bool there = row < r1;
+                Run<T, N> out;
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    float s = Elem<T>::load(dy[u].v[e]);
+                    if constexpr (BY == kByY) s = Elem<T>::load(y[u].v[e]) * p.sign > 0.f ? s : s * p.alpha;
+                    if constexpr (BY == kByPositive) s = pos[u].v[e] ? s : s * p.alpha;
+                    if constexpr (BY == kByZ) s *= slope_at<sizeof(T) == 2>(p.act, z[u].v[e]);
+                    sum[e] += there ? s : 0.f;
+                    out.v[e] = rounded<T>(s);
+                }
+                if (p.s && there) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.cols + c) = out;
+            }
         }
     }
     if (p.sums == nullptr) return;
@@ -893,7 +894,7 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
         const int64_t col = (int64_t)blockIdx.x * 64 * N + k;
         if (col >= p.cols) break;
         const float total = (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
-        if (gridDim.y == 1) ((T*)p.sums)[col] = Elem<T>::store(total * p.scale);
+        if (gridDim.y == 1) ((T*)p.sums)[col] = rounded<T>(total * p.scale);
         else p.partial[(int64_t)blockIdx.y * p.cols + col] = total;
     }
 }
@@ -947,8 +948,16 @@ template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* 
     const int64_t bx = (p.cols + 64 * n - 1) / (64 * n), by = p.rows == 0 ? 1 : slope_blocks(p.rows, p.cols);
     SG_REQUIRE(bx <= INT32_MAX && by <= 65535, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
     const dim3 grid((unsigned)bx, (unsigned)by);
-    if (packed) hipLaunchKernelGGL((linear_slope_kernel<T, N>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((linear_slope_kernel<T, 1>), grid, dim3(256), 0, stream, p);
+#define SG_SLOPE(BY)                                                                                                    \
+    do {                                                                                                                \
+        if (packed) hipLaunchKernelGGL((linear_slope_kernel<T, N, BY>), grid, dim3(256), 0, stream, p);                 \
+        else hipLaunchKernelGGL((linear_slope_kernel<T, 1, BY>), grid, dim3(256), 0, stream, p);                        \
+    } while (0)
+    if (p.y) SG_SLOPE(kByY);
+    else if (p.positive) SG_SLOPE(kByPositive);
+    else if (p.z) SG_SLOPE(kByZ);
+    else SG_SLOPE(kByNothing);
+#undef SG_SLOPE
     if (p.sums && by > 1)
         hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((p.cols + 63) / 64)), dim3(1024), 0, stream, p.partial, (int)by, p.cols, p.scale, (T*)p.sums);
     return check_launch(what);
