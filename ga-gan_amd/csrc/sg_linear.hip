@@ -3,7 +3,7 @@
 //   s = dy * act'(z)      dx = s w * (gain w_gain)    dw = s^T x * (gain w_gain)    db = sum over rows of s * (gain b_gain)
 // Three matrix products that differ in which index of each operand is contiguous; one kernel template covers them:
 //   C[i, j] = sum over p of A(i, p) B(j, p),   each operand stored with p contiguous ("rows") or with i / j contiguous ("columns").
-// An operand is never transposed in memory.  Tiles of 128 bytes along p travel to LDS as they lie (16 bytes per lane, straight
+// An operand is never transposed in memory.  Tiles of 64 or 128 bytes along p travel to LDS as they lie (16 bytes per lane, straight
 // into LDS where rows are 16-byte aligned), and a fragment of a "columns" operand is read by the transposing LDS read (16-bit)
 // or four rows at a time (float32).  16-bit operands multiply on v_mfma_f32_16x16x32, float32 ones on v_mfma_f32_16x16x4_f32,
 // whose products and sums are plain float32.  All sums are float32; every output is rounded once.
@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace sg {
 namespace {
@@ -27,7 +28,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kStepBytes = 128;                    // of p per LDS tile: 64 16-bit or 32 float32 elements
+constexpr int kPartBytes = 64;                     // of p per product: 32 16-bit or 4 x 4 float32 elements; a step has KK parts
 constexpr unsigned kOutside = 0x80000000u;         // a buffer offset beyond every descriptor: the load yields zeros
 
 enum { kActLinear = 1, kActRelu, kActLrelu, kActTanh, kActSigmoid, kActElu, kActSelu, kActSoftplus, kActSwish };
@@ -103,7 +104,7 @@ struct Gemm {
     const void* b;                       // operand of the columns j
     int64_t lda, ldb;                    // elements between rows as stored
     int64_t ni, nj, np;
-    int tiles_i, tiles_j, slices, slice_steps;
+    int tiles_i, tiles_j, slices, slice_steps;           // slice_steps: of 128 bytes along p
     float* partial;                      // [slices][ni][nj] when slices > 1
     void* out;                           // [ni][nj]
     float scale;
@@ -176,64 +177,65 @@ __device__ __forceinline__ i32x4_t descriptor(const void* p) {
     return i32x4_t{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)(a >> 32) & 0xffff), (int)kOutside, 0x00020000};
 }
 
-// 16 bytes per lane from `offset + more` behind the descriptor's address to LDS at lds + 16 * lane; zeros for kOutside.  Written as
-// assembly because of its wait: the compiler holds every LDS read behind all copies into LDS that came before it, those into
-// the other buffer included.  copies_landed() is the wait, and the kernel places it.
-__device__ __forceinline__ void copy_to_lds(i32x4_t from, unsigned offset, unsigned more, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(from), "s"(more) : "m0");
+// 16 bytes per lane from `offset` behind the descriptor's address to LDS at lds + PLACE + 16 * lane; zeros for kOutside.  Written as
+// assembly because of its wait: the compiler holds every LDS read behind all copies into LDS that came before it, those into the
+// other tiles included.  The kernel places the waits.  (One instruction sets the LDS address: a wave that has a SIMD to itself
+// issues one in four cycles, 32 in the time of 8 products, and a step is built to stay below that.)
+template <int PLACE> __device__ __forceinline__ void copy_to_lds(i32x4_t from, unsigned offset, unsigned lds) {
+    asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(lds), "n"(PLACE), "v"(offset), "s"(from) : "m0", "scc");
 }
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
-// One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: SIDE * 8 slots of 16 bytes, slot k * THREADS + t filled by
-// thread t.
-//   ROWS:  slot (row, c) holds the 16 bytes c ^ ((row >> 1) & 7) of the row: 16 lanes reading one column of 16 rows hit 16
-//          different 16-byte banks.
+// One operand's tile of SIDE rows i (or j) by KK * 64 bytes of p in LDS: slots of 16 bytes, slot k * THREADS + t filled by thread t.
+//   ROWS:  slot (row, c) holds the 16 bytes c ^ turn(row) of the row: the lanes that read at one time - 16 rows at one c, or 8 rows
+//          each at two - hit 16 different 16-byte banks.
 //   !ROWS: lines of SIDE elements at one p.  16-bit: the 32-byte block c of line q holds block c ^ swizzle(q), so that the
 //          transposing read of 16 lines hits each 32-byte bank twice, once per half wave; float32: as it lies.  Line q holds
 //          p = p_of(q): where a thread fills every 8th line (256 columns), bits 2 and 3 trade places, so that a thread's slots
 //          share one swizzle.
 // Either way a thread's slots are one address and constant distances apart.
-template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
-    static constexpr int ES = sizeof(T), E = 16 / ES, BK = kStepBytes / ES;
-    static constexpr int BYTES = SIDE * kStepBytes;
-    static constexpr int LOADS = SIDE * 8 / THREADS;               // 16-byte slots per thread
-    static constexpr int LINE = ROWS ? 8 : SIDE / E;               // slots per row or line
+template <class T, int SIDE, bool ROWS, int KK, int THREADS> struct Tile {
+    static constexpr int ES = sizeof(T), E = 16 / ES, PITCH = KK * kPartBytes, BK = PITCH / ES;
+    static constexpr int BYTES = SIDE * PITCH;
+    static constexpr int LOADS = BYTES / 16 / THREADS;             // 16-byte slots per thread
+    static constexpr int LINE = ROWS ? PITCH / 16 : SIDE / E;      // slots per row or line
     static constexpr int APART = THREADS / LINE;                   // rows or lines from one slot of a thread to its next
     static constexpr bool SWAP = !ROWS && ES == 2 && APART == 8;
-    static_assert(LOADS >= 1 && LOADS * THREADS == SIDE * 8, "slots divide among the threads");
+    static_assert(LOADS >= 1 && LOADS * THREADS * 16 == BYTES, "slots divide among the threads");
     static_assert(ROWS ? APART % 16 == 0 : ES == 4 || APART % 16 == 0 || SWAP, "a thread's slots share one swizzle");
 
+    static __device__ __forceinline__ constexpr int turn(int row) { return KK == 2 ? (row >> 1) & 7 : -(row >> 2) & 3; }
     static __device__ __forceinline__ constexpr int p_of(int q) { return SWAP ? (q & ~12) | (q & 4) << 1 | (q & 8) >> 1 : q; }
     static __device__ __forceinline__ int swizzle(int q) {
         if (ES == 4) return 0;
         if (SWAP) return q & 7;
         return SIDE >= 128 ? (q & 3) | ((q >> 3) & 1) << 2 : ((q >> 1) & 1) | ((q >> 3) & 1) << 1;
     }
-    // the slots of a thread: its first one as (side, p) within the tile
-    struct Slots { int side, p; unsigned off; };
-    static __device__ __forceinline__ Slots plan(int64_t ld) {
+    // distance of slot k from the first, along side (ROWS) or p (!ROWS)
+    static __device__ __forceinline__ constexpr int apart(int k) { return ROWS ? k * APART : p_of(k * APART); }
+    // the slots of a thread: its first one as (side, p) within the tile; byte offsets of all, kOutside beyond the matrix's side
+    struct Slots { int side, p; unsigned off[LOADS]; };
+    static __device__ __forceinline__ Slots plan(int64_t ld, int left_side) {
         Slots s;
         const int line = threadIdx.x / LINE, c = threadIdx.x % LINE;
         if (ROWS) {
             s.side = line;
-            s.p = (c ^ ((line >> 1) & 7)) * E;
+            s.p = (c ^ turn(line)) * E;
         } else {
             s.p = p_of(line);
             s.side = (c ^ (swizzle(line) << 1)) * E;
         }
-        s.off = (unsigned)((ROWS ? s.side : s.p) * (unsigned)ld + (ROWS ? s.p : s.side)) * ES;
+#pragma unroll
+        for (int k = 0; k < LOADS; k++)
+            s.off[k] = (ROWS ? s.side < left_side - apart(k) : s.side < left_side)
+                           ? (unsigned)((ROWS ? s.side + apart(k) : s.p + apart(k)) * (unsigned)ld + (ROWS ? s.p : s.side)) * ES : kOutside;
         return s;
     }
-    // distance of slot k from the first, along side (ROWS) or p (!ROWS)
-    static __device__ __forceinline__ constexpr int apart(int k) { return ROWS ? k * APART : p_of(k * APART); }
-    static __device__ __forceinline__ bool inside(const Slots& s, int k, int left_side, int left_p) {
-        return ROWS ? s.side < left_side - apart(k) && s.p < left_p : s.side < left_side && s.p < left_p - apart(k);
-    }
-    // slot k straight to LDS.  from: the tile's first element of this step; left_*: extent from there (at most 2^30)
-    static __device__ __forceinline__ void copy(const Slots& s, int k, i32x4_t from, unsigned ld, unsigned lds, int left_side, int left_p) {
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        copy_to_lds(from, inside(s, k, left_side, left_p) ? s.off : kOutside, (unsigned)apart(k) * ld * ES, lds + (k * THREADS + wave * 64) * 16);
+    // slot k straight to LDS, at `lds` (the wave's share of the tile) + FIRST.  FULL: the step lies whole within p, else left_p of it
+    template <int FIRST, int K, bool FULL> static __device__ __forceinline__ void copy(const Slots& s, i32x4_t from, unsigned lds, int left_p) {
+        const bool in = FULL || s.p < left_p - (ROWS ? 0 : apart(K));
+        copy_to_lds<FIRST + K * THREADS * 16>(from, in ? s.off[K] : kOutside, lds);
     }
     // by way of registers: any alignment, any extent
     // A slot that the end of its row cuts is read from the row's last 16 bytes and shifted into place when it is written to LDS, so
@@ -287,8 +289,9 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
     }
 };
 
-// Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for K-part kk (two per step: 32 16-bit or 16 float32 elements).
-template <class T, int SIDE, bool ROWS, int THREADS, int COUNT> struct Frags {
+// Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for part kk of a step.
+template <class T, int SIDE, bool ROWS, int KK, int THREADS, int COUNT> struct Frags {
+    using Here = Tile<T, SIDE, ROWS, KK, THREADS>;
     static constexpr int V = sizeof(T) == 4 && !ROWS ? (COUNT >= 4 ? 4 : COUNT) : 1;   // tiles whose rows interleave
     uint4 q[COUNT];                                                                   // 8 16-bit values, or 4 float32 (ROWS)
     float f[sizeof(T) == 4 && !ROWS ? COUNT : 1][4];
@@ -300,16 +303,15 @@ template <class T, int SIDE, bool ROWS, int THREADS, int COUNT> struct Frags {
     __device__ __forceinline__ void read(const unsigned char* lds, int first, int kk, int t) {
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
         if constexpr (ROWS) {
-            const int at = (first + l16) * kStepBytes + (((kk * 4 + g) ^ ((l16 >> 1) & 7)) << 4);
-            q[t] = *reinterpret_cast<const uint4*>(lds + at + t * 16 * kStepBytes);
+            const int at = (first + l16) * Here::PITCH + (((kk * 4 + g) ^ Here::turn(l16)) << 4);
+            q[t] = *reinterpret_cast<const uint4*>(lds + at + t * 16 * Here::PITCH);
         } else if constexpr (sizeof(T) == 2) {
             constexpr int LINE = SIDE * 2;
-            using Lines = Tile<T, SIDE, false, THREADS>;
-            const int q0 = Lines::p_of(kk * 32 + g * 8 + (l16 >> 2));        // (its own inverse)
-            const unsigned char* at = lds + q0 * LINE + (l16 & 3) * 8 + (((first >> 4) + t) ^ Lines::swizzle(q0)) * 32;
+            const int q0 = Here::p_of(kk * 32 + g * 8 + (l16 >> 2));        // (its own inverse)
+            const unsigned char* at = lds + q0 * LINE + (l16 & 3) * 8 + (((first >> 4) + t) ^ Here::swizzle(q0)) * 32;
             typedef __attribute__((address_space(3))) s16x4_t* Lds;
             const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at);
-            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + Lines::p_of(4) * LINE));
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + Here::p_of(4) * LINE));
             const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
             q[t] = make_uint4(a.x, a.y, b.x, b.y);
         } else {
@@ -368,17 +370,21 @@ template <int M, int N> __device__ __forceinline__ void settle(f32x4_t (&acc)[M]
         for (int s = 0; s < N; s++) asm volatile("" : "+a"(acc[t][s]));
 }
 
+// f(integral_constant 0), f(integral_constant 1), ...
+template <class F, int... K> __device__ __forceinline__ void for_each(F f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
+
 enum { kDirect, kLoose, kShort };
 
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int KK, int MODE>
 __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
     constexpr bool FORWARD = ROWS_A && ROWS_B;
-    constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
-    using TileA = Tile<T, BI, ROWS_A, THREADS>;
-    using TileB = Tile<T, BJ, ROWS_B, THREADS>;
-    using FragA = Frags<T, BI, ROWS_A, THREADS, TI>;
-    using FragB = Frags<T, BJ, ROWS_B, THREADS, TJ>;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[2 * (TileA::BYTES + TileB::BYTES)];
+    constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = KK * kPartBytes / (int)sizeof(T);
+    constexpr int RING = KK == 1 ? 4 : 2;                 // tiles of that many steps in LDS
+    using TileA = Tile<T, BI, ROWS_A, KK, THREADS>;
+    using TileB = Tile<T, BJ, ROWS_B, KK, THREADS>;
+    using FragA = Frags<T, BI, ROWS_A, KK, THREADS, TI>;
+    using FragB = Frags<T, BJ, ROWS_B, KK, THREADS, TJ>;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[RING * (TileA::BYTES + TileB::BYTES)];
     constexpr int BUF = TileA::BYTES + TileB::BYTES;
 
     // Workgroups go round robin over the 8 XCDs: each XCD gets a contiguous share of the tiles, in groups of 8 tile rows so that
@@ -398,8 +404,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     const T* b = (const T*)g.b + (ROWS_B ? j0 * g.ldb : j0);
     const int left_i = (int)min(g.ni - i0, (int64_t)BI), left_j = (int)min(g.nj - j0, (int64_t)BJ);
     const int steps_all = (int)((g.np + BK - 1) / BK);
-    const int first = (int)slice * g.slice_steps;
-    const int steps = min(g.slice_steps, steps_all - first);
+    const int first = (int)slice * g.slice_steps * (2 / KK), steps = min(g.slice_steps * (2 / KK), steps_all - first);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
@@ -410,8 +415,8 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         for (int s = 0; s < TI; s++) acc[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     auto left_p = [&](int step) { return (int)min(g.np - (int64_t)step * BK, (int64_t)BK); };
-    const typename TileA::Slots sa = TileA::plan(g.lda);
-    const typename TileB::Slots sb = TileB::plan(g.ldb);
+    const typename TileA::Slots sa = TileA::plan(g.lda, left_i);
+    const typename TileB::Slots sb = TileB::plan(g.ldb, left_j);
     auto at_a = [&](int step) { return a + (ROWS_A ? (int64_t)step * BK : (int64_t)step * BK * g.lda); };
     auto at_b = [&](int step) { return b + (ROWS_B ? (int64_t)step * BK : (int64_t)step * BK * g.ldb); };
     // column tile t of the wave's part
@@ -427,32 +432,41 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
         }
     };
     if constexpr (MODE == kDirect) {
-        // Two LDS buffers and two sets of fragments.  A step is two halves: the first multiplies the fragments of its first
-        // K-part while those of the second are read; then, behind the one barrier of a step, the second is multiplied while the
-        // first fragments of the next step are read and the copies of the step after it start into the buffer that has just
-        // been read for the last time.  So the matrix unit has operands in registers at the barrier, and a copy has a whole
-        // step to land.
-        const unsigned lds = lds_address(smem);
-        constexpr int PARTS = TI > TJ ? TI : TJ;
+        // Two sets of fragments: one is multiplied while the other is read, so that the matrix unit has its operands in registers at
+        // a barrier.  KK = 1: a ring of four tiles; in step n the fragments of step n + 1 are read and the copies of step n + 3
+        // start into the tile that step n - 1 was read from: a copy has two steps to land, and reads and copies lie evenly between
+        // the products (as a batch they hold up the wave's products behind them).  KK = 2: two tiles and half the barriers, for
+        // small tiles, where a barrier costs more than that; in the second half of step n, behind the barrier, the copies of step
+        // n + 2 start into the tile just read for the last time.  8192 x 4096 -> 4096, 256 x 256: 207 us with KK = 1, 215 with 2
+        // (without any copies 172, without reads 189); 4096^3 with 64 x 64: 278 and 182.
+        const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(smem) + wave * 1024);
+        constexpr int PARTS = TI > TJ ? TI : TJ, COPIES = TileA::LOADS + TileB::LOADS;
         FragA fa[2];
         FragB fb[2];
-        // share `part` of PARTS of the copies of step n (of one behind the last step: zeros, which nothing reads)
-        auto copy_part = [&](i32x4_t from_a, i32x4_t from_b, int n, int part) {
-            const int left = n < steps ? left_p(first + n) : 0;
-            const unsigned to = lds + (n & 1) * BUF;
-#pragma unroll
-            for (int k = 0; k < TileA::LOADS; k++)
-                if (k * PARTS / TileA::LOADS == part) TileA::copy(sa, k, from_a, (unsigned)g.lda, to, left_i, left);
-#pragma unroll
-            for (int k = 0; k < TileB::LOADS; k++)
-                if (k * PARTS / TileB::LOADS == part) TileB::copy(sb, k, from_b, (unsigned)g.ldb, to + TileA::BYTES, left_j, left);
+        // where the next step to be copied starts
+        const T *from_a = at_a(first), *from_b = at_b(first);
+        const int64_t step_a = ROWS_A ? BK : BK * g.lda, step_b = ROWS_B ? BK : BK * g.ldb;
+        // share `part` of PARTS of the copies of step n.  full: it lies whole within p, else `left` of it (none of a step behind the
+        // last: zeros, which count for nothing)
+        auto copy_part = [&](i32x4_t a4, i32x4_t b4, int n, int part, auto full, int left) {
+            const unsigned to = lds + (n & (RING - 1)) * BUF;
+            for_each([&](auto k) {
+                constexpr int K = decltype(k)::value;
+                if (K * PARTS / COPIES != part) return;
+                if constexpr (K < TileA::LOADS) TileA::template copy<0, K, decltype(full)::value>(sa, a4, to, left);
+                else TileB::template copy<TileA::BYTES, K - TileA::LOADS, decltype(full)::value>(sb, b4, to, left);
+            }, std::make_integer_sequence<int, COPIES>{});
         };
+        auto left_of = [&](int n) { return n < steps ? left_p(first + n) : 0; };
         auto copy_all = [&](int n) {
-            const i32x4_t from_a = descriptor(at_a(first + n)), from_b = descriptor(at_b(first + n));
+            const i32x4_t a4 = descriptor(from_a), b4 = descriptor(from_b);
+            const int left = left_of(n);
 #pragma unroll
-            for (int part = 0; part < PARTS; part++) copy_part(from_a, from_b, n, part);
+            for (int part = 0; part < PARTS; part++) copy_part(a4, b4, n, part, std::false_type{}, left);
+            from_a += step_a;
+            from_b += step_b;
         };
-        // share `part` of the reads of a half: spread over its first three quarters, so that the last of them are back in time
+        // share `part` of the reads: spread over the first three quarters, so that the last of them are back in time
         constexpr int READ_PARTS = PARTS >= 4 ? PARTS * 3 / 4 : PARTS;
         auto read_part = [&](int set, const unsigned char* from, int kk, int part) {
 #pragma unroll
@@ -462,36 +476,58 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
             for (int t = 0; t < TJ; t++)
                 if (t * READ_PARTS / TJ == part) fb[set].read(from + TileA::BYTES, wj, kk, t);
         };
+        constexpr int AHEAD = KK == 1 ? 3 : 2;
+        auto step = [&](int n, int set, auto full) {                     // set = n & 1 (KK = 1); full: step n + AHEAD is
+            const unsigned char* now = smem + (n & (RING - 1)) * BUF;
+            const unsigned char* next = smem + ((n + 1) & (RING - 1)) * BUF;
+            const int reading = KK == 1 ? set ^ 1 : 0;
+            if constexpr (KK == 1) {
+                // the copies of step n + 1 have landed (those of step n + 2 may be under way), everybody's
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(COPIES) : "memory");
+            } else {
+#pragma unroll
+                for (int t = 0; t < PARTS; t++) {
+                    read_part(1, now, 1, t);
+                    if (t < TJ) multiply_tile(fa[0], fb[0], t);
+                    __builtin_amdgcn_sched_barrier(0);                   // (or the reads gather behind the products)
+                }
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            const i32x4_t a4 = descriptor(from_a), b4 = descriptor(from_b);
+            const int left = full ? BK : left_of(n + AHEAD);
+            from_a += step_a;
+            from_b += step_b;
+#pragma unroll
+            for (int t = 0; t < PARTS; t++) {
+                copy_part(a4, b4, n + AHEAD, t, full, left);
+                read_part(reading, next, 0, t);
+                if (t < TJ) multiply_tile(fa[reading ^ 1], fb[reading ^ 1], t);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         if (steps > 0) {
             copy_all(0);
             copies_landed();
             __syncthreads();
-            copy_all(1);
+#pragma unroll
+            for (int k = 1; k < AHEAD; k++) copy_all(k);
             fa[0].read(smem, wi, 0);
             fb[0].read(smem + TileA::BYTES, wj, 0);
         }
-        // One body for every step: the last two read and copy what does not exist.
+        int n = 0;
+        const int full_steps = min(steps, (int)(g.np / BK) - first);      // of this slice
+        // (KK = 1: steps in pairs, so that the sets are constants; a step behind the last multiplies the zeros copied for it)
 #pragma unroll 1
-        for (int n = 0; n < steps; n++) {
-            const unsigned char* now = smem + (n & 1) * BUF;
-            const unsigned char* next = smem + (~n & 1) * BUF;
-#pragma unroll
-            for (int t = 0; t < PARTS; t++) {
-                read_part(1, now, 1, t);
-                if (t < TJ) multiply_tile(fa[0], fb[0], t);
-                __builtin_amdgcn_sched_barrier(0);        // (or the reads gather behind the products)
-            }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            const i32x4_t from_a = descriptor(at_a(first + n + 2)), from_b = descriptor(at_b(first + n + 2));
-#pragma unroll
-            for (int t = 0; t < PARTS; t++) {
-                copy_part(from_a, from_b, n + 2, t);
-                read_part(0, next, 0, t);
-                if (t < TJ) multiply_tile(fa[1], fb[1], t);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (; n + 4 < full_steps; n += 2) {
+            step(n, 0, std::true_type{});
+            step(n + 1, 1, std::true_type{});
         }
-        copies_landed();                                  // (the epilogue writes where they go)
+#pragma unroll 1
+        for (; n < steps; n += 2) {
+            step(n, 0, std::false_type{});
+            if (KK == 1 || n + 1 < steps) step(n + 1, 1, std::false_type{});
+        }
+        copies_landed();                                                 // (the epilogue writes where they go)
     } else {
         // Two LDS buffers and two sets of registers: a step's loads have the two steps before it to arrive; one barrier a step.
         // Steps go in pairs and every step loads, the last ones their own data again (behind a branch the compiler would wait
@@ -516,7 +552,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
             __syncthreads();
             fetch(n + 2, set);
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
+            for (int kk = 0; kk < KK; kk++) {
                 FragA fa;
                 FragB fb;
                 fa.read(smem + set * BUF, wi, kk);
@@ -543,7 +579,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     // down in LDS as rows of four-column chunks (chunk c of row r at c ^ r: the 16 rows a store touches lie in 16 different
     // 16-byte banks) and takes it up again in runs of consecutive columns: stores of 16 bytes, and one copy of the
     // epilogue's code.
-    constexpr int COLS = BJ / WJ, CHUNKS = COLS / 4, ROWS_MAX = BUF * 2 / (WI * WJ) / (COLS * 4);
+    constexpr int COLS = BJ / WJ, CHUNKS = COLS / 4, ROWS_MAX = BUF * RING / (WI * WJ) / (COLS * 4);
     constexpr int S_PASS = ROWS_MAX / 16 < TI ? ROWS_MAX / 16 : TI;      // A tiles per pass
     constexpr int N = 16 / (int)sizeof(T), RUNS = COLS / N;
     static_assert(S_PASS >= 1 && TI % S_PASS == 0, "the epilogue's passes");
@@ -979,16 +1015,16 @@ bool thin_fits(int dtype, bool rows_b, int64_t ni, int64_t nj, int64_t np) {
 // The tile and the number of slices with the least predicted time.  Measured on MI355X, us per step (128 bytes along p) of a
 // workgroup that has a CU to itself / of each of several that share one, by the number of "columns" operands, and us for the ends
 // of a tile (first copies, epilogue) that nothing overlaps:
-//   16-bit  64 x 64: 0.27 / 0.18, 0.29 / 0.18, 0.31 / 0.20, 0.4     128 x 128: 0.75 / 0.48, 0.75 / 0.50, 0.82 / 0.52, 1.2     256 x 256: 1.62 each, 5
-//   float32 64 x 64: 0.62 / 0.50, whichever, 0.4                 (a 128 x 128 tile takes four times that: not built)
+//   16-bit  64 x 64: 0.26 / 0.18, 0.24 / 0.18, 0.24 / 0.20, 0.4     128 x 128: 0.67 / 0.45, 0.59 / 0.50, 0.57 / 0.48, 1.2     256 x 256: 1.60, 1.55, 1.50, 5
+//   float32 64 x 64: 0.46 / 0.46, whichever, 0.4                 (a 128 x 128 tile takes four times that: not built)
 // 3 us for a launch; slices cost a second launch and a round trip of their float32 sums at 6 TB/s.
-// 1024^3 in bfloat16: 64 x 64 tiles 7 us, 128 x 128 12; 4096^3: 256 x 256 109 us (1257 TFLOP/s), 128 x 128 125, 64 x 64 182; a weight
-// gradient of 2048 x 2048 over 8192 rows: 256 x 256 in four slices 76, 128 x 128 97.
+// 1024^3 in bfloat16: 64 x 64 tiles 7 us, 128 x 128 12; 4096^3: 256 x 256 108 us (1270 TFLOP/s), 128 x 128 117, 64 x 64 187; a weight
+// gradient of 2048 x 2048 over 8192 rows: 256 x 256 in four slices 78, 128 x 128 76, 256 x 256 whole 164.
 Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
     struct Kind { int tile; double alone[3], shared[3], ends; };
-    static const Kind kinds[] = {{64, {0.27, 0.29, 0.31}, {0.18, 0.18, 0.20}, 0.4}, {128, {0.75, 0.75, 0.82}, {0.48, 0.50, 0.52}, 1.2},
-                                 {256, {1.62, 1.62, 1.62}, {1.62, 1.62, 1.62}, 5.0}};
-    static const Kind kinds32[] = {{64, {0.62, 0.62, 0.62}, {0.50, 0.50, 0.50}, 0.4}};
+    static const Kind kinds[] = {{64, {0.26, 0.24, 0.24}, {0.18, 0.18, 0.20}, 0.4}, {128, {0.67, 0.59, 0.57}, {0.45, 0.50, 0.48}, 1.2},
+                                 {256, {1.60, 1.55, 1.50}, {1.60, 1.55, 1.50}, 5.0}};
+    static const Kind kinds32[] = {{64, {0.46, 0.46, 0.46}, {0.46, 0.46, 0.46}, 0.4}};
     Shape best;
     best.thin = columns < 2 && thin_fits(dtype, columns == 0, ni, nj, np);
     const int bk = dtype == SG_F32 ? 32 : 64;
@@ -1018,7 +1054,8 @@ Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
 
 template <class T, int TILE, bool RA, bool RB, int MODE> void launch_gemm(const Gemm& g, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices));
-    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, MODE>), grid, dim3(256), 0, stream, g);
+    constexpr int KK = MODE == kDirect && (TILE == 256 || (TILE == 128 && !(RA && RB))) ? 1 : 2;      // (what was faster where it is used)
+    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, KK, MODE>), grid, dim3(256), 0, stream, g);
 }
 
 template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
