@@ -105,6 +105,7 @@ struct Gemm {
     int64_t lda, ldb;                    // elements between rows as stored
     int64_t ni, nj, np;
     int tiles_i, tiles_j, slices, slice_steps;           // slice_steps: of 128 bytes along p
+    int a_padded, b_padded;              // its rows go on with zeros to whole 16-byte packets
     float* partial;                      // [slices][ni][nj] when slices > 1
     void* out;                           // [ni][nj]
     float scale;
@@ -866,10 +867,10 @@ struct SlopeParams {
     const void* y;                       // the layer's output, or NULL   (slope by its sign)
     const uint8_t* positive;             // or NULL
     const float* z;                      // or NULL
-    void* s;                             // [rows][cols], or NULL: column sums only
+    void* s;                             // [rows][lds], or NULL: column sums only; columns behind cols become zeros
     float* partial;                      // [row blocks][cols]
     void* sums;                          // [cols], written directly when there is one row block
-    int64_t rows, cols, ld;
+    int64_t rows, cols, ld, lds;
     int rows_per_block;
     int act;
     float alpha, sign;                   // sign: of the layer's gain
@@ -891,6 +892,8 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
     float sum[N];
 #pragma unroll
     for (int e = 0; e < N; e++) sum[e] = 0.f;
+    if (c >= p.cols && c < p.lds && p.s)                  // (N = 1: otherwise rows are whole packets)
+        for (int64_t r = r0 + wave; r < r1; r += 4) ((T*)p.s)[r * p.lds + c] = rounded<T>(0.f);
     if (c < p.cols) {
         for (int64_t r = r0 + wave; r < r1; r += 4 * UNROLL) {
             Run<T, N> dy[UNROLL], y[UNROLL];
@@ -918,7 +921,7 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
                     sum[e] += there ? s : 0.f;
                     out.v[e] = rounded<T>(s);
                 }
-                if (p.s && there) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.cols + c) = out;
+                if (p.s && there) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.lds + c) = out;
             }
         }
     }
@@ -958,6 +961,40 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const float* __restri
     }
 }
 
+// ---- operands whose rows are not whole packets ------------------------------------------------------------------------------------
+// Copies with rows of whole aligned packets, zeros behind the last element: two passes over an operand, and from there on the tiles
+// travel to LDS directly and not by way of registers, and may be large ones.  Forward / gradients of x / of w in us, without and with:
+//   float16  1000 x 771 -> 1025    16.9 / 17.7 / 16.2      16.9 / 17.3 / 18.2 (the last two together share one launch for the copies)
+//   float32  1000 x 771 -> 1025    42.2 / 39.7 / 36.1      38.3 / 29.6 / 30.9
+//   float16  2047 x 2049 -> 2051   74 / 75 / 73            66 / 64 / 49
+//   bfloat16 8192 x 4095 -> 4097   546 / 435 / 559         339 / 284 / 363
+//   float32  64 x 8191 -> 511      18.5 / 19.7 / 12.8      23.1 / 19.8 / 14.9
+// so products from 2^29 terms on are laid out so, smaller ones are not.
+struct PackParams {
+    struct { const void* src; void* dst; int64_t ld, rows, cols, packets; } m[3];      // packets: per row
+    int64_t first[4];                    // number of packets of the matrices before
+};
+
+template <class T> __global__ void __launch_bounds__(256) linear_pack_kernel(const PackParams p) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (k >= p.first[3]) return;
+    const int which = k >= p.first[2] ? 2 : k >= p.first[1] ? 1 : 0;
+    const auto& m = p.m[which];
+    const int64_t at = k - p.first[which];
+    const int64_t row = (uint64_t)at >> 32 ? at / m.packets : (uint32_t)at / (uint32_t)m.packets, c = (at - row * m.packets) * E;
+    const T* src = (const T*)m.src + row * m.ld + c;
+    Pack<T> q;
+    if (c + E <= m.cols) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Loose { Pack<T> v; };
+        q = reinterpret_cast<const Loose*>(src)->v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) q.v[e] = c + e < m.cols ? src[e] : rounded<T>(0.f);
+    }
+    store_pack((T*)m.dst + (row * m.packets) * E + c, q);
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -981,7 +1018,8 @@ template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* 
     const bool packed = p.cols % N == 0 && p.ld % N == 0 && aligned16(p.dy) && aligned16(p.y) && aligned16(p.s) && aligned16(p.z) &&
                         reinterpret_cast<uintptr_t>(p.positive) % N == 0;
     const int n = packed ? N : 1;
-    const int64_t bx = (p.cols + 64 * n - 1) / (64 * n), by = p.rows == 0 ? 1 : slope_blocks(p.rows, p.cols);
+    if (p.s == nullptr || p.lds < p.cols) p.lds = p.cols;
+    const int64_t bx = (p.lds + 64 * n - 1) / (64 * n), by = p.rows == 0 ? 1 : slope_blocks(p.rows, p.cols);
     SG_REQUIRE(bx <= INT32_MAX && by <= 65535, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
     const dim3 grid((unsigned)bx, (unsigned)by);
 #define SG_SLOPE(BY)                                                                                                    \
@@ -1065,7 +1103,8 @@ template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStr
     // offsets within a tile's lines are 32-bit
     SG_REQUIRE((g.lda + 1) * ES * 256 < (int64_t)kOutside && (g.ldb + 1) * ES * 256 < (int64_t)kOutside, SG_ERR_UNSUPPORTED,
                "%s: rows of %lld / %lld elements are too long", what, (long long)g.lda, (long long)g.ldb);
-    const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && (RA ? g.np : g.ni) % E == 0 && (RB ? g.np : g.nj) % E == 0;
+    const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && ((RA ? g.np : g.ni) % E == 0 || g.a_padded) &&
+                        ((RB ? g.np : g.nj) % E == 0 || g.b_padded);
     g.whole = runs_aligned<T>(g);
     if constexpr (RA && (RB || ES == 4)) {
         if (s.thin && aligned16(g.a) && g.lda % E == 0 && (RB ? aligned16(g.b) && g.ldb % E == 0 : reinterpret_cast<uintptr_t>(g.b) % 8 == 0 && g.ldb % 2 == 0)) {
@@ -1076,23 +1115,17 @@ template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStr
             return check_launch(what);
         }
     }
-    int tile = s.tile;
-    if (tile == 256 && !direct) {          // no registers to spare there for operands that need them on their way to LDS
-        tile = 128;
-        g.tiles_i = (int)((g.ni + 127) / 128);
-        g.tiles_j = (int)((g.nj + 127) / 128);
-    }
-    const bool is_short = (RA ? g.np : g.ni) < E || (RB ? g.np : g.nj) < E;
-    if (tile == 128 && is_short) {
-        tile = 64;
+    // (operands that travel by way of registers are those of small products: others are copied into packets first)
+    const int tile = direct ? s.tile : 64;
+    if (tile != s.tile) {
         g.tiles_i = (int)((g.ni + 63) / 64);
         g.tiles_j = (int)((g.nj + 63) / 64);
     }
     SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    const bool is_short = (RA ? g.np : g.ni) < E || (RB ? g.np : g.nj) < E;
     if constexpr (ES == 2) {
         if (tile == 256) launch_gemm<T, 256, RA, RB, kDirect>(g, stream);
-        else if (tile == 128 && direct) launch_gemm<T, 128, RA, RB, kDirect>(g, stream);
-        else if (tile == 128) launch_gemm<T, 128, RA, RB, kLoose>(g, stream);
+        if (tile == 128) launch_gemm<T, 128, RA, RB, kDirect>(g, stream);
     }
     if (tile == 64) {
         if (direct) launch_gemm<T, 64, RA, RB, kDirect>(g, stream);
@@ -1122,23 +1155,94 @@ int check(const sg_linear_params* p, const char* what) {
 
 bool piecewise(int act) { return act == kActRelu || act == kActLrelu; }
 
+constexpr double kCopiedFrom = (double)(1 << 29);        // terms of a product; measured above
+
+// An operand as the products read it: where it lies, or its copy in the workspace.
+struct Operand {
+    const void* p = nullptr;
+    int64_t ld = 0;
+    int padded = 0;
+    size_t at = 0, bytes = 0;            // of the copy; none: 0 bytes
+};
+
+int elements(int dtype) { return dtype == SG_F32 ? 4 : 8; }
+int64_t whole_packets(int64_t cols, int dtype) { return (cols + elements(dtype) - 1) / elements(dtype) * elements(dtype); }
+
+// x and w of a layer; `at`: where in the workspace copies may lie (moved on behind them).  Products from 2^29 terms on.
+void place_operands(const sg_linear_params& p, size_t& at, Operand& x, Operand& w) {
+    const int e = elements(p.dtype);
+    const bool large = (double)p.m * p.n * p.k >= kCopiedFrom;
+    auto place = [&](Operand& o, const void* src, int64_t ld, int64_t rows) {
+        o.p = src;
+        o.ld = ld;
+        if (!large || (aligned16(src) && ld % e == 0 && p.k % e == 0)) return;
+        o.ld = whole_packets(p.k, p.dtype);
+        o.padded = 1;
+        o.at = at;
+        o.bytes = up256((size_t)rows * o.ld * (16 / e));
+        at += o.bytes;
+    };
+    place(x, p.x, p.ldx, p.m);
+    place(w, p.w, p.ldw, p.n);
+}
+
+template <class T> int run_pack(PackParams& q, int count, hipStream_t stream, const char* what) {
+    for (int i = 0; i < 3; i++) q.first[i + 1] = q.first[i] + (i < count ? q.m[i].rows * q.m[i].packets : 0);
+    if (q.first[3] == 0) return SG_OK;
+    SG_REQUIRE((q.first[3] + 255) / 256 <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)((q.first[3] + 255) / 256)), dim3(256), 0, stream, q);
+    return check_launch(what);
+}
+
+// Adds an operand's copy to the launch; from then on it is read there.
+void add_pack(PackParams& q, int& count, Operand& o, char* ws, int64_t rows, int64_t cols, int64_t ld, int dtype) {
+    if (o.bytes == 0) return;
+    q.m[count].src = o.p; q.m[count].dst = ws + o.at;
+    q.m[count].ld = ld; q.m[count].rows = rows; q.m[count].cols = cols;
+    q.m[count].packets = o.ld / elements(dtype);
+    count++;
+    o.p = ws + o.at;
+}
+
+struct ForwardPlan {
+    Shape y;
+    Operand x, w;
+    size_t total = 0;                     // the slices' sums come first
+};
+
+ForwardPlan plan_forward(const sg_linear_params& p) {
+    ForwardPlan f;
+    f.y = shape_of(p.dtype, 0, p.m, p.n, p.k);
+    f.total = f.y.partial_bytes;
+    place_operands(p, f.total, f.x, f.w);
+    return f;
+}
+
 struct BackwardPlan {
-    Shape x, w;
-    size_t s = 0, sums = 0, partial = 0, total = 0;      // offsets: the activation's gradient, row-block sums, slices
+    Shape dx, dw;
+    Operand x, w, s;                      // s: the activation's gradient, or dy (copied only for its own n)
+    size_t sums = 0, partial = 0, total = 0;
 };
 
 BackwardPlan plan_backward(const sg_linear_params& p) {
     BackwardPlan b;
-    const int es = p.dtype == SG_F32 ? 4 : 2;
+    const int e = elements(p.dtype);
     size_t at = 0;
-    b.s = at;
-    if (p.act != kActLinear) at += up256((size_t)p.m * p.n * es);
+    b.s.ld = p.n;
+    const bool large = (double)p.m * p.n * p.k >= kCopiedFrom;
+    if (p.act != kActLinear || (large && p.n % e != 0)) {
+        b.s.ld = large ? whole_packets(p.n, p.dtype) : p.n;
+        b.s.padded = b.s.ld != p.n;
+        b.s.bytes = up256((size_t)p.m * b.s.ld * (16 / e));
+        at += b.s.bytes;
+    }
     b.sums = at;
     at += up256((size_t)slope_blocks(p.m, p.n) * p.n * 4);
-    b.x = shape_of(p.dtype, 1, p.m, p.k, p.n);
-    b.w = shape_of(p.dtype, 2, p.n, p.k, p.m);
+    b.dx = shape_of(p.dtype, 1, p.m, p.k, p.n);
+    b.dw = shape_of(p.dtype, 2, p.n, p.k, p.m);
     b.partial = at;
-    at += b.x.partial_bytes > b.w.partial_bytes ? b.x.partial_bytes : b.w.partial_bytes;
+    at += std::max(b.dx.partial_bytes, b.dw.partial_bytes);
+    place_operands(p, at, b.x, b.w);
     b.total = at;
     return b;
 }
@@ -1160,7 +1264,7 @@ int column_sums(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ld
 extern "C" size_t sg_linear_workspace_bytes(const sg_linear_params* p) {
     using namespace sg;
     if (check(p, "linear") != SG_OK) return 0;
-    return shape_of(p->dtype, 0, p->m, p->n, p->k).partial_bytes;
+    return plan_forward(*p).total;
 }
 
 extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* positive, void* workspace, size_t workspace_bytes, sg_stream_t stream) {
@@ -1170,11 +1274,21 @@ extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* 
     if (p->m == 0 || p->n == 0) return SG_OK;
     SG_REQUIRE(y != nullptr, SG_ERR_NULL_POINTER, "linear: y is NULL");
     SG_REQUIRE(p->residual == nullptr || p->ldr >= p->n, SG_ERR_INVALID_ARGUMENT, "linear: the residual's row stride is smaller than its rows");
-    const Shape s = shape_of(p->dtype, 0, p->m, p->n, p->k);
-    SG_REQUIRE(s.partial_bytes == 0 || (workspace && workspace_bytes >= s.partial_bytes && aligned16(workspace)), SG_ERR_INVALID_ARGUMENT,
-               "linear: needs %zu bytes of aligned workspace", s.partial_bytes);
+    ForwardPlan f = plan_forward(*p);
+    SG_REQUIRE(f.total == 0 || (workspace && workspace_bytes >= f.total && aligned16(workspace)), SG_ERR_INVALID_ARGUMENT,
+               "linear: needs %zu bytes of aligned workspace", f.total);
+    PackParams q{};
+    int copies = 0;
+    add_pack(q, copies, f.x, (char*)workspace, p->m, p->k, p->ldx, p->dtype);
+    add_pack(q, copies, f.w, (char*)workspace, p->n, p->k, p->ldw, p->dtype);
+    if (copies) {
+        int done = SG_OK;
+        SG_DISPATCH_16_32(p->dtype, done = run_pack<T>(q, copies, (hipStream_t)stream, "sg_linear"));
+        if (done != SG_OK) return done;
+    }
     Gemm g{};
-    g.a = p->x; g.lda = p->ldx; g.b = p->w; g.ldb = p->ldw;
+    g.a = f.x.p; g.lda = f.x.ld; g.a_padded = f.x.padded;
+    g.b = f.w.p; g.ldb = f.w.ld; g.b_padded = f.w.padded;
     g.ni = p->m; g.nj = p->n; g.np = p->k;
     g.partial = (float*)workspace;
     g.out = y; g.scale = p->w_gain;
@@ -1182,7 +1296,7 @@ extern "C" int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* 
     g.residual = p->residual; g.ldr = p->ldr;
     g.z = z; g.positive = positive;
     g.act = p->act; g.alpha = p->alpha; g.gain = p->gain;
-    SG_DISPATCH_16_32(p->dtype, return (run_gemm<T, true, true>(g, s, (hipStream_t)stream, "sg_linear")));
+    SG_DISPATCH_16_32(p->dtype, return (run_gemm<T, true, true>(g, f.y, (hipStream_t)stream, "sg_linear")));
     return SG_OK;
 }
 
@@ -1205,46 +1319,61 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
                p->act == kActLinear ? "none" : "one");
     SG_REQUIRE(!any || p->act == kActLinear || (z != nullptr) != piecewise(p->act), SG_ERR_INVALID_ARGUMENT,
                "linear_backward: activation %d takes %s", p->act, piecewise(p->act) ? "y or positive" : "z");
-    const BackwardPlan plan = plan_backward(*p);
+    BackwardPlan plan = plan_backward(*p);
     SG_REQUIRE(plan.total == 0 || (workspace && workspace_bytes >= plan.total && aligned16(workspace)), SG_ERR_INVALID_ARGUMENT,
                "linear_backward: needs %zu bytes of aligned workspace", plan.total);
     char* ws = (char*)workspace;
-    const bool own_s = p->act != kActLinear;
-    const void* s = own_s ? (const void*)(ws + plan.s) : dy;
-    if ((own_s && any && (dx || dw)) || db) {
-        SlopeParams q{};
-        q.dy = dy; q.y = y; q.positive = positive; q.z = z;
-        q.s = own_s && (dx || dw) ? ws + plan.s : nullptr;
-        q.partial = (float*)(ws + plan.sums);
-        q.sums = db;
-        q.rows = p->m; q.cols = p->n; q.ld = p->n;
-        q.act = p->act;
-        q.alpha = p->act == kActRelu ? 0.f : p->alpha;
-        q.sign = p->gain < 0.f ? -1.f : 1.f;
-        q.scale = p->gain * p->b_gain;
+    const bool own_s = p->act != kActLinear, products = any && (dx || dw);
+    PackParams q{};
+    int copies = 0;
+    if (products) {
+        if (own_s) plan.s.p = ws + plan.s.at;
+        else plan.s.p = dy;
+        if (!own_s) add_pack(q, copies, plan.s, ws, p->m, p->n, p->n, p->dtype);
+        if (dw) add_pack(q, copies, plan.x, ws, p->m, p->k, p->ldx, p->dtype);
+        if (dx) add_pack(q, copies, plan.w, ws, p->n, p->k, p->ldw, p->dtype);
+    }
+    if (copies) {
         int done = SG_OK;
-        SG_DISPATCH_16_32(p->dtype, done = run_slope<T>(q, stream, "sg_linear_backward"));
+        SG_DISPATCH_16_32(p->dtype, done = run_pack<T>(q, copies, stream, "sg_linear_backward"));
+        if (done != SG_OK) return done;
+    }
+    if ((own_s && products) || db) {
+        SlopeParams r{};
+        r.dy = dy; r.y = y; r.positive = positive; r.z = z;
+        r.s = own_s && products ? ws + plan.s.at : nullptr;
+        r.lds = plan.s.ld;
+        r.partial = (float*)(ws + plan.sums);
+        r.sums = db;
+        r.rows = p->m; r.cols = p->n; r.ld = p->n;
+        r.act = p->act;
+        r.alpha = p->act == kActRelu ? 0.f : p->alpha;
+        r.sign = p->gain < 0.f ? -1.f : 1.f;
+        r.scale = p->gain * p->b_gain;
+        int done = SG_OK;
+        SG_DISPATCH_16_32(p->dtype, done = run_slope<T>(r, stream, "sg_linear_backward"));
         if (done != SG_OK) return done;
     }
     Gemm g{};
     g.partial = (float*)(ws + plan.partial);
     g.scale = p->gain * p->w_gain;
+    g.a = plan.s.p; g.lda = plan.s.ld; g.a_padded = plan.s.padded;
     if (dx) {                            // [m, k] = s [m, n] w [n, k]
-        Gemm q = g;
-        q.a = s; q.lda = p->n; q.b = p->w; q.ldb = p->ldw;
-        q.ni = p->m; q.nj = p->k; q.np = p->n;
-        q.out = dx;
+        Gemm q2 = g;
+        q2.b = plan.w.p; q2.ldb = plan.w.ld; q2.b_padded = plan.w.padded;
+        q2.ni = p->m; q2.nj = p->k; q2.np = p->n;
+        q2.out = dx;
         int done = SG_OK;
-        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, true, false>(q, plan.x, stream, "sg_linear_backward")));
+        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, true, false>(q2, plan.dx, stream, "sg_linear_backward")));
         if (done != SG_OK) return done;
     }
     if (dw) {                            // [n, k] = s [m, n]^T x [m, k]
-        Gemm q = g;
-        q.a = s; q.lda = p->n; q.b = p->x; q.ldb = p->ldx;
-        q.ni = p->n; q.nj = p->k; q.np = p->m;
-        q.out = dw;
+        Gemm q2 = g;
+        q2.b = plan.x.p; q2.ldb = plan.x.ld; q2.b_padded = plan.x.padded;
+        q2.ni = p->n; q2.nj = p->k; q2.np = p->m;
+        q2.out = dw;
         int done = SG_OK;
-        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, false, false>(q, plan.w, stream, "sg_linear_backward")));
+        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, false, false>(q2, plan.dw, stream, "sg_linear_backward")));
         if (done != SG_OK) return done;
     }
     return SG_OK;

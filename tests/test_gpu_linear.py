@@ -47,7 +47,9 @@ def compare(x, w, b, r, dy, act='lrelu', **kw):
 # one row; one of everything; odd sizes; rows of whole packets; long sums over few tiles (slices); many small tiles
 SIZES = [(1, 512, 512), (1, 1, 1), (3, 5, 7), (2, 8, 1), (32, 512, 512), (33, 129, 65), (64, 64, 64), (128, 256, 128), (257, 100, 300), (40, 8192, 72),
          (1000, 24, 40), (4100, 7, 9), (5, 3000, 11), (16, 2048, 48), (17, 2052, 50), (31, 520, 1024), (32, 1000, 6),
-         (1000, 771, 1025), (130, 9, 200), (200, 70, 8), (70, 1, 70), (70, 3, 70), (3, 70, 70)]
+         (1000, 771, 1025), (130, 9, 200), (200, 70, 8), (70, 1, 70), (70, 3, 70), (3, 70, 70),
+         (500, 403, 700), (333, 520, 777), (1001, 779, 700), (801, 776, 901),
+         (6100, 9, 9800)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
