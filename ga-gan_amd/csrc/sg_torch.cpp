@@ -98,10 +98,11 @@ int dtype_code(const Tensor& t, const char* what) {
 
 Tensor or_undefined(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
-// (t or a dense copy, elements between its rows): unit stride within a row, rows that do not overlap
+// (t or a dense copy, elements between its rows): unit stride within a row, rows that do not overlap and that lie less than the
+// 2^23 bytes apart that the library's 32-bit offsets within a tile allow
 std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
     const int64_t rows = t.size(0), cols = t.size(1);
-    if ((cols <= 1 || t.stride(1) == 1) && (rows <= 1 || t.stride(0) >= std::max<int64_t>(cols, 1)))
+    if ((cols <= 1 || t.stride(1) == 1) && (rows <= 1 || (t.stride(0) >= std::max<int64_t>(cols, 1) && t.stride(0) < (1 << 23) / (int64_t)t.element_size() - 1)))
         return {t, rows > 1 ? t.stride(0) : std::max<int64_t>(cols, 1)};
     return {t.contiguous(), std::max<int64_t>(cols, 1)};
 }
@@ -166,8 +167,8 @@ Tensor linear_composite(const Tensor& x, const Tensor& w, const Tensor& b, const
 }
 
 // What the backward pass keeps besides x and w: nothing for linear; for relu and lrelu the output itself, whose sign is the
-// pre-activation's, or - where a residual, a zero gain or a negative slope hides it - a byte per element; for the others the
-// pre-activation values in float32 (rounded to 16 bits they would cost the gradient more accuracy than its own rounding does).
+// pre-activation's, or - where a residual, a gain that may take positive values to zero (float16: any), or a negative slope
+// hides it - a byte per element; for the others the pre-activation values in float32 (rounded to 16 bits they would cost the gradient more accuracy than its own rounding does).
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
     enum Kept { kNothing, kY, kPositive, kZ };
 
@@ -177,7 +178,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         const Tensor b = or_undefined(b_), residual = or_undefined(residual_);
         const bool slopes = c.act != kLinear && (x.requires_grad() || w.requires_grad() || (b.defined() && b.requires_grad()));
         const bool by_sign = c.act == kRelu || c.act == kLrelu;
-        const bool from_y = by_sign && !residual.defined() && c.gain != 0 && (c.act == kRelu || c.alpha >= 0);
+        const bool from_y = by_sign && !residual.defined() && x.scalar_type() != at::kHalf && std::abs(c.gain) >= 1.0 / 256 && (c.act == kRelu || c.alpha >= 0);
         const Kept kept = !slopes ? kNothing : from_y ? kY : by_sign ? kPositive : kZ;
         Tensor aux;
         Tensor y = linear_forward(x, w, b, residual, c, kept == kZ ? &aux : nullptr, kept == kPositive ? &aux : nullptr);

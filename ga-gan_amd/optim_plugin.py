@@ -96,7 +96,7 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps
             return torch.zeros([])
         if not grad_limit > 0:
             raise RuntimeError('adam_step: grad_limit must be positive')
-        return _lib.ext().adam_step_clipped(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, max_grad_norm, CLIP_EPS)
+        return _lib.ext().adam_step_clipped(params, grads, exp_avgs, exp_avg_sqs, [int(k) for k in steps], lr, beta1, beta2, eps, grad_limit, max_grad_norm, CLIP_EPS)
     for i in range(0, len(params), MAX_TENSORS):
         chunk = range(i, min(i + MAX_TENSORS, len(params)))
         table = (AdamTensor * len(chunk))()
@@ -147,10 +147,15 @@ class FusedAdam(torch.optim.Optimizer):
     steps; `last_grad_norm` is the norm of the last step that clipped (a device scalar).  All parameters must then live on
     one device."""
 
+    max_grad_norm = None           # (class attributes: a pickle or copy made without them steps unclipped)
+    last_grad_norm = None
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, grad_limit=1e5, max_grad_norm=None):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, grad_limit=grad_limit))
         self.max_grad_norm = None if max_grad_norm is None else _max_norm(max_grad_norm, 'FusedAdam')
-        self.last_grad_norm = None
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm)
 
     def load_state_dict(self, state_dict):
         """As torch.optim.Optimizer.load_state_dict; the step counts are brought back to the host afterwards (a
@@ -167,6 +172,10 @@ class FusedAdam(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if self.max_grad_norm is not None:
+            _max_norm(self.max_grad_norm, 'FusedAdam')
+            if len({group['grad_limit'] for group in self.param_groups}) > 1:
+                raise RuntimeError('FusedAdam: parameter groups that are clipped together must share grad_limit')
         work = []
         for group in self.param_groups:
             params, grads, ms, vs, steps = [], [], [], [], []
@@ -195,8 +204,6 @@ class FusedAdam(torch.optim.Optimizer):
             group, lists = work[0]
             self.last_grad_norm = adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], self.max_grad_norm)
         elif work:
-            if len({group['grad_limit'] for group, _ in work}) > 1:
-                raise RuntimeError('FusedAdam: parameter groups that are clipped together must share grad_limit')
             ext = _lib.ext()
             out = ext.grad_norm([g for _, lists in work for g in lists[1]], work[0][0]['grad_limit'], self.max_grad_norm, CLIP_EPS)
             for group, lists in work:

@@ -3,7 +3,7 @@
     y[..., :] = table[index[...]] * w_gain + b * b_gain                index [...] int32 / int64, table [V, F], b [F]
 
 The label embedding of a conditional network: what `self.embed(one_hot)` of the reference's mapping network
-(DissimilarDomains/training/networks.py:732, 748) computes with a product over all classes - bit for bit in float32 - given
+(DissimilarDomains/training/networks.py:765-842) computes with a product over all classes - bit for bit in float32 - given
 the class numbers themselves; `table` is then the layer's weight transposed (a view: no copy is made, and its gradient comes
 in the same layout).  The gradient sums the rows of dy that share an index in the order of the tokens, in float32 and without
 atomics, so that the same inputs give the same bits (`sg_embedding`, `sg_embedding_backward`).  The pair of functions is

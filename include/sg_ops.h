@@ -573,13 +573,14 @@ int sg_lerp_multi(const sg_lerp_params* p, sg_stream_t stream);
  * elements between rows or NULL, y [m, n] dense; all of `dtype` (SG_F32, SG_F16, SG_BF16), with float32 sums and one rounding.
  * act counts as in sg_bias_act (1 linear .. 9 swish); alpha is the slope of lrelu.  k == 0 gives z = b * b_gain.
  * For the backward pass the call also writes, where the pointer is not NULL, z [m, n] (float32) and positive [m, n] (z > 0).
- * It stands for the `FullyConnectedLayer.forward` of training/networks.py:691-700 (a library product and `bias_act`).
+ * It stands for the `FullyConnectedLayer.forward` of training/networks.py:691-704 (a library product and `bias_act`).
+ * ldx, ldw and, in the backward pass, n are below 2^23 bytes (SG_ERR_UNSUPPORTED otherwise); m, n, k below 2^31.
  *
  * Backward: with s = dy * act'(z), dy [m, n] dense,
  *   dx [m, k] = s w * (gain w_gain)     dw [n, k] = s^T x * (gain w_gain)     db [n] = column sums of s * (gain b_gain)
  * each dense, of `dtype`, and skipped when its pointer is NULL.  The slope comes from exactly one of: y (the layer's output, for
  * relu / lrelu without a residual and with gain != 0), positive (relu / lrelu), z (every other activation but linear, which
- * takes none).  p->b and p->residual are not read.  `workspace`: device memory, 16-byte aligned, private to the call until the
+ * takes none).  With y, a positive pre-activation value that the output rounds to zero counts as negative.  p->b and p->residual are not read.  `workspace`: device memory, 16-byte aligned, private to the call until the
  * stream has passed it.  Sums run in an order that depends on the sizes alone. */
 typedef struct sg_linear_params {
     const void* x;
@@ -605,7 +606,7 @@ int sg_linear_backward(const sg_linear_params* p, const void* dy, const void* y,
  * index [tokens] int32 or int64 (index_bytes 4 or 8, device memory); table [v, f] with strides in elements in either order,
  * bias [f] or NULL, y [tokens, f] dense; all of `dtype` (SG_F32, SG_F16, SG_BF16).  The product and the sum are rounded to
  * float32 one after the other, so that with float32 the result is bit for bit what a product with one-hot rows gives: it stands
- * for the label embedding `self.embed(c)` of training/networks.py:732, 748.  An index outside [0, v) yields a row of NaN.
+ * for the label embedding `self.embed(c)` of training/networks.py:765-842 (`MappingNetwork`).  An index outside [0, v) yields a row of NaN.
  *
  * Backward: p->table is the table's gradient, dense in either order ([v, f] or its transpose), 16-byte aligned, and written whole:
  *   dtable[v][f] = w_gain * sum over the tokens t with index[t] == v, in order, of dy[t][f]      (zero without tokens)

@@ -148,3 +148,33 @@ def test_python_entry_points_refuse_host_tensors():
     with pytest.raises(RuntimeError, match='negative'):
         optim_plugin.FusedAdam([p], max_grad_norm=-1.0)
     assert float(optim_plugin.grad_norm([])) == 0
+
+
+def test_copies_of_the_optimizer_clip_as_it_does():
+    """Copies and pickles keep max_grad_norm; a state from before it existed steps unclipped."""
+    import copy
+    import pickle
+    from ga_gan_amd import optim_plugin
+    opt = optim_plugin.FusedAdam([torch.nn.Parameter(torch.zeros(3))], max_grad_norm=0.5)
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert twin.max_grad_norm == 0.5 and twin.last_grad_norm is None
+    old = opt.__getstate__()
+    del old['max_grad_norm']
+    twin = optim_plugin.FusedAdam.__new__(optim_plugin.FusedAdam)
+    twin.__setstate__(old)
+    assert twin.max_grad_norm is None
+
+
+def test_a_step_that_is_refused_counts_for_nothing():
+    from ga_gan_amd import optim_plugin
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(2))
+    opt = optim_plugin.FusedAdam([dict(params=[p]), dict(params=[q], grad_limit=7.0)], max_grad_norm=1.0)
+    p.grad, q.grad = torch.ones(3), torch.ones(2)
+    with pytest.raises(RuntimeError, match='grad_limit'):
+        opt.step()
+    assert not opt.state[p] and not opt.state[q]
+    opt = optim_plugin.FusedAdam([p])
+    opt.max_grad_norm = -1.0
+    with pytest.raises(RuntimeError, match='negative'):
+        opt.step()
+    assert not opt.state[p]

@@ -156,6 +156,42 @@ def test_trainer_with_class_numbers_and_clipping(fused_dense):
     t.load_snapshot(state)
 
 
+def test_recorded_phases_with_class_numbers_and_clipping(fused_dense):
+    """A conditional trainer whose phases are recorded and replayed: a replay gives the gradients of a launch from the host on the
+    same parameters, labels and latents, and the steps clip."""
+    from ga_gan_amd.training import training_loop
+    opts = training_loop.setup_training_options(cfg='paper256', resolution=32, batch_size=4, c_dim=5, max_grad_norm=0.1, fp32=True, glrate=1e-5, dlrate=1e-5,
+                                                **training_loop.FULL)
+    opts['loss_kwargs'].update(style_mixing_prob=0, pl_weight=0)
+    t = training_loop.Trainer(rank=0, random_seed=1, use_graphs=True, **opts)
+    t.loss.synthesis_kwargs = dict(noise_mode='const')
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    for _ in range(3):                                              # host launches and recordings, then replays
+        real = torch.randint(0, 256, [4, 3, 32, 32], dtype=torch.uint8, device=DEV, generator=gen)
+        labels = torch.randint(0, 5, [4], device=DEV, generator=gen)
+        z = torch.randn([len(t.phases) * 4, 512], device=DEV, generator=gen)
+        gen_labels = torch.randint(0, 5, [len(t.phases) * 4], device=DEV, generator=gen)
+        t.step(real, labels, gen_z=z, gen_c=gen_labels)
+    assert set(t._graphs) == {'Gmain', 'Dmain', 'Dreg'}
+    real_f = real.float() / 127.5 - 1
+    for phase in t.phases:
+        if phase.name not in t._graphs:
+            continue
+        phase.opt.zero_grad(set_to_none=True)
+        training_loop.set_requires_grad(phase.module, parts=['all'])
+        t.loss.accumulate_gradients(phase=phase.name, real_img=real_f, real_c=labels, gen_z=z[:4], gen_c=gen_labels[:4], sync=True, gain=phase.interval)
+        phase.module.requires_grad_(False)
+        host = {n: p.grad.clone() for n, p in phase.module.named_parameters() if p.grad is not None}
+        for _ in range(3):
+            t._replay_phase(phase, real_f, labels, z[:4], gen_labels[:4])
+            torch.cuda.synchronize()
+            replay = {n: p.grad for n, p in phase.module.named_parameters() if p.grad is not None}
+            assert set(host) == set(replay)
+            num = sum(float((host[n].double() - replay[n].double()).square().sum()) for n in host)
+            assert math.sqrt(num / sum(float(v.double().square().sum()) for v in host.values())) <= 2e-2, phase.name     # (float atomics elsewhere)
+        assert math.isfinite(float(phase.opt.last_grad_norm))
+
+
 def test_launches_appear_in_a_recording():
     """The package's own per-launch timing sees the operators' launches."""
     from ga_gan_amd import _lib, optim_plugin

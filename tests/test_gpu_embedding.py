@@ -99,6 +99,31 @@ def test_table_sizes_at_a_digit_border(v, tokens):
     compare(index, table, b, dy)
 
 
+def test_indices_of_four_digits():
+    index, table, b, dy = make(5000, (1 << 24) + 5, 2, torch.float32)
+    index[:2], index[-1] = (1 << 24) + 4, 1 << 24
+    compare(index, table, b, dy)
+
+
+def test_more_than_32_bits_of_offset():
+    """A table and outputs beyond 2^32 bytes: rows on both sides of the border, exactly (gains of one, no bias, indices once)."""
+    v, f = (1 << 20) + 3, 2056
+    table = torch.empty([v, f], dtype=torch.bfloat16, device=DEV)
+    ramp = torch.arange(f, device=DEV)
+    number = torch.arange(v, device=DEV)
+    for i in range(0, v, 1 << 18):
+        part = number[i:i + (1 << 18), None] * 31 + ramp
+        table[i:i + (1 << 18)] = (part % 251).bfloat16()          # (whole numbers below 256 are bfloat16's)
+    index = torch.randperm(v, device=DEV)
+    table.requires_grad_(True)
+    y = op()(index, table)
+    for i in (0, 1 << 19, (1 << 20) - 2045, v - 3000):
+        assert torch.equal(y[i:i + 3000], table[index[i:i + 3000]])
+    grad, = torch.autograd.grad(y, table, y.detach())
+    for i in (0, 1 << 19, (1 << 20) - 2045, v - 3000):
+        assert torch.equal(grad[i:i + 3000], table[i:i + 3000])
+
+
 def test_strides_and_index_types():
     g = torch.Generator(device=DEV).manual_seed(1)
     big = torch.randn([60, 90], device=DEV, generator=g)

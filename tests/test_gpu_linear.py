@@ -79,6 +79,15 @@ def test_gains(kw, dtype):
     compare(*make(33, 64, 40, dtype), **kw)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('act', ['relu', 'lrelu'])
+@pytest.mark.parametrize('gain', [2.0 ** -22, -2.0 ** -22, 2.0 ** -9])
+def test_slope_where_the_output_rounds_to_zero(act, gain, dtype):
+    """Pre-activation values around one times 2^-22: most float16 outputs are zero, the slopes are not."""
+    x, w, b, _, dy = make(33, 64, 40, dtype)
+    compare(x * 0.125, w, b * 0.125, None, dy * 2 ** 12, act, gain=gain)
+
+
 def test_large_pre_activations():
     """Exponentials of +-300 must not turn into NaN."""
     x, w, b, r, dy = make(16, 8, 24, torch.float32)
@@ -102,6 +111,53 @@ def test_strides(dtype):
     compare(x[:1].expand(35, 64), w, b, r, dy)                    # rows at distance zero
     compare(x[:, :1], w[:, :1], b, None, dy)
     compare(big[:35, 5:6], big[:50, 9:10], b, None, dy)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_rows_far_apart(dtype):
+    """Rows 2^23 bytes apart and more are copied; rows of that length are refused."""
+    x, w, b, r, dy = make(3, 40, 5, dtype, residual=True)
+    far = (1 << 23) // x.element_size()
+    for step in (far - 8, far, far + 1):
+        big = torch.zeros(3 * step, dtype=dtype, device=DEV)
+        spread = torch.as_strided(big, x.shape, (step, 1))
+        spread.copy_(x)
+        compare(spread, w, b, r, dy)
+    with pytest.raises(RuntimeError, match='too long'):
+        op()(torch.zeros(2, far, dtype=dtype, device=DEV), torch.zeros(2, far, dtype=dtype, device=DEV))
+
+
+def test_more_than_32_bits_of_offset():
+    """A weight and outputs of 8 GiB, k at hand: rows on both sides of every 4 GiB border against 64 bits, elementwise within the
+    bounds; the gradients' sums run along the 2^17 rows."""
+    m, k, n = 1 << 17, 24, (1 << 15) + 8
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn([m, k], device=DEV, generator=g).bfloat16()
+    w = (torch.randn([n, k], device=DEV, generator=g) / 5).bfloat16()
+    b = torch.randn([n], device=DEV, generator=g).bfloat16()
+    rows = torch.tensor([0, 1, 65519, 65520, 65521, 65535, 65536, 131039, 131040, m - 2, m - 1], device=DEV)
+    y = op()(x, w, b, act='lrelu')
+    assert y.numel() * 2 > 1 << 33
+    check(y[rows], bounds(x[rows], w, b, None, 'lrelu')['y'], 'y')
+    sx, sw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(op()(sx, sw, act='linear'), (sx, sw), y)          # (y stands in for a gradient of its size)
+    check(dx[rows], bounds(x[rows], w, None, None, 'linear', y[rows])['dx'], 'dx')
+    for cols in (slice(0, 8), slice(n - 8, n)):
+        check(dw[cols], bounds(x, w[cols], None, None, 'linear', y[:, cols].contiguous())['dw'], 'dw')
+    # y as the weight: [m, n] with rows of n
+    v = torch.randn([3, n], device=DEV, generator=g).bfloat16()
+    sv, sy = v.clone().requires_grad_(True), y.requires_grad_(True)
+    out = op()(sv, sy, w_gain=0.01)
+    check(out.t()[rows].t(), bounds(v, y.detach()[rows], None, None, 'linear', w_gain=0.01)['y'], 'by a large weight')
+    dy = torch.randn([3, m], device=DEV, generator=g).bfloat16()
+    dv, dw = torch.autograd.grad(out, (sv, sy), dy)
+    assert dw.shape == y.shape
+    check(dw[rows], bounds(v, y.detach()[rows], None, None, 'linear', dy[:, rows].contiguous(), w_gain=0.01)['dw'], 'gradient of a large weight')
+    some = [0, 7, n - 1]
+    part = y.detach()[:, some].double()
+    want = dy.double() @ part * 0.01
+    bound = 0.01 * (m + 8) * 2.0 ** -24 * (dy.double().abs() @ part.abs()) + 2.0 ** -8 * want.abs()
+    assert bool(((dv[:, some].double() - want).abs() <= bound).all())
 
 
 def test_batch_dimensions():
@@ -181,6 +237,44 @@ def test_second_order(act):
     want = penalty(lambda *a: definition(*a, None, act, w_gain=0.7, b_gain=0.5), *[t.double().detach().requires_grad_(True) for t in (x, w, b)])
     for a, e in zip(got, want):
         assert float((a.double() - e).abs().max()) <= 1e-4 * float(e.abs().max())
+
+
+def test_second_order_without_bias_and_with_residual():
+    """As above; the residual's own path is linear."""
+    x, w, _, r, dy = make(12, 40, 30, torch.float32, residual=True)
+
+    def penalty(f, *leaves):
+        y = f(*leaves)
+        g = torch.autograd.grad(y, leaves[:2], dy.to(y.dtype), create_graph=True)
+        return torch.autograd.grad(sum(t.square().sum() for t in g) + y.square().sum(), leaves)
+
+    got = penalty(lambda a, b, c: op()(a, b, residual=c, act='lrelu', gain=0.8), *[t.clone().requires_grad_(True) for t in (x, w, r)])
+    want = penalty(lambda a, b, c: definition(a, b, None, c, 'lrelu', gain=0.8), *[t.double().detach().requires_grad_(True) for t in (x, w, r)])
+    for a, e in zip(got, want):
+        assert float((a.double() - e).abs().max()) <= 1e-4 * float(e.abs().max())
+
+
+def test_nothing_outlives_its_graph():
+    """The output that is kept for the slopes does not hold its own graph (a graph that lives on keeps its leaves' accumulators
+    on the eager stream, which a recorded backward pass would then join)."""
+    x, w, b, _, dy = make(64, 64, 64, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    torch.autograd.grad(op()(*leaves, act='lrelu'), leaves, dy)
+    before = torch.cuda.memory_allocated()
+    for act in ACTS:
+        y = op()(*leaves, act=act)
+        torch.autograd.grad(y, leaves, dy)
+        del y
+        assert torch.cuda.memory_allocated() == before
+
+
+def test_output_changed_in_place_is_noticed():
+    x, w, b, _, dy = make(8, 16, 8, torch.float32)
+    x.requires_grad_(True)
+    y = op()(x, w, b, act='lrelu')
+    y.mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward(dy)
 
 
 def test_partial_gradients():
