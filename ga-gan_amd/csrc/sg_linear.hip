@@ -376,8 +376,10 @@ template <class F, int... K> __device__ __forceinline__ void for_each(F f, std::
 
 enum { kDirect, kLoose, kShort };
 
+template <int BI, int BJ, int KK> constexpr int kTileBytes = (KK == 1 ? 4 : 2) * (BI + BJ) * KK * kPartBytes;      // LDS of a workgroup
+
 template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int KK, int MODE>
-__global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
+__device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned char* smem) {
     constexpr bool FORWARD = ROWS_A && ROWS_B;
     constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = KK * kPartBytes / (int)sizeof(T);
     constexpr int RING = KK == 1 ? 4 : 2;                 // tiles of that many steps in LDS
@@ -385,13 +387,12 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     using TileB = Tile<T, BJ, ROWS_B, KK, THREADS>;
     using FragA = Frags<T, BI, ROWS_A, KK, THREADS, TI>;
     using FragB = Frags<T, BJ, ROWS_B, KK, THREADS, TJ>;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[RING * (TileA::BYTES + TileB::BYTES)];
     constexpr int BUF = TileA::BYTES + TileB::BYTES;
+    static_assert(RING * BUF == kTileBytes<BI, BJ, KK>, "the kernel's LDS");
 
     // Workgroups go round robin over the 8 XCDs: each XCD gets a contiguous share of the tiles, in groups of 8 tile rows so that
     // the tiles it works on at one time share rows of A and columns of B in its L2.
     const unsigned tiles = (unsigned)g.tiles_i * g.tiles_j, total = tiles * g.slices;
-    unsigned id = blockIdx.x;
     {
         const unsigned per = total / 8, extra = total % 8, xcd = id % 8, k = id / 8;
         id = xcd * per + (xcd < extra ? xcd : extra) + k;
@@ -764,6 +765,12 @@ __global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g)
     }
 }
 
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int KK, int MODE>
+__global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ, KK>];
+    gemm_tile<T, BI, BJ, WI, WJ, ROWS_A, ROWS_B, KK, MODE>(g, blockIdx.x, smem);
+}
+
 // Few rows (at most 32) and a short sum: the tile kernel would spend most of its products on rows that are not there, and need
 // slices and a second launch to use more than a few CUs.  Here eight waves share the sum of 16 (ROWS_B) or 32 columns: operands go
 // from global memory to fragments, 64 bytes of p per wave and turn (the eight waves' turns lie side by side), the waves' sums are
@@ -839,9 +846,8 @@ __global__ void __launch_bounds__(512) linear_thin_kernel(const Gemm g) {
 }
 
 // The slices' partial sums, added in slice order, and the epilogue.
-template <class T, int RUN, bool FORWARD>
-__global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
-    const int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * RUN;
+template <class T, int RUN, bool FORWARD> __device__ __forceinline__ void join_slices(const Gemm& g, unsigned block) {
+    const int64_t k = ((int64_t)block * 256 + threadIdx.x) * RUN;
     const int64_t plane = g.ni * g.nj;
     if (k >= plane) return;
     float v[RUN];
@@ -859,6 +865,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) {
     }
     finish<T, RUN, FORWARD>(g, k / g.nj, k % g.nj, v);
 }
+
+template <class T, int RUN, bool FORWARD> __global__ void __launch_bounds__(256) linear_join_kernel(const Gemm g) { join_slices<T, RUN, FORWARD>(g, blockIdx.x); }
 
 // ---- the activation's gradient and column sums ----------------------------------------------------------------------------------
 
@@ -938,27 +946,72 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(1024) column_join_kernel(const float* __restrict__ partial, int blocks, int64_t cols, float scale, T* __restrict__ out) {
-    __shared__ float part[16][64];
+struct ColumnJoin {
+    const float* partial;                // [blocks][cols]
+    void* out;                           // [cols]
+    int64_t cols;
+    int blocks;
+    float scale;
+};
+
+// 64 columns a workgroup of WAVES waves: sixteen shares of every 16th partial sum, four under way at a time, whichever waves take them.
+template <class T, int WAVES> __device__ __forceinline__ void join_columns(const ColumnJoin& p, unsigned block, float* part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-    float sum = 0.f;
-    for (int b = wave; b < blocks; b += 16 * 4) {
-        float v[4];
+    const int64_t c = (int64_t)block * 64 + lane;
 #pragma unroll
-        for (int u = 0; u < 4; u++) v[u] = b + 16 * u < blocks && c < cols ? partial[(int64_t)(b + 16 * u) * cols + c] : 0.f;
+    for (int share = wave; share < 16; share += WAVES) {
+        float sum = 0.f;
+        for (int b = share; b < p.blocks; b += 16 * 4) {
+            float v[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) sum += v[u];
+            for (int u = 0; u < 4; u++) v[u] = b + 16 * u < p.blocks && c < p.cols ? p.partial[(int64_t)(b + 16 * u) * p.cols + c] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 4; u++) sum += v[u];
+        }
+        part[share * 64 + lane] = sum;
     }
-    part[wave][lane] = sum;
     __syncthreads();
-    if (wave == 0 && c < cols) {
-        sum = 0.f;
+    if (wave == 0 && c < p.cols) {
+        float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 16; w++) sum += part[w][lane];
-        out[c] = Elem<T>::store(sum * scale);
+        for (int share = 0; share < 16; share++) sum += part[share * 64 + lane];
+        ((T*)p.out)[c] = Elem<T>::store(sum * p.scale);
     }
+}
+
+template <class T> __global__ void __launch_bounds__(1024) column_join_kernel(const ColumnJoin p) {
+    __shared__ float part[16 * 64];
+    join_columns<T, 16>(p, blockIdx.x, part);
+}
+
+// ---- both gradients in one launch ---------------------------------------------------------------------------------------------------
+// The gradients of x and w read the same s and do not wait for each other: where both are made of 64 x 64 tiles, one launch holds
+// the tiles of both and the last sums of the bias gradient, and one more joins the slices of both.  All three gradients, us with a
+// launch each (few rows: linear_thin_kernel for x) and so: float32 512 -> 512 with 32 rows 13.7 and 10.7, 256 rows 21 and 14.7, 10000
+// rows 107 and 100; 8192 -> 512 with 64 rows 27 and 22; bfloat16 1024 -> 1024 with 1024 rows 27 and 16.5.
+struct Pair {
+    Gemm x, w;
+    ColumnJoin columns;
+    unsigned blocks_x, blocks_w;         // then the columns' workgroups
+    int x_first;                         // the longer sums start first, or they would end last and alone
+};
+
+template <class T, int MODE> __global__ void __launch_bounds__(256) linear_pair_kernel(const Pair p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<64, 64, 2>];
+    const unsigned first_x = p.x_first ? 0 : p.blocks_w, first_w = p.x_first ? p.blocks_x : 0;
+    if (blockIdx.x - first_x < p.blocks_x) gemm_tile<T, 64, 64, 2, 2, true, false, 2, MODE>(p.x, blockIdx.x - first_x, smem);
+    else if (blockIdx.x - first_w < p.blocks_w) gemm_tile<T, 64, 64, 2, 2, false, false, 2, MODE>(p.w, blockIdx.x - first_w, smem);
+    else join_columns<T, 4>(p.columns, blockIdx.x - p.blocks_x - p.blocks_w, reinterpret_cast<float*>(smem));
+}
+
+template <class T> __device__ __forceinline__ void join_slices_either(const Gemm& g, unsigned block) {
+    if (g.whole) join_slices<T, 4, false>(g, block);
+    else join_slices<T, 1, false>(g, block);
+}
+
+template <class T> __global__ void __launch_bounds__(256) linear_pair_join_kernel(const Pair p) {       // blocks_x, blocks_w: of this launch
+    if (blockIdx.x < p.blocks_x) join_slices_either<T>(p.x, blockIdx.x);
+    else join_slices_either<T>(p.w, blockIdx.x - p.blocks_x);
 }
 
 // ---- operands whose rows are not whole packets ------------------------------------------------------------------------------------
@@ -1011,7 +1064,9 @@ int slope_rows(int64_t rows, int64_t cols) {
 
 int64_t slope_blocks(int64_t rows, int64_t cols) { return rows == 0 ? 0 : (rows + slope_rows(rows, cols) - 1) / slope_rows(rows, cols); }
 
-template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* what) {
+// columns: where given, receives the last sums over the row blocks instead of their launch (no blocks: there are none to make).
+template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* what, ColumnJoin* columns = nullptr) {
+    if (columns) columns->blocks = 0;
     if (p.cols == 0) return SG_OK;
     p.rows_per_block = slope_rows(p.rows, p.cols);
     constexpr int N = Pack<T>::N;
@@ -1032,8 +1087,11 @@ template <class T> int run_slope(SlopeParams p, hipStream_t stream, const char* 
     else if (p.z) SG_SLOPE(kByZ);
     else SG_SLOPE(kByNothing);
 #undef SG_SLOPE
-    if (p.sums && by > 1)
-        hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((p.cols + 63) / 64)), dim3(1024), 0, stream, p.partial, (int)by, p.cols, p.scale, (T*)p.sums);
+    if (p.sums && by > 1) {
+        const ColumnJoin join{p.partial, p.sums, p.cols, (int)by, p.scale};
+        if (columns) *columns = join;
+        else hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((p.cols + 63) / 64)), dim3(1024), 0, stream, join);
+    }
     return check_launch(what);
 }
 
@@ -1096,18 +1154,43 @@ template <class T, int TILE, bool RA, bool RB, int MODE> void launch_gemm(const 
     hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, KK, MODE>), grid, dim3(256), 0, stream, g);
 }
 
-template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
+// How a product's operands can travel, and the tiles that follow from it.
+struct Route {
+    bool thin = false, direct = false, is_short = false;
+    int tile = 0;
+};
+
+template <class T, bool RA, bool RB> int route_gemm(Gemm& g, const Shape& s, Route& r, const char* what) {
     constexpr int ES = sizeof(T), E = 16 / ES;
-    if (g.ni == 0 || g.nj == 0) return SG_OK;
     g.tiles_i = s.tiles_i; g.tiles_j = s.tiles_j; g.slices = s.slices; g.slice_steps = s.slice_steps;
     // offsets within a tile's lines are 32-bit
     SG_REQUIRE((g.lda + 1) * ES * 256 < (int64_t)kOutside && (g.ldb + 1) * ES * 256 < (int64_t)kOutside, SG_ERR_UNSUPPORTED,
                "%s: rows of %lld / %lld elements are too long", what, (long long)g.lda, (long long)g.ldb);
-    const bool direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && ((RA ? g.np : g.ni) % E == 0 || g.a_padded) &&
-                        ((RB ? g.np : g.nj) % E == 0 || g.b_padded);
+    r.direct = aligned16(g.a) && aligned16(g.b) && g.lda % E == 0 && g.ldb % E == 0 && ((RA ? g.np : g.ni) % E == 0 || g.a_padded) &&
+               ((RB ? g.np : g.nj) % E == 0 || g.b_padded);
     g.whole = runs_aligned<T>(g);
-    if constexpr (RA && (RB || ES == 4)) {
-        if (s.thin && aligned16(g.a) && g.lda % E == 0 && (RB ? aligned16(g.b) && g.ldb % E == 0 : reinterpret_cast<uintptr_t>(g.b) % 8 == 0 && g.ldb % 2 == 0)) {
+    r.thin = RA && (RB || ES == 4) && s.thin && aligned16(g.a) && g.lda % E == 0 &&
+             (RB ? aligned16(g.b) && g.ldb % E == 0 : reinterpret_cast<uintptr_t>(g.b) % 8 == 0 && g.ldb % 2 == 0);
+    // (operands that travel by way of registers are those of small products: others are copied into packets first)
+    r.tile = r.direct ? s.tile : 64;
+    if (r.tile != s.tile) {
+        g.tiles_i = (int)((g.ni + 63) / 64);
+        g.tiles_j = (int)((g.nj + 63) / 64);
+    }
+    SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    r.is_short = (RA ? g.np : g.ni) < E || (RB ? g.np : g.nj) < E;
+    return SG_OK;
+}
+
+int64_t join_blocks(const Gemm& g) { return g.slices > 1 ? (g.ni * g.nj / (g.whole ? 4 : 1) + 255) / 256 : 0; }
+
+template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStream_t stream, const char* what) {
+    if (g.ni == 0 || g.nj == 0) return SG_OK;
+    Route r;
+    const int rc = route_gemm<T, RA, RB>(g, s, r, what);
+    if (rc != SG_OK) return rc;
+    if constexpr (RA && (RB || sizeof(T) == 4)) {
+        if (r.thin) {
             const int cols = RB ? 16 : 32;
             const dim3 grid((unsigned)((g.nj + cols - 1) / cols));
             if (g.ni <= 16) hipLaunchKernelGGL((linear_thin_kernel<T, 1, RB>), grid, dim3(512), 0, stream, g);
@@ -1115,30 +1198,44 @@ template <class T, bool RA, bool RB> int run_gemm(Gemm g, const Shape& s, hipStr
             return check_launch(what);
         }
     }
-    // (operands that travel by way of registers are those of small products: others are copied into packets first)
-    const int tile = direct ? s.tile : 64;
-    if (tile != s.tile) {
-        g.tiles_i = (int)((g.ni + 63) / 64);
-        g.tiles_j = (int)((g.nj + 63) / 64);
+    if constexpr (sizeof(T) == 2) {
+        if (r.tile == 256) launch_gemm<T, 256, RA, RB, kDirect>(g, stream);
+        if (r.tile == 128) launch_gemm<T, 128, RA, RB, kDirect>(g, stream);
     }
-    SG_REQUIRE((int64_t)g.tiles_i * g.tiles_j * g.slices <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
-    const bool is_short = (RA ? g.np : g.ni) < E || (RB ? g.np : g.nj) < E;
-    if constexpr (ES == 2) {
-        if (tile == 256) launch_gemm<T, 256, RA, RB, kDirect>(g, stream);
-        if (tile == 128) launch_gemm<T, 128, RA, RB, kDirect>(g, stream);
-    }
-    if (tile == 64) {
-        if (direct) launch_gemm<T, 64, RA, RB, kDirect>(g, stream);
-        else if (is_short) launch_gemm<T, 64, RA, RB, kShort>(g, stream);
+    if (r.tile == 64) {
+        if (r.direct) launch_gemm<T, 64, RA, RB, kDirect>(g, stream);
+        else if (r.is_short) launch_gemm<T, 64, RA, RB, kShort>(g, stream);
         else launch_gemm<T, 64, RA, RB, kLoose>(g, stream);
     }
-    if (g.slices > 1) {
-        const int run = g.whole ? 4 : 1;
-        const int64_t blocks = (g.ni * g.nj / run + 255) / 256;
-        SG_REQUIRE(blocks <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
-        if (g.whole) hipLaunchKernelGGL((linear_join_kernel<T, 4, RA && RB>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
-        else hipLaunchKernelGGL((linear_join_kernel<T, 1, RA && RB>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+    const int64_t blocks = join_blocks(g);
+    SG_REQUIRE(blocks <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    if (blocks && g.whole) hipLaunchKernelGGL((linear_join_kernel<T, 4, RA && RB>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+    else if (blocks) hipLaunchKernelGGL((linear_join_kernel<T, 1, RA && RB>), dim3((unsigned)blocks), dim3(256), 0, stream, g);
+    return check_launch(what);
+}
+
+// The two products of the backward pass (w's partial sums lie behind x's) and the columns that run_slope left.
+template <class T> int run_pair(Gemm x, const Shape& sx, Gemm w, const Shape& sw, const ColumnJoin& columns, hipStream_t stream, const char* what) {
+    Route rx, rw;
+    int rc = route_gemm<T, true, false>(x, sx, rx, what);
+    if (rc == SG_OK) rc = route_gemm<T, false, false>(w, sw, rw, what);
+    if (rc != SG_OK) return rc;
+    Pair p{x, w, columns, (unsigned)(x.tiles_i * x.tiles_j * x.slices), (unsigned)(w.tiles_i * w.tiles_j * w.slices), x.slice_steps >= w.slice_steps};
+    const bool direct = rx.direct && rw.direct, loose = !rx.is_short && !rw.is_short;
+    if (rx.tile != 64 || rw.tile != 64 || !(direct || loose)) {
+        if (columns.blocks)
+            hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((columns.cols + 63) / 64)), dim3(1024), 0, stream, columns);
+        rc = run_gemm<T, true, false>(x, sx, stream, what);
+        return rc != SG_OK ? rc : run_gemm<T, false, false>(w, sw, stream, what);
     }
+    const int64_t blocks = (int64_t)p.blocks_x + p.blocks_w + (columns.blocks ? (columns.cols + 63) / 64 : 0);
+    SG_REQUIRE(blocks <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    if (direct) hipLaunchKernelGGL((linear_pair_kernel<T, kDirect>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((linear_pair_kernel<T, kLoose>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    const int64_t jx = join_blocks(x), jw = join_blocks(w);
+    SG_REQUIRE(jx + jw <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
+    p.blocks_x = (unsigned)jx;
+    if (jx + jw) hipLaunchKernelGGL((linear_pair_join_kernel<T>), dim3((unsigned)(jx + jw)), dim3(256), 0, stream, p);
     return check_launch(what);
 }
 
@@ -1221,7 +1318,7 @@ ForwardPlan plan_forward(const sg_linear_params& p) {
 struct BackwardPlan {
     Shape dx, dw;
     Operand x, w, s;                      // s: the activation's gradient, or dy (copied only for its own n)
-    size_t sums = 0, partial = 0, total = 0;
+    size_t sums = 0, partial = 0, partial_w = 0, total = 0;
 };
 
 BackwardPlan plan_backward(const sg_linear_params& p) {
@@ -1241,7 +1338,8 @@ BackwardPlan plan_backward(const sg_linear_params& p) {
     b.dx = shape_of(p.dtype, 1, p.m, p.k, p.n);
     b.dw = shape_of(p.dtype, 2, p.n, p.k, p.m);
     b.partial = at;
-    at += std::max(b.dx.partial_bytes, b.dw.partial_bytes);
+    b.partial_w = at + b.dx.partial_bytes;
+    at += b.dx.partial_bytes + b.dw.partial_bytes;
     place_operands(p, at, b.x, b.w);
     b.total = at;
     return b;
@@ -1338,6 +1436,8 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         SG_DISPATCH_16_32(p->dtype, done = run_pack<T>(q, copies, stream, "sg_linear_backward"));
         if (done != SG_OK) return done;
     }
+    ColumnJoin columns{};
+    const bool pair = products && dx && dw && p->k > 0;
     if ((own_s && products) || db) {
         SlopeParams r{};
         r.dy = dy; r.y = y; r.positive = positive; r.z = z;
@@ -1351,30 +1451,25 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         r.sign = p->gain < 0.f ? -1.f : 1.f;
         r.scale = p->gain * p->b_gain;
         int done = SG_OK;
-        SG_DISPATCH_16_32(p->dtype, done = run_slope<T>(r, stream, "sg_linear_backward"));
+        SG_DISPATCH_16_32(p->dtype, done = run_slope<T>(r, stream, "sg_linear_backward", pair ? &columns : nullptr));
         if (done != SG_OK) return done;
     }
-    Gemm g{};
-    g.partial = (float*)(ws + plan.partial);
-    g.scale = p->gain * p->w_gain;
-    g.a = plan.s.p; g.lda = plan.s.ld; g.a_padded = plan.s.padded;
-    if (dx) {                            // [m, k] = s [m, n] w [n, k]
-        Gemm q2 = g;
-        q2.b = plan.w.p; q2.ldb = plan.w.ld; q2.b_padded = plan.w.padded;
-        q2.ni = p->m; q2.nj = p->k; q2.np = p->n;
-        q2.out = dx;
-        int done = SG_OK;
-        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, true, false>(q2, plan.dx, stream, "sg_linear_backward")));
-        if (done != SG_OK) return done;
+    Gemm gx{}, gw{};
+    gx.scale = gw.scale = p->gain * p->w_gain;
+    gx.a = gw.a = plan.s.p; gx.lda = gw.lda = plan.s.ld; gx.a_padded = gw.a_padded = plan.s.padded;
+    gx.partial = (float*)(ws + plan.partial);                      // [m, k] = s [m, n] w [n, k]
+    gx.b = plan.w.p; gx.ldb = plan.w.ld; gx.b_padded = plan.w.padded;
+    gx.ni = p->m; gx.nj = p->k; gx.np = p->n;
+    gx.out = dx;
+    gw.partial = (float*)(ws + plan.partial_w);                    // [n, k] = s [m, n]^T x [m, k]
+    gw.b = plan.x.p; gw.ldb = plan.x.ld; gw.b_padded = plan.x.padded;
+    gw.ni = p->n; gw.nj = p->k; gw.np = p->m;
+    gw.out = dw;
+    if (pair) {
+        SG_DISPATCH_16_32(p->dtype, return run_pair<T>(gx, plan.dx, gw, plan.dw, columns, stream, "sg_linear_backward"));
     }
-    if (dw) {                            // [n, k] = s [m, n]^T x [m, k]
-        Gemm q2 = g;
-        q2.b = plan.x.p; q2.ldb = plan.x.ld; q2.b_padded = plan.x.padded;
-        q2.ni = p->n; q2.nj = p->k; q2.np = p->m;
-        q2.out = dw;
-        int done = SG_OK;
-        SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, false, false>(q2, plan.dw, stream, "sg_linear_backward")));
-        if (done != SG_OK) return done;
-    }
-    return SG_OK;
+    int done = SG_OK;
+    if (dx) SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, true, false>(gx, plan.dx, stream, "sg_linear_backward")));
+    if (dw && done == SG_OK) SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, false, false>(gw, plan.dw, stream, "sg_linear_backward")));
+    return done;
 }

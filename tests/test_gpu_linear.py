@@ -277,6 +277,19 @@ def test_output_changed_in_place_is_noticed():
         y.backward(dy)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('size', [(40, 64, 24), (300, 129, 65), (64, 4096, 200), (700, 96, 640)])
+def test_partial_gradients_of_sizes(size, dtype):
+    """One gradient at a time, or all of them: the same bits."""
+    x, w, b, r, dy = make(*size, dtype)
+    full = run(x, w, b, None, dy, 'tanh')[1]
+    for wanted in ([0], [1], [2], [0, 1], [1, 2]):
+        leaves = [t.detach().clone().requires_grad_(i in wanted) for i, t in enumerate((x, w, b))]
+        y = op()(*leaves, act='tanh')
+        for i, g in zip(wanted, torch.autograd.grad(y, [leaves[i] for i in wanted], dy)):
+            assert torch.equal(g, full[('dx', 'dw', 'db')[i]])
+
+
 def test_partial_gradients():
     x, w, b, r, dy = make(40, 64, 24, torch.float32, residual=True)
     full = run(x, w, b, r, dy)[1]
