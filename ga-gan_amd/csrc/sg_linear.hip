@@ -702,7 +702,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
             else edge ? rounds(No{}, Yes{}) : rounds(No{}, No{});
         } else if (g.slices == 1) {
             // Rows that start anywhere: a lane takes single elements, neighbouring lanes neighbouring columns.
-            constexpr int SETS = COLS > 64 ? COLS / 64 : 1, STRIDE = COLS > 64 ? 1 : 64 / COLS, U = 8;     // columns per lane; rows per round
+            constexpr int SETS = COLS > 64 ? COLS / 64 : 1, STRIDE = COLS > 64 ? 1 : 64 / COLS, U = sizeof(T) == 2 ? 8 : 4;     // columns per lane; rows per round
             static_assert(S_PASS * 16 % (STRIDE * U) == 0, "whole rounds");
 #pragma unroll 1
             for (int set = 0; set < SETS; set++) {
@@ -765,8 +765,9 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     }
 }
 
+// (64 x 64: five workgroups on a CU, as many as its LDS holds.  float32 10000 x 512 -> 512, 1256 of them: 55 us with four, 49 with five)
 template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int KK, int MODE>
-__global__ void __launch_bounds__(WI * WJ * 64) linear_gemm_kernel(const Gemm g) {
+__global__ void __launch_bounds__(WI * WJ * 64, BI == 64 && MODE == kDirect ? 5 : 1) linear_gemm_kernel(const Gemm g) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ, KK>];
     gemm_tile<T, BI, BJ, WI, WJ, ROWS_A, ROWS_B, KK, MODE>(g, blockIdx.x, smem);
 }
