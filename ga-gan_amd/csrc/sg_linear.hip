@@ -3,7 +3,7 @@
 //   s = dy * act'(z)      dx = s w * (gain w_gain)    dw = s^T x * (gain w_gain)    db = sum over rows of s * (gain b_gain)
 // Three matrix products that differ in which index of each operand is contiguous; one kernel template covers them:
 //   C[i, j] = sum over p of A(i, p) B(j, p),   each operand stored with p contiguous ("rows") or with i / j contiguous ("columns").
-// An operand is never transposed in memory.  Tiles of 64 or 128 bytes along p travel to LDS as they lie (16 bytes per lane, straight
+// An operand is never transposed in memory.  Tiles of 128 bytes along p travel to LDS as they lie (16 bytes per lane, straight
 // into LDS where rows are 16-byte aligned), and a fragment of a "columns" operand is read by the transposing LDS read (16-bit)
 // or four rows at a time (float32).  16-bit operands multiply on v_mfma_f32_16x16x32, float32 ones on v_mfma_f32_16x16x4_f32,
 // whose products and sums are plain float32.  All sums are float32; every output is rounded once.
@@ -28,7 +28,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kPartBytes = 64;                     // of p per product: 32 16-bit or 4 x 4 float32 elements; a step has KK parts
+constexpr int kStepBytes = 128;                    // of p per step: two halves of 32 16-bit elements (one product) or 16 float32 ones (four)
 constexpr unsigned kOutside = 0x80000000u;         // a buffer offset beyond every descriptor: the load yields zeros
 
 enum { kActLinear = 1, kActRelu, kActLrelu, kActTanh, kActSigmoid, kActElu, kActSelu, kActSoftplus, kActSwish };
@@ -104,7 +104,7 @@ struct Gemm {
     const void* b;                       // operand of the columns j
     int64_t lda, ldb;                    // elements between rows as stored
     int64_t ni, nj, np;
-    int tiles_i, tiles_j, slices, slice_steps;           // slice_steps: of 128 bytes along p
+    int tiles_i, tiles_j, slices, slice_steps;           // slice_steps: steps of 128 bytes along p
     int a_padded, b_padded;              // its rows go on with zeros to whole 16-byte packets
     float* partial;                      // [slices][ni][nj] when slices > 1
     void* out;                           // [ni][nj]
@@ -188,7 +188,7 @@ template <int PLACE> __device__ __forceinline__ void copy_to_lds(i32x4_t from, u
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
-// One operand's tile of SIDE rows i (or j) by KK * 64 bytes of p in LDS: slots of 16 bytes, slot k * THREADS + t filled by thread t.
+// One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: slots of 16 bytes, slot k * THREADS + t filled by thread t.
 //   ROWS:  slot (row, c) holds the 16 bytes c ^ turn(row) of the row: the lanes that read at one time - 16 rows at one c, or 8 rows
 //          each at two - hit 16 different 16-byte banks.
 //   !ROWS: lines of SIDE elements at one p.  16-bit: the 32-byte block c of line q holds block c ^ swizzle(q), so that the
@@ -196,8 +196,8 @@ __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigne
 //          p = p_of(q): where a thread fills every 8th line (256 columns), bits 2 and 3 trade places, so that a thread's slots
 //          share one swizzle.
 // Either way a thread's slots are one address and constant distances apart.
-template <class T, int SIDE, bool ROWS, int KK, int THREADS> struct Tile {
-    static constexpr int ES = sizeof(T), E = 16 / ES, PITCH = KK * kPartBytes, BK = PITCH / ES;
+template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
+    static constexpr int ES = sizeof(T), E = 16 / ES, PITCH = kStepBytes, BK = PITCH / ES;
     static constexpr int BYTES = SIDE * PITCH;
     static constexpr int LOADS = BYTES / 16 / THREADS;             // 16-byte slots per thread
     static constexpr int LINE = ROWS ? PITCH / 16 : SIDE / E;      // slots per row or line
@@ -206,7 +206,7 @@ template <class T, int SIDE, bool ROWS, int KK, int THREADS> struct Tile {
     static_assert(LOADS >= 1 && LOADS * THREADS * 16 == BYTES, "slots divide among the threads");
     static_assert(ROWS ? APART % 16 == 0 : ES == 4 || APART % 16 == 0 || SWAP, "a thread's slots share one swizzle");
 
-    static __device__ __forceinline__ constexpr int turn(int row) { return KK == 2 ? (row >> 1) & 7 : -(row >> 2) & 3; }
+    static __device__ __forceinline__ constexpr int turn(int row) { return (row >> 1) & 7; }
     static __device__ __forceinline__ constexpr int p_of(int q) { return SWAP ? (q & ~12) | (q & 4) << 1 | (q & 8) >> 1 : q; }
     static __device__ __forceinline__ int swizzle(int q) {
         if (ES == 4) return 0;
@@ -290,9 +290,9 @@ template <class T, int SIDE, bool ROWS, int KK, int THREADS> struct Tile {
     }
 };
 
-// Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for part kk of a step.
-template <class T, int SIDE, bool ROWS, int KK, int THREADS, int COUNT> struct Frags {
-    using Here = Tile<T, SIDE, ROWS, KK, THREADS>;
+// Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for half kk of a step.
+template <class T, int SIDE, bool ROWS, int THREADS, int COUNT> struct Frags {
+    using Here = Tile<T, SIDE, ROWS, THREADS>;
     static constexpr int V = sizeof(T) == 4 && !ROWS ? (COUNT >= 4 ? 4 : COUNT) : 1;   // tiles whose rows interleave
     uint4 q[COUNT];                                                                   // 8 16-bit values, or 4 float32 (ROWS)
     float f[sizeof(T) == 4 && !ROWS ? COUNT : 1][4];
@@ -376,19 +376,20 @@ template <class F, int... K> __device__ __forceinline__ void for_each(F f, std::
 
 enum { kDirect, kLoose, kShort };
 
-template <int BI, int BJ, int KK> constexpr int kTileBytes = (KK == 1 ? 4 : 2) * (BI + BJ) * KK * kPartBytes;      // LDS of a workgroup
+// LDS of a workgroup: two steps of both operands, and a third one of A where it is alone on its CU, or one of two
+template <int BI, int BJ> constexpr int kRingA = BI >= 128 ? 3 : 2;
+template <int BI, int BJ> constexpr int kTileBytes = (kRingA<BI, BJ> * BI + 2 * BJ) * kStepBytes;
 
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int KK, int MODE>
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
 __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned char* smem) {
     constexpr bool FORWARD = ROWS_A && ROWS_B;
-    constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = KK * kPartBytes / (int)sizeof(T);
-    constexpr int RING = KK == 1 ? 4 : 2;                 // tiles of that many steps in LDS
-    using TileA = Tile<T, BI, ROWS_A, KK, THREADS>;
-    using TileB = Tile<T, BJ, ROWS_B, KK, THREADS>;
-    using FragA = Frags<T, BI, ROWS_A, KK, THREADS, TI>;
-    using FragB = Frags<T, BJ, ROWS_B, KK, THREADS, TJ>;
+    constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
+    constexpr int RING_A = kRingA<BI, BJ>;            // steps of A in LDS; two of B behind them
+    using TileA = Tile<T, BI, ROWS_A, THREADS>;
+    using TileB = Tile<T, BJ, ROWS_B, THREADS>;
+    using FragA = Frags<T, BI, ROWS_A, THREADS, TI>;
+    using FragB = Frags<T, BJ, ROWS_B, THREADS, TJ>;
     constexpr int BUF = TileA::BYTES + TileB::BYTES;
-    static_assert(RING * BUF == kTileBytes<BI, BJ, KK>, "the kernel's LDS");
 
     // Workgroups go round robin over the 8 XCDs: each XCD gets a contiguous share of the tiles, in groups of 8 tile rows so that
     // the tiles it works on at one time share rows of A and columns of B in its L2.
@@ -406,7 +407,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     const T* b = (const T*)g.b + (ROWS_B ? j0 * g.ldb : j0);
     const int left_i = (int)min(g.ni - i0, (int64_t)BI), left_j = (int)min(g.nj - j0, (int64_t)BJ);
     const int steps_all = (int)((g.np + BK - 1) / BK);
-    const int first = (int)slice * g.slice_steps * (2 / KK), steps = min(g.slice_steps * (2 / KK), steps_all - first);
+    const int first = (int)slice * g.slice_steps, steps = min(g.slice_steps, steps_all - first);
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
@@ -421,114 +422,122 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     const typename TileB::Slots sb = TileB::plan(g.ldb, left_j);
     auto at_a = [&](int step) { return a + (ROWS_A ? (int64_t)step * BK : (int64_t)step * BK * g.lda); };
     auto at_b = [&](int step) { return b + (ROWS_B ? (int64_t)step * BK : (int64_t)step * BK * g.ldb); };
+    auto multiply = [&](const FragA& fa, const FragB& fb, int t, int s) {
+        if constexpr (sizeof(T) == 2) {
+            mfma_in_place(acc[t][s], fb.q[t], fa.q[s], T());
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb.value(t, e), fa.value(s, e), acc[t][s], 0, 0, 0);
+        }
+    };
     // column tile t of the wave's part
     auto multiply_tile = [&](const FragA& fa, const FragB& fb, int t) {
 #pragma unroll
-        for (int s = 0; s < TI; s++) {
-            if constexpr (sizeof(T) == 2) {
-                mfma_in_place(acc[t][s], fb.q[t], fa.q[s], T());
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb.value(t, e), fa.value(s, e), acc[t][s], 0, 0, 0);
-            }
-        }
+        for (int s = 0; s < TI; s++) multiply(fa, fb, t, s);
     };
     if constexpr (MODE == kDirect) {
-        // Two sets of fragments: one is multiplied while the other is read, so that the matrix unit has its operands in registers at
-        // a barrier.  KK = 1: a ring of four tiles; in step n the fragments of step n + 1 are read and the copies of step n + 3
-        // start into the tile that step n - 1 was read from: a copy has two steps to land, and reads and copies lie evenly between
-        // the products (as a batch they hold up the wave's products behind them).  KK = 2: two tiles and half the barriers, for
-        // small tiles, where a barrier costs more than that; in the second half of step n, behind the barrier, the copies of step
-        // n + 2 start into the tile just read for the last time.  8192 x 4096 -> 4096, 256 x 256: 207 us with KK = 1, 215 with 2
-        // (without any copies 172, without reads 189); 4096^3 with 64 x 64: 278 and 182.
+        // Two sets of fragments, one for each half of a step: one is multiplied while the other is read, so that the matrix unit has
+        // its operands in registers at the barrier between the halves: every wave has read the step's tiles for the last time, and
+        // the next step's have landed.  Behind it the copies of B of step n + 2 start into the tile just read.  Those of A do so too
+        // (RING_A = 2), or start in the first half of the step after, into a third tile: reads and copies then lie evenly
+        // between the products.  (As a batch they hold up the wave's products behind them.)
         const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(smem) + wave * 1024);
-        constexpr int PARTS = TI > TJ ? TI : TJ, COPIES = TileA::LOADS + TileB::LOADS;
+        constexpr int PARTS = TI > TJ ? TI : TJ, BASE_B = RING_A * TileA::BYTES;
         FragA fa[2];
         FragB fb[2];
-        // where the next step to be copied starts
+        // where the next step to be copied starts, and goes
         const T *from_a = at_a(first), *from_b = at_b(first);
         const int64_t step_a = ROWS_A ? BK : BK * g.lda, step_b = ROWS_B ? BK : BK * g.ldb;
-        // share `part` of PARTS of the copies of step n.  full: it lies whole within p, else `left` of it (none of a step behind the
+        i32x4_t a4 = descriptor(from_a), b4 = descriptor(from_b);
+        unsigned to_a = lds, to_b = lds + BASE_B;
+        // share `part` of PARTS of a step's copies.  full: it lies whole within p, else `left` of it (none of a step behind the
         // last: zeros, which count for nothing)
-        auto copy_part = [&](i32x4_t a4, i32x4_t b4, int n, int part, auto full, int left) {
-            const unsigned to = lds + (n & (RING - 1)) * BUF;
+        auto copy_a = [&](int part, auto full, int left) {
             for_each([&](auto k) {
                 constexpr int K = decltype(k)::value;
-                if (K * PARTS / COPIES != part) return;
-                if constexpr (K < TileA::LOADS) TileA::template copy<0, K, decltype(full)::value>(sa, a4, to, left);
-                else TileB::template copy<TileA::BYTES, K - TileA::LOADS, decltype(full)::value>(sb, b4, to, left);
-            }, std::make_integer_sequence<int, COPIES>{});
+                if (K * PARTS / TileA::LOADS == part) TileA::template copy<0, K, decltype(full)::value>(sa, a4, to_a, left);
+            }, std::make_integer_sequence<int, TileA::LOADS>{});
+        };
+        auto copy_b = [&](int part, auto full, int left) {
+            for_each([&](auto k) {
+                constexpr int K = decltype(k)::value;
+                if (K * PARTS / TileB::LOADS == part) TileB::template copy<0, K, decltype(full)::value>(sb, b4, to_b, left);
+            }, std::make_integer_sequence<int, TileB::LOADS>{});
+        };
+        auto next_a = [&] {
+            from_a += step_a;
+            a4 = descriptor(from_a);
+            to_a = to_a == lds + (RING_A - 1) * TileA::BYTES ? lds : to_a + TileA::BYTES;
+        };
+        auto next_b = [&] {
+            from_b += step_b;
+            b4 = descriptor(from_b);
+            to_b = to_b == lds + BASE_B ? to_b + TileB::BYTES : lds + BASE_B;
         };
         auto left_of = [&](int n) { return n < steps ? left_p(first + n) : 0; };
         auto copy_all = [&](int n) {
-            const i32x4_t a4 = descriptor(from_a), b4 = descriptor(from_b);
             const int left = left_of(n);
 #pragma unroll
-            for (int part = 0; part < PARTS; part++) copy_part(a4, b4, n, part, std::false_type{}, left);
-            from_a += step_a;
-            from_b += step_b;
+            for (int part = 0; part < PARTS; part++) {
+                copy_a(part, std::false_type{}, left);
+                copy_b(part, std::false_type{}, left);
+            }
+            next_a();
+            next_b();
         };
         // share `part` of the reads: spread over the first three quarters, so that the last of them are back in time
         constexpr int READ_PARTS = PARTS >= 4 ? PARTS * 3 / 4 : PARTS;
-        auto read_part = [&](int set, const unsigned char* from, int kk, int part) {
+        auto read_a = [&](int set, const unsigned char* from, int part) {
 #pragma unroll
             for (int t = 0; t < TI; t++)
-                if (t * READ_PARTS / TI == part) fa[set].read(from, wi, kk, t);
+                if (t * READ_PARTS / TI == part) fa[set].read(from, wi, set, t);
+        };
+        auto read_b = [&](int set, const unsigned char* from, int part) {
 #pragma unroll
             for (int t = 0; t < TJ; t++)
-                if (t * READ_PARTS / TJ == part) fb[set].read(from + TileA::BYTES, wj, kk, t);
+                if (t * READ_PARTS / TJ == part) fb[set].read(from, wj, set, t);
         };
-        constexpr int AHEAD = KK == 1 ? 3 : 2;
-        auto step = [&](int n, int set, auto full) {                     // set = n & 1 (KK = 1); full: step n + AHEAD is
-            const unsigned char* now = smem + (n & (RING - 1)) * BUF;
-            const unsigned char* next = smem + ((n + 1) & (RING - 1)) * BUF;
-            const int reading = KK == 1 ? set ^ 1 : 0;
-            if constexpr (KK == 1) {
-                // the copies of step n + 1 have landed (those of step n + 2 may be under way), everybody's
-                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(COPIES) : "memory");
-            } else {
-#pragma unroll
-                for (int t = 0; t < PARTS; t++) {
-                    read_part(1, now, 1, t);
-                    if (t < TJ) multiply_tile(fa[0], fb[0], t);
-                    __builtin_amdgcn_sched_barrier(0);                   // (or the reads gather behind the products)
-                }
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            }
-            const i32x4_t a4 = descriptor(from_a), b4 = descriptor(from_b);
-            const int left = full ? BK : left_of(n + AHEAD);
-            from_a += step_a;
-            from_b += step_b;
+        const unsigned char *now_a = smem, *now_b = smem + BASE_B;
+        // half a step: multiplies set, reads the other one, copies between the products
+        auto half = [&](auto set, auto copies, auto next) {
+            constexpr int SET = decltype(set)::value;
 #pragma unroll
             for (int t = 0; t < PARTS; t++) {
-                copy_part(a4, b4, n + AHEAD, t, full, left);
-                read_part(reading, next, 0, t);
-                if (t < TJ) multiply_tile(fa[reading ^ 1], fb[reading ^ 1], t);
-                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int s = 0; s < TI; s++) {
+                    if (s == 0) copies(t);
+                    if (s == TI / 4) read_a(SET ^ 1, now_a, t);
+                    if (s == TI / 2) read_b(SET ^ 1, now_b, t);
+                    if (t == PARTS - 1 && s == TI / 4) next();
+                    if (t < TJ) multiply(fa[SET], fb[SET], t, s);
+                    if (TI == 8 || s == TI - 1) __builtin_amdgcn_sched_barrier(0);      // (or the reads gather behind the products)
+                }
             }
+        };
+        using First = std::integral_constant<int, 0>;
+        using Second = std::integral_constant<int, 1>;
+        auto step = [&](int n, auto full) {                              // full: step n + 2 is
+            const int left = full ? BK : left_of(n + 2);
+            half(First{}, [&](int t) { if (RING_A == 3) copy_a(t, full, left); }, [&] { if (RING_A == 3) next_a(); });
+            now_a = now_a == smem + (RING_A - 1) * TileA::BYTES ? smem : now_a + TileA::BYTES;
+            now_b = now_b == smem + BASE_B ? now_b + TileB::BYTES : smem + BASE_B;
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(RING_A == 3 ? TileA::LOADS : 0) : "memory");
+            half(Second{}, [&](int t) { if (RING_A == 2) copy_a(t, full, left); copy_b(t, full, left); }, [&] { if (RING_A == 2) next_a(); next_b(); });
         };
         if (steps > 0) {
             copy_all(0);
             copies_landed();
             __syncthreads();
-#pragma unroll
-            for (int k = 1; k < AHEAD; k++) copy_all(k);
+            copy_all(1);
             fa[0].read(smem, wi, 0);
-            fb[0].read(smem + TileA::BYTES, wj, 0);
+            fb[0].read(smem + BASE_B, wj, 0);
         }
         int n = 0;
         const int full_steps = min(steps, (int)(g.np / BK) - first);      // of this slice
-        // (KK = 1: steps in pairs, so that the sets are constants; a step behind the last multiplies the zeros copied for it)
 #pragma unroll 1
-        for (; n + 4 < full_steps; n += 2) {
-            step(n, 0, std::true_type{});
-            step(n + 1, 1, std::true_type{});
-        }
+        for (; n + 2 < full_steps; n++) step(n, std::true_type{});
 #pragma unroll 1
-        for (; n < steps; n += 2) {
-            step(n, 0, std::false_type{});
-            if (KK == 1 || n + 1 < steps) step(n + 1, 1, std::false_type{});
-        }
+        for (; n < steps; n++) step(n, std::false_type{});
         copies_landed();                                                 // (the epilogue writes where they go)
     } else {
         // Two LDS buffers and two sets of registers: a step's loads have the two steps before it to arrive; one barrier a step.
@@ -554,7 +563,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
             __syncthreads();
             fetch(n + 2, set);
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
+            for (int kk = 0; kk < 2; kk++) {
                 FragA fa;
                 FragB fb;
                 fa.read(smem + set * BUF, wi, kk);
@@ -581,7 +590,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     // down in LDS as rows of four-column chunks (chunk c of row r at c ^ r: the 16 rows a store touches lie in 16 different
     // 16-byte banks) and takes it up again in runs of consecutive columns: stores of 16 bytes, and one copy of the
     // epilogue's code.
-    constexpr int COLS = BJ / WJ, CHUNKS = COLS / 4, ROWS_MAX = BUF * RING / (WI * WJ) / (COLS * 4);
+    constexpr int COLS = BJ / WJ, CHUNKS = COLS / 4, ROWS_MAX = BUF * 2 / (WI * WJ) / (COLS * 4);
     constexpr int S_PASS = ROWS_MAX / 16 < TI ? ROWS_MAX / 16 : TI;      // A tiles per pass
     constexpr int N = 16 / (int)sizeof(T), RUNS = COLS / N;
     static_assert(S_PASS >= 1 && TI % S_PASS == 0, "the epilogue's passes");
@@ -766,10 +775,10 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
 }
 
 // (64 x 64: five workgroups on a CU, as many as its LDS holds.  float32 10000 x 512 -> 512, 1256 of them: 55 us with four, 49 with five)
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int KK, int MODE>
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
 __global__ void __launch_bounds__(WI * WJ * 64, BI == 64 && MODE == kDirect ? 5 : 1) linear_gemm_kernel(const Gemm g) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ, KK>];
-    gemm_tile<T, BI, BJ, WI, WJ, ROWS_A, ROWS_B, KK, MODE>(g, blockIdx.x, smem);
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ>];
+    gemm_tile<T, BI, BJ, WI, WJ, ROWS_A, ROWS_B, MODE>(g, blockIdx.x, smem);
 }
 
 // Few rows (at most 32) and a short sum: the tile kernel would spend most of its products on rows that are not there, and need
@@ -998,10 +1007,10 @@ struct Pair {
 };
 
 template <class T, int MODE> __global__ void __launch_bounds__(256) linear_pair_kernel(const Pair p) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<64, 64, 2>];
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<64, 64>];
     const unsigned first_x = p.x_first ? 0 : p.blocks_w, first_w = p.x_first ? p.blocks_x : 0;
-    if (blockIdx.x - first_x < p.blocks_x) gemm_tile<T, 64, 64, 2, 2, true, false, 2, MODE>(p.x, blockIdx.x - first_x, smem);
-    else if (blockIdx.x - first_w < p.blocks_w) gemm_tile<T, 64, 64, 2, 2, false, false, 2, MODE>(p.w, blockIdx.x - first_w, smem);
+    if (blockIdx.x - first_x < p.blocks_x) gemm_tile<T, 64, 64, 2, 2, true, false, MODE>(p.x, blockIdx.x - first_x, smem);
+    else if (blockIdx.x - first_w < p.blocks_w) gemm_tile<T, 64, 64, 2, 2, false, false, MODE>(p.w, blockIdx.x - first_w, smem);
     else join_columns<T, 4>(p.columns, blockIdx.x - p.blocks_x - p.blocks_w, reinterpret_cast<float*>(smem));
 }
 
@@ -1151,8 +1160,7 @@ Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
 
 template <class T, int TILE, bool RA, bool RB, int MODE> void launch_gemm(const Gemm& g, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices));
-    constexpr int KK = MODE == kDirect && (TILE == 256 || (TILE == 128 && !(RA && RB))) ? 1 : 2;      // (what was faster where it is used)
-    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, KK, MODE>), grid, dim3(256), 0, stream, g);
+    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, MODE>), grid, dim3(256), 0, stream, g);
 }
 
 // How a product's operands can travel, and the tiles that follow from it.
