@@ -376,15 +376,15 @@ template <class F, int... K> __device__ __forceinline__ void for_each(F f, std::
 
 enum { kDirect, kLoose, kShort };
 
-// LDS of a workgroup: two steps of both operands, and a third one of A where it is alone on its CU, or one of two
-template <int BI, int BJ> constexpr int kRingA = BI >= 128 ? 3 : 2;
-template <int BI, int BJ> constexpr int kTileBytes = (kRingA<BI, BJ> * BI + 2 * BJ) * kStepBytes;
+// Steps of A and B in LDS: RING of both, and one more of A in tiles that have a CU to themselves or share it with one other.
+template <int BI, int RING> constexpr int kRingA = BI >= 128 ? RING + 1 : RING;
+template <int BI, int BJ, int RING> constexpr int kTileBytes = (kRingA<BI, RING> * BI + RING * BJ) * kStepBytes;
 
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE, int RING>
 __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned char* smem) {
     constexpr bool FORWARD = ROWS_A && ROWS_B;
     constexpr int THREADS = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, BK = kStepBytes / (int)sizeof(T);
-    constexpr int RING_A = kRingA<BI, BJ>;            // steps of A in LDS; two of B behind them
+    constexpr int RING_A = kRingA<BI, RING>;
     using TileA = Tile<T, BI, ROWS_A, THREADS>;
     using TileB = Tile<T, BJ, ROWS_B, THREADS>;
     using FragA = Frags<T, BI, ROWS_A, THREADS, TI>;
@@ -438,11 +438,12 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     if constexpr (MODE == kDirect) {
         // Two sets of fragments, one for each half of a step: one is multiplied while the other is read, so that the matrix unit has
         // its operands in registers at the barrier between the halves: every wave has read the step's tiles for the last time, and
-        // the next step's have landed.  Behind it the copies of B of step n + 2 start into the tile just read.  Those of A do so too
-        // (RING_A = 2), or start in the first half of the step after, into a third tile: reads and copies then lie evenly
-        // between the products.  (As a batch they hold up the wave's products behind them.)
+        // the next step's have landed.  Behind it the copies of step n + RING start into the tiles just read.  With a tile
+        // more of A, those of A start in the first half of the step after: reads and copies then lie evenly between the
+        // products.  (As a batch they hold up the wave's products behind them.)
         const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(smem) + wave * 1024);
-        constexpr int PARTS = TI > TJ ? TI : TJ, BASE_B = RING_A * TileA::BYTES;
+        constexpr int PARTS = TI > TJ ? TI : TJ, BASE_B = RING_A * TileA::BYTES, COPIES = TileA::LOADS + TileB::LOADS;
+        constexpr bool EARLY_A = RING_A > RING;
         FragA fa[2];
         FragB fb[2];
         // where the next step to be copied starts, and goes
@@ -472,7 +473,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
         auto next_b = [&] {
             from_b += step_b;
             b4 = descriptor(from_b);
-            to_b = to_b == lds + BASE_B ? to_b + TileB::BYTES : lds + BASE_B;
+            to_b = to_b == lds + BASE_B + (RING - 1) * TileB::BYTES ? lds + BASE_B : to_b + TileB::BYTES;
         };
         auto left_of = [&](int n) { return n < steps ? left_p(first + n) : 0; };
         auto copy_all = [&](int n) {
@@ -516,26 +517,25 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
         };
         using First = std::integral_constant<int, 0>;
         using Second = std::integral_constant<int, 1>;
-        auto step = [&](int n, auto full) {                              // full: step n + 2 is
-            const int left = full ? BK : left_of(n + 2);
-            half(First{}, [&](int t) { if (RING_A == 3) copy_a(t, full, left); }, [&] { if (RING_A == 3) next_a(); });
+        auto step = [&](int n, auto full) {                              // full: step n + RING is
+            const int left = full ? BK : left_of(n + RING);
+            half(First{}, [&](int t) { if (EARLY_A) copy_a(t, full, left); }, [&] { if (EARLY_A) next_a(); });
             now_a = now_a == smem + (RING_A - 1) * TileA::BYTES ? smem : now_a + TileA::BYTES;
-            now_b = now_b == smem + BASE_B ? now_b + TileB::BYTES : smem + BASE_B;
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(RING_A == 3 ? TileA::LOADS : 0) : "memory");
-            half(Second{}, [&](int t) { if (RING_A == 2) copy_a(t, full, left); copy_b(t, full, left); }, [&] { if (RING_A == 2) next_a(); next_b(); });
+            now_b = now_b == smem + BASE_B + (RING - 1) * TileB::BYTES ? smem + BASE_B : now_b + TileB::BYTES;
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((RING - 2) * COPIES + (EARLY_A ? TileA::LOADS : 0)) : "memory");
+            half(Second{}, [&](int t) { if (!EARLY_A) copy_a(t, full, left); copy_b(t, full, left); }, [&] { if (!EARLY_A) next_a(); next_b(); });
         };
         if (steps > 0) {
-            copy_all(0);
-            copies_landed();
-            __syncthreads();
-            copy_all(1);
+#pragma unroll
+            for (int k = 0; k < RING; k++) copy_all(k);
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((RING - 1) * COPIES) : "memory");
             fa[0].read(smem, wi, 0);
             fb[0].read(smem + BASE_B, wj, 0);
         }
         int n = 0;
         const int full_steps = min(steps, (int)(g.np / BK) - first);      // of this slice
 #pragma unroll 1
-        for (; n + 2 < full_steps; n++) step(n, std::true_type{});
+        for (; n + RING < full_steps; n++) step(n, std::true_type{});
 #pragma unroll 1
         for (; n < steps; n++) step(n, std::false_type{});
         copies_landed();                                                 // (the epilogue writes where they go)
@@ -775,10 +775,10 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
 }
 
 // (64 x 64: five workgroups on a CU, as many as its LDS holds.  float32 10000 x 512 -> 512, 1256 of them: 55 us with four, 49 with five)
-template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE>
-__global__ void __launch_bounds__(WI * WJ * 64, BI == 64 && MODE == kDirect ? 5 : 1) linear_gemm_kernel(const Gemm g) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ>];
-    gemm_tile<T, BI, BJ, WI, WJ, ROWS_A, ROWS_B, MODE>(g, blockIdx.x, smem);
+template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE, int RING>
+__global__ void __launch_bounds__(WI * WJ * 64, BI == 64 && MODE == kDirect && RING == 2 ? 5 : 1) linear_gemm_kernel(const Gemm g) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ, RING>];
+    gemm_tile<T, BI, BJ, WI, WJ, ROWS_A, ROWS_B, MODE, RING>(g, blockIdx.x, smem);
 }
 
 // Few rows (at most 32) and a short sum: the tile kernel would spend most of its products on rows that are not there, and need
@@ -1006,11 +1006,11 @@ struct Pair {
     int x_first;                         // the longer sums start first, or they would end last and alone
 };
 
-template <class T, int MODE> __global__ void __launch_bounds__(256) linear_pair_kernel(const Pair p) {
-    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<64, 64>];
+template <class T, int MODE, int RING> __global__ void __launch_bounds__(256) linear_pair_kernel(const Pair p) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<64, 64, RING>];
     const unsigned first_x = p.x_first ? 0 : p.blocks_w, first_w = p.x_first ? p.blocks_x : 0;
-    if (blockIdx.x - first_x < p.blocks_x) gemm_tile<T, 64, 64, 2, 2, true, false, MODE>(p.x, blockIdx.x - first_x, smem);
-    else if (blockIdx.x - first_w < p.blocks_w) gemm_tile<T, 64, 64, 2, 2, false, false, MODE>(p.w, blockIdx.x - first_w, smem);
+    if (blockIdx.x - first_x < p.blocks_x) gemm_tile<T, 64, 64, 2, 2, true, false, MODE, RING>(p.x, blockIdx.x - first_x, smem);
+    else if (blockIdx.x - first_w < p.blocks_w) gemm_tile<T, 64, 64, 2, 2, false, false, MODE, RING>(p.w, blockIdx.x - first_w, smem);
     else join_columns<T, 4>(p.columns, blockIdx.x - p.blocks_x - p.blocks_w, reinterpret_cast<float*>(smem));
 }
 
@@ -1121,15 +1121,15 @@ bool thin_fits(int dtype, bool rows_b, int64_t ni, int64_t nj, int64_t np) {
 // The tile and the number of slices with the least predicted time.  Measured on MI355X, us per step (128 bytes along p) of a
 // workgroup that has a CU to itself / of each of several that share one, by the number of "columns" operands, and us for the ends
 // of a tile (first copies, epilogue) that nothing overlaps:
-//   16-bit  64 x 64: 0.26 / 0.18, 0.24 / 0.18, 0.24 / 0.20, 0.4     128 x 128: 0.67 / 0.45, 0.59 / 0.50, 0.57 / 0.48, 1.2     256 x 256: 1.60, 1.55, 1.50, 5
+//   16-bit  64 x 64: 0.22 / 0.19 (columns 0.20, 0.21), 0.4      128 x 128: 0.56 / 0.43 (two columns 0.46), 1      256 x 256: 1.35, 10
 //   float32 64 x 64: 0.46 / 0.46, whichever, 0.4                 (a 128 x 128 tile takes four times that: not built)
 // 3 us for a launch; slices cost a second launch and a round trip of their float32 sums at 6 TB/s.
-// 1024^3 in bfloat16: 64 x 64 tiles 7 us, 128 x 128 12; 4096^3: 256 x 256 108 us (1270 TFLOP/s), 128 x 128 117, 64 x 64 187; a weight
-// gradient of 2048 x 2048 over 8192 rows: 256 x 256 in four slices 78, 128 x 128 76, 256 x 256 whole 164.
+// 1024^3 in bfloat16: 64 x 64 tiles 6.5 us, 128 x 128 10; 2048^3: 27, 21 and (256 x 256) 46; 4096^3: 190, 113 and 99 (1390 TFLOP/s); a
+// weight gradient of 2048 x 2048 over 8192 rows: 256 x 256 in four slices 75, whole 160, 128 x 128 73.
 Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
     struct Kind { int tile; double alone[3], shared[3], ends; };
-    static const Kind kinds[] = {{64, {0.26, 0.24, 0.24}, {0.18, 0.18, 0.20}, 0.4}, {128, {0.67, 0.59, 0.57}, {0.45, 0.50, 0.48}, 1.2},
-                                 {256, {1.60, 1.55, 1.50}, {1.60, 1.55, 1.50}, 5.0}};
+    static const Kind kinds[] = {{64, {0.22, 0.22, 0.22}, {0.19, 0.20, 0.21}, 0.4}, {128, {0.56, 0.56, 0.56}, {0.43, 0.43, 0.46}, 1.0},
+                                 {256, {1.35, 1.35, 1.35}, {1.35, 1.35, 1.35}, 10.0}};
     static const Kind kinds32[] = {{64, {0.46, 0.46, 0.46}, {0.46, 0.46, 0.46}, 0.4}};
     Shape best;
     best.thin = columns < 2 && thin_fits(dtype, columns == 0, ni, nj, np);
@@ -1158,9 +1158,21 @@ Shape shape_of(int dtype, int columns, int64_t ni, int64_t nj, int64_t np) {
     return best;
 }
 
+// Steps in LDS for 64 x 64 tiles.  Three of them let a copy take two steps, but only three workgroups fit on a CU, two let five.
+// 16-bit, us with two / three: 1024 x 1024 over 4096 rows (256 tiles of 64 steps) 29.3 / 17.6, 300 x 4096 -> 4096 (320 of 64) 30 / 23,
+// 6000 x 768 -> 768 (1128 of 12) 16.9 / 15.7, 16384 x 256 -> 1024 (4096 of 4) 22.4 / 25.2: three for sums of eight steps or more.
+// float32, whose steps take long enough: 10000 x 512 -> 512 44 / 46, two.
+template <class T> bool three_steps(const Gemm& g) { return sizeof(T) == 2 && g.slice_steps >= 8; }
+
 template <class T, int TILE, bool RA, bool RB, int MODE> void launch_gemm(const Gemm& g, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)g.tiles_i * g.tiles_j * g.slices));
-    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, MODE>), grid, dim3(256), 0, stream, g);
+    if constexpr (TILE == 64 && MODE == kDirect && sizeof(T) == 2) {
+        if (three_steps<T>(g)) {
+            hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, MODE, 3>), grid, dim3(256), 0, stream, g);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((linear_gemm_kernel<T, TILE, TILE, 2, 2, RA, RB, MODE, 2>), grid, dim3(256), 0, stream, g);
 }
 
 // How a product's operands can travel, and the tiles that follow from it.
@@ -1239,8 +1251,13 @@ template <class T> int run_pair(Gemm x, const Shape& sx, Gemm w, const Shape& sw
     }
     const int64_t blocks = (int64_t)p.blocks_x + p.blocks_w + (columns.blocks ? (columns.cols + 63) / 64 : 0);
     SG_REQUIRE(blocks <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
-    if (direct) hipLaunchKernelGGL((linear_pair_kernel<T, kDirect>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((linear_pair_kernel<T, kLoose>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    const dim3 grid((unsigned)blocks);
+    const bool three = direct && three_steps<T>(x) && three_steps<T>(w);
+    if constexpr (sizeof(T) == 2) {
+        if (three) hipLaunchKernelGGL((linear_pair_kernel<T, kDirect, 3>), grid, dim3(256), 0, stream, p);
+    }
+    if (direct && !three) hipLaunchKernelGGL((linear_pair_kernel<T, kDirect, 2>), grid, dim3(256), 0, stream, p);
+    if (!direct) hipLaunchKernelGGL((linear_pair_kernel<T, kLoose, 2>), grid, dim3(256), 0, stream, p);
     const int64_t jx = join_blocks(x), jw = join_blocks(w);
     SG_REQUIRE(jx + jw <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "%s: too many elements", what);
     p.blocks_x = (unsigned)jx;
