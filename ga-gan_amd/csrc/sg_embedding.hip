@@ -4,14 +4,17 @@
 // Every operand is moved once; all of it is bound by HBM (few tokens: by launches).  The forward pass is a gather.  The table's
 // gradient sums, in float32 and in the order of the tokens, the rows of dy that share an index; no atomics, so that the same
 // inputs give the same bits:
-//   * up to kOwnerTokens tokens: one launch.  A workgroup owns 64 classes x 64 features of the table, each wave a quarter of
+//   * few tokens (plan_grad): one launch.  A workgroup owns 64 classes x 64 features of the table, each wave a quarter of
 //     the classes; it lists the tokens that fall on its classes, sums them and writes the tile, zeros included.
 //   * beyond: the tokens are sorted by index (stable radix sort, 8 bits a pass; one launch while one workgroup can hold
-//     them, two launches a pass otherwise) and a wave walks a fixed number of sorted positions with the running sum in
+//     them, two launches a pass otherwise: 4096 tokens of 1000 x 512 24.6 us the first way, 28.7 the second) and a wave walks a fixed number of sorted positions with the running sum in
 //     registers.  A run of equal indices inside one wave's positions is written straight to its row.  A run that crosses
 //     into other waves' positions leaves one partial sum per wave, and a second kernel adds those in order: the most
 //     frequent index costs no more than any other.  Rows without tokens are zeroed by the sort's first launch.
 // An index outside [0, v) reads as a row of NaN and takes no gradient.
+// 65536 tokens of 32000 x 1024 in bfloat16, natural frequencies: lookup 40 us (268 MB moved, repeated rows from the caches), gradient
+// 84: sort and clearing 27, sums 46 (200 MB, 4.3 TB/s), runs that cross spans 8; a bias 9 more.  64 labels of 1000 x 512 in float32: 3.7
+// and 4.9 us.
 #include "sg_common.h"
 #include "sg_column_sums.h"
 
@@ -362,6 +365,7 @@ struct RunParams {
     const void* dy;
     void* dtable;
     float* partial;                      // [spans][2][f]: slot 0 the run that began in an earlier span, slot 1 the one that goes on
+    float* columns;                      // [spans][f] or NULL: sums over all of the span's tokens, for the bias
     int64_t tokens, v, f, stride_v, stride_f;
     float w_gain;
     int span;                            // sorted positions per wave, at most 64
@@ -387,9 +391,9 @@ __global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const RunParam
     const unsigned key_before = p0 > 0 ? p.keys[p0 - 1] : none;
     const unsigned key_after = p0 + here < p.tokens ? p.keys[p0 + here] : none;
     const T* __restrict__ dy = (const T*)p.dy;
-    float acc[N];
+    float acc[N], all[N];
 #pragma unroll
-    for (int j = 0; j < N; j++) acc[j] = 0.f;
+    for (int j = 0; j < N; j++) acc[j] = all[j] = 0.f;
     unsigned key = __builtin_amdgcn_readfirstlane(my_key);
     bool from_before = key == key_before;
     auto flush = [&](bool goes_on) {
@@ -437,10 +441,16 @@ __global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const RunParam
                 from_before = false;
             }
 #pragma unroll
-            for (int j = 0; j < N; j++) acc[j] += Elem<T>::load(g[u][j]);
+            for (int j = 0; j < N; j++) {
+                acc[j] += Elem<T>::load(g[u][j]);
+                all[j] += Elem<T>::load(g[u][j]);
+            }
         }
     }
     flush(key == key_after);
+    if (p.columns && inside)
+#pragma unroll
+        for (int j = 0; j < N; j++) p.columns[(int64_t)span * p.f + f + j] = all[j];
 }
 
 // Runs that cross spans: the workgroup of the span a run begins in adds the later spans' partial sums to its own.  A wave takes 64 * N
@@ -545,7 +555,10 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 GradPlan plan_grad(const sg_embedding_params& p, int packet) {
     GradPlan g;
-    g.owner = p.tokens <= kOwnerTokens;
+    // Owner or sort, us, float32: 64 tokens of 1000 x 512 4 / 17, 256 tokens 5 / 19.5 (all on ten classes 11 / 18, on one class 26 / 18), 512
+    // tokens 7 / 19.5 (20 / 18, 50 / 19).  Every tile looks at every token: 64 of 60000 x 512 18 / 26, 256 of them 28 / 26, 256 of 20000 x
+    // 1024 in bfloat16 33 / 21.
+    g.owner = p.tokens <= kOwnerTokens && p.tokens * ((p.v + kOwnTile - 1) / kOwnTile) * ((p.f + kOwnTile - 1) / kOwnTile) <= 1 << 20;
     if (g.owner) return g;
     while (((uint64_t)p.v >> (8 * g.passes)) != 0) g.passes++;
     // sorted positions per wave: 64, halved (down to 16) while the launch would not reach eight waves on every CU
@@ -566,7 +579,7 @@ GradPlan plan_grad(const sg_embedding_params& p, int packet) {
     g.partial = at;
     at += up256((size_t)g.spans * 2 * p.f * 4);
     g.sums = at;
-    at += up256(column_sums_workspace_bytes(p.tokens, p.f));
+    at += up256((size_t)g.spans * p.f * 4);
     g.total = at;
     return g;
 }
@@ -665,7 +678,8 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
         perm = i_in;
     }
     const int tiles = (int)((p->f + 64 * n - 1) / (64 * n));
-    const RunParams r{keys, perm, dy, dtable, (float*)(ws + g.partial), p->tokens, p->v, p->f, p->stride_v, p->stride_f, p->w_gain, g.span, g.spans, tiles};
+    const RunParams r{keys, perm, dy, dtable, (float*)(ws + g.partial), dbias ? (float*)(ws + g.sums) : nullptr,
+                      p->tokens, p->v, p->f, p->stride_v, p->stride_f, p->w_gain, g.span, g.spans, tiles};
     const int64_t items = (int64_t)g.spans * tiles;
     SG_REQUIRE((items + 3) / 4 <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "embedding_backward: too many elements");
     SG_DISPATCH_16_32(p->dtype, {
@@ -679,5 +693,5 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
     });
     const int done = check_launch("sg_embedding_backward");
     if (done != SG_OK || dbias == nullptr) return done;
-    return column_sums(dy, p->dtype, p->tokens, p->f, p->f, p->b_gain, dbias, ws + g.sums, stream);
+    return join_column_sums((const float*)(ws + g.sums), g.spans, p->f, p->b_gain, p->dtype, dbias, stream);
 }

@@ -7,6 +7,9 @@
 // into LDS where rows are 16-byte aligned), and a fragment of a "columns" operand is read by the transposing LDS read (16-bit)
 // or four rows at a time (float32).  16-bit operands multiply on v_mfma_f32_16x16x32, float32 ones on v_mfma_f32_16x16x4_f32,
 // whose products and sums are plain float32.  All sums are float32; every output is rounded once.
+// Large products are bound by the matrix unit at the clock that power leaves: bfloat16 8192 x 4096 -> 4096 with bias, activation and
+// residual 199 to 217 us (1270 to 1380 TFLOP/s), its gradients 200 to 207 each; float32 4096^3 915 to 975 (141 to 150).  Small ones
+// are bound by launches: one row of 512 -> 512 3.8 us, a training step of 32 rows 18 in four launches.
 //
 // The gradient of the activation is s above without the gains: for the piecewise linear activations with slope 1 on one side
 // its 16-bit rounding is exact there, so that folding sqrt(2) into the products' scale keeps it that way.
@@ -355,7 +358,7 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
 // two "rows" operands are the forward pass and carry its epilogue.
 // c += a b, written as assembly for the one thing the builtin does not say: c is read and written in place, in accumulation
 // registers.  (With 256 of them a lane the register allocator otherwise moves accumulators about, up to 448 moves in a step of 128
-// products: 400 us instead of 240 for 8192 x 4096 -> 4096.)  Products of one accumulator are at least a tile row apart, and settle()
+// products and two thirds more time.)  Products of one accumulator are at least a tile row apart, and settle()
 // is the wait before anything else reads them.
 __device__ __forceinline__ void mfma_in_place(f32x4_t& c, const uint4& a, const uint4& b, __hip_bfloat16) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(bf16x8_t, a)), "v"(__builtin_bit_cast(bf16x8_t, b)));
@@ -784,7 +787,8 @@ __global__ void __launch_bounds__(WI * WJ * 64, BI == 64 && MODE == kDirect && R
 // Few rows (at most 32) and a short sum: the tile kernel would spend most of its products on rows that are not there, and need
 // slices and a second launch to use more than a few CUs.  Here eight waves share the sum of 16 (ROWS_B) or 32 columns: operands go
 // from global memory to fragments, 64 bytes of p per wave and turn (the eight waves' turns lie side by side), the waves' sums are
-// added in wave order.  Rows of both operands are whole aligned packets.  TI: row tiles.
+// added in wave order.  Rows of both operands are whole aligned packets.  TI: row tiles.  One row of 512 -> 512 in float32: 3.8 us, and
+// 7.5 as one 64 x 64 tile in eight slices.
 template <class T, int TI, bool ROWS_B>
 __global__ void __launch_bounds__(512) linear_thin_kernel(const Gemm g) {
     constexpr int WAVES = 8, TJ = ROWS_B ? 1 : 2, COLS = 16 * TJ, E = 16 / (int)sizeof(T), UNIT = 4 * E, UNROLL = 4;
@@ -897,7 +901,7 @@ struct SlopeParams {
 
 // A workgroup: 64 * N columns (N: elements per lane, one 16-byte packet or a single one), rows_per_block rows, the waves taking
 // every fourth row, UNROLL of them requested at a time (rows behind the last read it again and count as nothing).  BY: where the
-// slope comes from.
+// slope comes from.  Bound by HBM: 8192 x 2048 in bfloat16 by a byte an element 15 us (84 MB, 5.6 TB/s).
 enum { kByNothing, kByY, kByPositive, kByZ };
 
 template <class T, int N, int BY>
@@ -1027,11 +1031,11 @@ template <class T> __global__ void __launch_bounds__(256) linear_pair_join_kerne
 // ---- operands whose rows are not whole packets ------------------------------------------------------------------------------------
 // Copies with rows of whole aligned packets, zeros behind the last element: two passes over an operand, and from there on the tiles
 // travel to LDS directly and not by way of registers, and may be large ones.  Forward / gradients of x / of w in us, without and with:
-//   float16  1000 x 771 -> 1025    16.9 / 17.7 / 16.2      16.9 / 17.3 / 18.2 (the last two together share one launch for the copies)
-//   float32  1000 x 771 -> 1025    42.2 / 39.7 / 36.1      38.3 / 29.6 / 30.9
-//   float16  2047 x 2049 -> 2051   74 / 75 / 73            66 / 64 / 49
-//   bfloat16 8192 x 4095 -> 4097   546 / 435 / 559         339 / 284 / 363
-//   float32  64 x 8191 -> 511      18.5 / 19.7 / 12.8      23.1 / 19.8 / 14.9
+//   float16  1000 x 771 -> 1025    17.2 / 17.8 / 16.8      16.6 / 14.8 / 15.6 (the last two together share one launch for the copies)
+//   float32  1000 x 771 -> 1025    42.8 / 39.8 / 36.6      40.5 / 31.6 / 31.9
+//   float16  2047 x 2049 -> 2051   74 / 75 / 68            59 / 52 / 49
+//   bfloat16 8192 x 4095 -> 4097   741 / 680 / 775         322 / 272 / 357
+//   float32  64 x 8191 -> 511      19.0 / 19.4 / 13.0      23.1 / 19.8 / 14.9
 // so products from 2^29 terms on are laid out so, smaller ones are not.
 struct PackParams {
     struct { const void* src; void* dst; int64_t ld, rows, cols, packets; } m[3];      // packets: per row
@@ -1373,14 +1377,10 @@ BackwardPlan plan_backward(const sg_linear_params& p) {
 
 }  // namespace
 
-size_t column_sums_workspace_bytes(int64_t rows, int64_t cols) { return up256((size_t)slope_blocks(rows, cols) * cols * 4); }
-
-int column_sums(const void* g, int dtype, int64_t rows, int64_t cols, int64_t ld, float scale, void* out, void* workspace, hipStream_t stream) {
-    SlopeParams p{};
-    p.dy = g; p.partial = (float*)workspace; p.sums = out;
-    p.rows = rows; p.cols = cols; p.ld = ld; p.scale = scale;
-    SG_DISPATCH_16_32(dtype, return run_slope<T>(p, stream, "column sums"));
-    return SG_OK;
+int join_column_sums(const float* partial, int blocks, int64_t cols, float scale, int dtype, void* out, hipStream_t stream) {
+    const ColumnJoin p{partial, out, cols, blocks, scale};
+    SG_DISPATCH_16_32(dtype, hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, stream, p));
+    return check_launch("column sums");
 }
 
 }  // namespace sg

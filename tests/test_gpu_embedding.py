@@ -65,7 +65,8 @@ def make(tokens, v, f, dtype, kind='uniform', columns=False, bias=True, seed=0):
 
 # the three ways a gradient is formed: up to 256 tokens, up to 4096 (one workgroup sorts), beyond
 SIZES = [(1, 1, 1), (1, 5, 512), (0, 4, 8), (64, 1000, 512), (255, 3, 65), (256, 257, 64), (257, 256, 64), (300, 255, 7), (1000, 65536, 24), (4096, 70, 130),
-         (4097, 70000, 40), (20000, 300, 96), (5000, 1, 33)]
+         (4097, 70000, 40), (20000, 300, 96), (5000, 1, 33),
+         (200, 20000, 1100), (20, 60000, 72)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
