@@ -13,7 +13,7 @@
 //     frequent index costs no more than any other.  Rows without tokens are zeroed by the sort's first launch.
 // An index outside [0, v) reads as a row of NaN and takes no gradient.
 // 65536 tokens of 32000 x 1024 in bfloat16, natural frequencies: lookup 40 us (268 MB moved, repeated rows from the caches), gradient
-// 84: sort and clearing 27, sums 46 (200 MB, 4.3 TB/s), runs that cross spans 8; a bias 9 more.  64 labels of 1000 x 512 in float32: 3.7
+// 84: sort and clearing 27, sums 46 (200 MB, 4.3 TB/s), runs that cross spans 8; a bias 6 more.  64 labels of 1000 x 512 in float32: 3.7
 // and 4.9 us.
 #include "sg_common.h"
 #include "sg_column_sums.h"
@@ -456,9 +456,13 @@ __global__ void __launch_bounds__(256) embedding_grad_runs_kernel(const RunParam
 // Runs that cross spans: the workgroup of the span a run begins in adds the later spans' partial sums to its own.  A wave takes 64 * N
 // features; where that leaves waves over, 2, 4 or 8 of them take consecutive shares of the spans, which are added in their order.
 template <class T, int N>
-__global__ void __launch_bounds__(512) embedding_grad_join_kernel(const RunParams p) {
+__global__ void __launch_bounds__(512) embedding_grad_join_kernel(const RunParams p, const ColumnJoin columns) {
     constexpr int WAVES = 8;
-    __shared__ float part[WAVES][64 * N];
+    __shared__ float part[WAVES][64 * (N > 2 ? N : 2)];
+    if ((int)blockIdx.x >= p.spans) {                                  // the workgroups behind the spans': the bias
+        join_columns<T, WAVES>(columns, blockIdx.x - p.spans, &part[0][0]);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int span = blockIdx.x;
     const int64_t p0 = (int64_t)span * p.span, end = p0 + p.span;
@@ -681,17 +685,17 @@ extern "C" int sg_embedding_backward(const sg_embedding_params* p, const void* d
     const RunParams r{keys, perm, dy, dtable, (float*)(ws + g.partial), dbias ? (float*)(ws + g.sums) : nullptr,
                       p->tokens, p->v, p->f, p->stride_v, p->stride_f, p->w_gain, g.span, g.spans, tiles};
     const int64_t items = (int64_t)g.spans * tiles;
+    const ColumnJoin columns{r.columns, dbias, p->f, g.spans, p->b_gain};
+    const unsigned joins = (unsigned)(g.spans + (dbias ? (p->f + 63) / 64 : 0));
     SG_REQUIRE((items + 3) / 4 <= INT32_MAX, SG_ERR_INVALID_ARGUMENT, "embedding_backward: too many elements");
     SG_DISPATCH_16_32(p->dtype, {
         if (packed) {
             hipLaunchKernelGGL((embedding_grad_runs_kernel<T, Pack<T>::N>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
-            hipLaunchKernelGGL((embedding_grad_join_kernel<T, Pack<T>::N>), dim3((unsigned)g.spans), dim3(512), 0, stream, r);
+            hipLaunchKernelGGL((embedding_grad_join_kernel<T, Pack<T>::N>), dim3(joins), dim3(512), 0, stream, r, columns);
         } else {
             hipLaunchKernelGGL((embedding_grad_runs_kernel<T, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream, r);
-            hipLaunchKernelGGL((embedding_grad_join_kernel<T, 1>), dim3((unsigned)g.spans), dim3(512), 0, stream, r);
+            hipLaunchKernelGGL((embedding_grad_join_kernel<T, 1>), dim3(joins), dim3(512), 0, stream, r, columns);
         }
     });
-    const int done = check_launch("sg_embedding_backward");
-    if (done != SG_OK || dbias == nullptr) return done;
-    return join_column_sums((const float*)(ws + g.sums), g.spans, p->f, p->b_gain, p->dtype, dbias, stream);
+    return check_launch("sg_embedding_backward");
 }

@@ -960,39 +960,6 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
     }
 }
 
-struct ColumnJoin {
-    const float* partial;                // [blocks][cols]
-    void* out;                           // [cols]
-    int64_t cols;
-    int blocks;
-    float scale;
-};
-
-// 64 columns a workgroup of WAVES waves: sixteen shares of every 16th partial sum, four under way at a time, whichever waves take them.
-template <class T, int WAVES> __device__ __forceinline__ void join_columns(const ColumnJoin& p, unsigned block, float* part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)block * 64 + lane;
-#pragma unroll
-    for (int share = wave; share < 16; share += WAVES) {
-        float sum = 0.f;
-        for (int b = share; b < p.blocks; b += 16 * 4) {
-            float v[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = b + 16 * u < p.blocks && c < p.cols ? p.partial[(int64_t)(b + 16 * u) * p.cols + c] : 0.f;
-#pragma unroll
-            for (int u = 0; u < 4; u++) sum += v[u];
-        }
-        part[share * 64 + lane] = sum;
-    }
-    __syncthreads();
-    if (wave == 0 && c < p.cols) {
-        float sum = 0.f;
-#pragma unroll
-        for (int share = 0; share < 16; share++) sum += part[share * 64 + lane];
-        ((T*)p.out)[c] = Elem<T>::store(sum * p.scale);
-    }
-}
-
 template <class T> __global__ void __launch_bounds__(1024) column_join_kernel(const ColumnJoin p) {
     __shared__ float part[16 * 64];
     join_columns<T, 16>(p, blockIdx.x, part);
@@ -1376,12 +1343,6 @@ BackwardPlan plan_backward(const sg_linear_params& p) {
 }
 
 }  // namespace
-
-int join_column_sums(const float* partial, int blocks, int64_t cols, float scale, int dtype, void* out, hipStream_t stream) {
-    const ColumnJoin p{partial, out, cols, blocks, scale};
-    SG_DISPATCH_16_32(dtype, hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, stream, p));
-    return check_launch("column sums");
-}
 
 }  // namespace sg
 
