@@ -353,13 +353,10 @@ __device__ __forceinline__ f32x4_t mfma(const uint4& a, const uint4& b, f32x4_t 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// Tile BI x BJ per workgroup of WI x WJ waves.  How operands travel: kDirect, rows of both are whole aligned 16-byte packets;
-// kLoose, rows start anywhere and end anywhere; kShort, rows of one of them are shorter than 16 bytes.  Products of
-// two "rows" operands are the forward pass and carry its epilogue.
 // c += a b, written as assembly for the one thing the builtin does not say: c is read and written in place, in accumulation
 // registers.  (With 256 of them a lane the register allocator otherwise moves accumulators about, up to 448 moves in a step of 128
-// products and two thirds more time.)  Products of one accumulator are at least a tile row apart, and settle()
-// is the wait before anything else reads them.
+// products and two thirds more time.)  Products of one accumulator are four or more products apart, and settle() is the wait
+// before anything else reads them.
 __device__ __forceinline__ void mfma_in_place(f32x4_t& c, const uint4& a, const uint4& b, __hip_bfloat16) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(__builtin_bit_cast(bf16x8_t, a)), "v"(__builtin_bit_cast(bf16x8_t, b)));
 }
@@ -377,12 +374,15 @@ template <int M, int N> __device__ __forceinline__ void settle(f32x4_t (&acc)[M]
 // f(integral_constant 0), f(integral_constant 1), ...
 template <class F, int... K> __device__ __forceinline__ void for_each(F f, std::integer_sequence<int, K...>) { (f(std::integral_constant<int, K>{}), ...); }
 
+// How operands travel: kDirect, rows of both are whole aligned 16-byte packets; kLoose, rows start anywhere and end anywhere;
+// kShort, rows of one of them are shorter than 16 bytes.
 enum { kDirect, kLoose, kShort };
 
 // Steps of A and B in LDS: RING of both, and one more of A in tiles that have a CU to themselves or share it with one other.
 template <int BI, int RING> constexpr int kRingA = BI >= 128 ? RING + 1 : RING;
 template <int BI, int BJ, int RING> constexpr int kTileBytes = (kRingA<BI, RING> * BI + RING * BJ) * kStepBytes;
 
+// One tile BI x BJ by a workgroup of WI x WJ waves.  Products of two "rows" operands are the forward pass and carry its epilogue.
 template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE, int RING>
 __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned char* smem) {
     constexpr bool FORWARD = ROWS_A && ROWS_B;
