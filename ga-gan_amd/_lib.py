@@ -21,7 +21,7 @@ SYMBOLS = ('sg_version', 'sg_last_error', 'sg_init', 'sg_upfirdn2d_out_size', 's
            'sg_upfirdn2d_add', 'sg_upfirdn2d_add_supported', 'sg_upfirdn2d_kernel', 'sg_planes_segments', 'sg_scale_planes', 'sg_dot_planes',
            'sg_styles', 'sg_styles_backward', 'sg_pack_weights',
            'sg_conv2d_prepared_weight_bytes', 'sg_conv2d_prepare_weights', 'sg_conv2d_supports_addend',
-           'sg_linear', 'sg_linear_workspace_bytes', 'sg_linear_backward', 'sg_linear_backward_workspace_bytes',
+           'sg_linear', 'sg_linear_kernel', 'sg_linear_workspace_bytes', 'sg_linear_backward', 'sg_linear_backward_workspace_bytes',
            'sg_embedding', 'sg_embedding_backward', 'sg_embedding_backward_workspace_bytes',
            'sg_adam_step_list', 'sg_grad_norm', 'sg_grad_norm_workspace_bytes', 'sg_scale_grads')
 
@@ -118,6 +118,8 @@ def lib():
                      'sg_grad_norm_workspace_bytes'):
             getattr(handle, name).argtypes = [vp]
             getattr(handle, name).restype = size_t
+        handle.sg_linear_kernel.argtypes = [vp, i32]
+        handle.sg_linear_kernel.restype = ctypes.c_char_p
         handle.sg_conv2d_reduce_rows.argtypes = [vp]
         handle.sg_conv2d_reduce_rows.restype = ctypes.c_int
         handle.sg_conv2d_kernel.argtypes = [vp]

@@ -1460,3 +1460,41 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
     if (dw && done == SG_OK) SG_DISPATCH_16_32(p->dtype, done = (run_gemm<T, false, false>(gw, plan.dw, stream, "sg_linear_backward")));
     return done;
 }
+
+extern "C" const char* sg_linear_kernel(const sg_linear_params* p, int32_t product) {
+    using namespace sg;
+    static thread_local char text[96];
+    if (check(p, "linear_kernel") != SG_OK || product < 0 || product > 2) return "";
+    // (copies in the workspace are whole packets wherever it lies)
+    auto here = [](const Operand& o) { return o.bytes ? reinterpret_cast<const void*>((uintptr_t)o.at) : o.p; };
+    Gemm g{};
+    Shape s;
+    if (product == 0) {
+        const ForwardPlan f = plan_forward(*p);
+        s = f.y;
+        g.a = here(f.x); g.lda = f.x.ld; g.a_padded = f.x.padded;
+        g.b = here(f.w); g.ldb = f.w.ld; g.b_padded = f.w.padded;
+        g.ni = p->m; g.nj = p->n; g.np = p->k;
+    } else {
+        const BackwardPlan b = plan_backward(*p);
+        const Operand& o = product == 1 ? b.w : b.x;
+        s = product == 1 ? b.dx : b.dw;
+        g.lda = b.s.ld; g.a_padded = b.s.padded;
+        g.b = here(o); g.ldb = o.ld; g.b_padded = o.padded;
+        g.ni = product == 1 ? p->m : p->n; g.nj = p->k; g.np = product == 1 ? p->n : p->m;
+    }
+    Route r;
+    int rc = SG_OK;
+    auto route = [&](auto element) {
+        using T = decltype(element);
+        rc = product == 0 ? route_gemm<T, true, true>(g, s, r, "linear_kernel") : product == 1 ? route_gemm<T, true, false>(g, s, r, "linear_kernel")
+                                                                                              : route_gemm<T, false, false>(g, s, r, "linear_kernel");
+    };
+    if (p->dtype == SG_F32) route(float());
+    else if (p->dtype == SG_F16) route(__half());
+    else route(__hip_bfloat16());
+    if (rc != SG_OK) return "";
+    if (r.thin) return "linear_thin_kernel";
+    snprintf(text, sizeof text, "linear_gemm_kernel<%d, %s> %d x %d", r.tile, r.direct ? "direct" : r.is_short ? "short" : "loose", g.slices, g.slice_steps);
+    return text;
+}

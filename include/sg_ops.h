@@ -593,6 +593,11 @@ typedef struct sg_linear_params {
     int64_t ldx, ldw, ldr;
 } sg_linear_params;
 
+/* The kernel that a product of the layer runs (0 the forward pass, 1 the gradient of x, 2 of w), as its name with the tile and how
+ * operands travel, then slices x steps of 128 bytes along the sum; for operands and gradients that are 16-byte aligned where the
+ * params do not say.  Host only; the text is valid until the thread's next call.  "" for params that are refused. */
+const char* sg_linear_kernel(const sg_linear_params* p, int32_t product);
+
 size_t sg_linear_workspace_bytes(const sg_linear_params* p);
 int sg_linear(const sg_linear_params* p, void* y, float* z, uint8_t* positive, void* workspace, size_t workspace_bytes,
               sg_stream_t stream);
