@@ -937,8 +937,10 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     float s = Elem<T>::load(dy[u].v[e]);
-                    if constexpr (BY == kByY) s = Elem<T>::load(y[u].v[e]) * p.sign > 0.f ? s : s * p.alpha;
-                    if constexpr (BY == kByPositive) s = pos[u].v[e] ? s : s * p.alpha;
+                    // (relu selects its zero: a dy that is not finite stays out of the gradient of a unit that is off)
+                    const float off = p.act == kActRelu ? 0.f : s * p.alpha;
+                    if constexpr (BY == kByY) s = Elem<T>::load(y[u].v[e]) * p.sign > 0.f ? s : off;
+                    if constexpr (BY == kByPositive) s = pos[u].v[e] ? s : off;
                     if constexpr (BY == kByZ) s *= slope_at<sizeof(T) == 2>(p.act, z[u].v[e]);
                     sum[e] += there ? s : 0.f;
                     out.v[e] = rounded<T>(s);
@@ -1434,7 +1436,7 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         r.sums = db;
         r.rows = p->m; r.cols = p->n; r.ld = p->n;
         r.act = p->act;
-        r.alpha = p->act == kActRelu ? 0.f : p->alpha;
+        r.alpha = p->alpha;
         r.sign = p->gain < 0.f ? -1.f : 1.f;
         r.scale = p->gain * p->b_gain;
         int done = SG_OK;
