@@ -12,11 +12,15 @@
 // are bound by launches: one row of 512 -> 512 3.8 us, a training step of 32 rows 18 in four launches.
 //
 // The gradient of the activation is s above without the gains: for the piecewise linear activations with slope 1 on one side
-// its 16-bit rounding is exact there, so that folding sqrt(2) into the products' scale keeps it that way.
+// its 16-bit rounding is exact there, so that folding sqrt(2) into the products' scale keeps it that way.  float16, whose range a
+// slope above one leaves at the upper end and one far below at the lower, holds s times the power of two that brings
+// max |dy| * (largest slope) to 2^14 .. 2^15; the sums are multiplied by its inverse (exact both ways).
+#include "sg_absmax.h"
 #include "sg_common.h"
 #include "sg_column_sums.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -112,6 +116,7 @@ struct Gemm {
     float* partial;                      // [slices][ni][nj] when slices > 1
     void* out;                           // [ni][nj]
     float scale;
+    const float* rescale;                // device value the scale is multiplied with (float16 gradients: a power of two), or NULL
     // epilogue of the forward pass
     const void* bias;                    // [nj]
     const void* residual;                // [ni][ldr]
@@ -122,6 +127,12 @@ struct Gemm {
     float alpha, gain, b_gain;
     int whole;                           // rows of everything the epilogue touches are whole aligned 16-byte packets
 };
+
+// Factor of the sums.  (The forward pass has none but the host's, and only float16 has one on the device.)
+template <class T, bool FORWARD> __device__ __forceinline__ float scale_of(const Gemm& g) {
+    if constexpr (!FORWARD && std::is_same_v<T, __half>) return g.rescale ? g.scale * *g.rescale : g.scale;
+    else return g.scale;
+}
 
 template <class T, int N> struct alignas(N * sizeof(T)) Run { T v[N]; };
 
@@ -139,8 +150,9 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int64_t j, floa
     }
     const int64_t at = i * g.nj + j;
     Run<T, N> out;
+    const float scale = scale_of<T, FORWARD>(g);
 #pragma unroll
-    for (int e = 0; e < N; e++) v[e] *= g.scale;
+    for (int e = 0; e < N; e++) v[e] *= scale;
     if constexpr (FORWARD) {
         if (g.bias)
 #pragma unroll
@@ -600,6 +612,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     const int lane = threadIdx.x & 63, l16 = lane & 15, quad = lane >> 4;
     float* mine = reinterpret_cast<float*>(smem) + wave * (S_PASS * 16 * COLS);
     auto chunk_at = [&](int row, int chunk) -> f32x4_t& { return *reinterpret_cast<f32x4_t*>(mine + row * COLS + (chunk ^ (row & (CHUNKS - 1))) * 4); };
+    const float scale = scale_of<T, FORWARD>(g);
     __syncthreads();                                                     // every wave is done with the tiles
     auto lay_down = [&](int s, int row) {                                 // A tile s, constant, as the region's rows from `row` on
 #pragma unroll
@@ -676,7 +689,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
 #pragma unroll
                     for (int u = 0; u < U; u++) take(round + u, v + u * N);
 #pragma unroll
-                    for (int e = 0; e < U * N; e++) v[e] = v[e] * g.scale + bias[e % N];
+                    for (int e = 0; e < U * N; e++) v[e] = v[e] * scale + bias[e % N];
                     if constexpr (FORWARD) {
                         if (g.z)
 #pragma unroll
@@ -733,7 +746,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
                         const int64_t i = i0 + wi + FragA::row(s0 + row / 16, row % 16);
                         there[u] = i < g.ni;
                         at[u] = i * g.nj + jj;
-                        v[u] = chunk_at(row, col / 4)[col % 4] * g.scale + bias;
+                        v[u] = chunk_at(row, col / 4)[col % 4] * scale + bias;
                         if (FORWARD && g.residual) res[u] = Elem<T>::load(((const T*)g.residual)[(there[u] ? i : 0) * g.ldr + jj]);
                     }
                     if constexpr (FORWARD) {
@@ -897,7 +910,50 @@ struct SlopeParams {
     int act;
     float alpha, sign;                   // sign: of the layer's gain
     float scale;
+    // float16: the largest finite |dy| of each of range_blocks shares, and where the inverse of s's factor goes; or NULL
+    const float* range;
+    float* rescale;
+    int range_blocks;
+    float largest_slope;
 };
+
+// The largest finite |dy| of each workgroup's share, packets or (dy starting anywhere) elements.  One read of dy, which the slope
+// kernel then finds in the last-level cache.
+constexpr int kRangeBlocks = 256;
+
+__global__ void __launch_bounds__(256) linear_range_kernel(const __half* __restrict__ dy, int64_t n, float* __restrict__ range) {
+    __shared__ unsigned part[4];
+    const unsigned short* bits = reinterpret_cast<const unsigned short*>(dy);
+    const int64_t packets = aligned16(dy) ? n / 8 : 0, first = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
+    unsigned largest = 0;                                               // magnitudes of halves are ordered as their bits are
+    auto take = [&](unsigned v) { v &= 0x7fff; largest = max(largest, v < 0x7c00 ? v : 0u); };
+    for (int64_t i = first; i < packets; i += stride) {
+        const uint4 q = reinterpret_cast<const uint4*>(dy)[i];
+        take(q.x); take(q.x >> 16); take(q.y); take(q.y >> 16); take(q.z); take(q.z >> 16); take(q.w); take(q.w >> 16);
+    }
+    for (int64_t i = packets * 8 + first; i < n; i += stride) take(bits[i]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) largest = max(largest, (unsigned)__shfl_xor((int)largest, d, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = largest;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned short all = (unsigned short)max(max(part[0], part[1]), max(part[2], part[3]));
+        range[blockIdx.x] = __half2float(__builtin_bit_cast(__half, all));
+    }
+}
+
+// The factor of s from all shares, the same in every workgroup (256 threads); the first one leaves its inverse for the products.
+__device__ __forceinline__ float range_factor(const SlopeParams& p, float (&part)[4]) {
+    float largest = (int)threadIdx.x < p.range_blocks ? p.range[threadIdx.x] : 0.f;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = largest;
+    __syncthreads();
+    float factor, inverse;
+    half_range_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.largest_slope, factor, inverse);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.rescale = inverse;
+    return factor;
+}
 
 // A workgroup: 64 * N columns (N: elements per lane, one 16-byte packet or a single one), rows_per_block rows, the waves taking
 // every fourth row, UNROLL of them requested at a time (rows behind the last read it again and count as nothing).  BY: where the
@@ -910,6 +966,11 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
     __shared__ float part[4][64 * N];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * N;
+    float factor = 1.f;
+    if constexpr (std::is_same_v<T, __half>) {
+        __shared__ float range_part[4];
+        if (p.range) factor = range_factor(p, range_part);
+    }
     const int64_t r0 = (int64_t)blockIdx.y * p.rows_per_block, r1 = min(r0 + p.rows_per_block, p.rows);
     float sum[N];
 #pragma unroll
@@ -943,7 +1004,7 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const SlopeParams p) 
                     if constexpr (BY == kByPositive) s = pos[u].v[e] ? s : off;
                     if constexpr (BY == kByZ) s *= slope_at<sizeof(T) == 2>(p.act, z[u].v[e]);
                     sum[e] += there ? s : 0.f;
-                    out.v[e] = rounded<T>(s);
+                    out.v[e] = rounded<T>(s * factor);
                 }
                 if (p.s && there) *reinterpret_cast<Run<T, N>*>((T*)p.s + row * p.lds + c) = out;
             }
@@ -1251,6 +1312,16 @@ int check(const sg_linear_params* p, const char* what) {
 
 bool piecewise(int act) { return act == kActRelu || act == kActLrelu; }
 
+// A bound of |act'|.
+float largest_slope(int act, float alpha) {
+    switch (act) {
+        case kActLrelu: return std::max(1.f, std::fabs(alpha));
+        case kActSelu: return kSeluScale * kSeluAlpha;
+        case kActSwish: return 1.1f;
+        default: return 1.f;
+    }
+}
+
 constexpr double kCopiedFrom = (double)(1 << 29);        // terms of a product; measured above
 
 // An operand as the products read it: where it lies, or its copy in the workspace.
@@ -1317,7 +1388,8 @@ ForwardPlan plan_forward(const sg_linear_params& p) {
 struct BackwardPlan {
     Shape dx, dw;
     Operand x, w, s;                      // s: the activation's gradient, or dy (copied only for its own n)
-    size_t sums = 0, partial = 0, partial_w = 0, total = 0;
+    bool ranged = false;                  // s times a power of two (float16; relu's s is dy or zero)
+    size_t sums = 0, range = 0, partial = 0, partial_w = 0, total = 0;
 };
 
 BackwardPlan plan_backward(const sg_linear_params& p) {
@@ -1334,6 +1406,9 @@ BackwardPlan plan_backward(const sg_linear_params& p) {
     }
     b.sums = at;
     at += up256((size_t)slope_blocks(p.m, p.n) * p.n * 4);
+    b.ranged = p.dtype == SG_F16 && p.act != kActLinear && p.act != kActRelu;
+    b.range = at;
+    if (b.ranged) at += up256((kRangeBlocks + 1) * 4);                  // the shares' largest values, then the inverse factor
     b.dx = shape_of(p.dtype, 1, p.m, p.k, p.n);
     b.dw = shape_of(p.dtype, 2, p.n, p.k, p.m);
     b.partial = at;
@@ -1439,12 +1514,22 @@ extern "C" int sg_linear_backward(const sg_linear_params* p, const void* dy, con
         r.alpha = p->alpha;
         r.sign = p->gain < 0.f ? -1.f : 1.f;
         r.scale = p->gain * p->b_gain;
+        if (plan.ranged && products) {
+            float* range = (float*)(ws + plan.range);
+            const int64_t count = p->m * p->n;
+            r.range = range;
+            r.rescale = range + kRangeBlocks;
+            r.range_blocks = (int)std::min<int64_t>((count + 2047) / 2048, kRangeBlocks);       // (a packet a lane, or more)
+            r.largest_slope = largest_slope(p->act, p->alpha);
+            hipLaunchKernelGGL(linear_range_kernel, dim3((unsigned)r.range_blocks), dim3(256), 0, stream, (const __half*)dy, count, range);
+        }
         int done = SG_OK;
         SG_DISPATCH_16_32(p->dtype, done = run_slope<T>(r, stream, "sg_linear_backward", pair ? &columns : nullptr));
         if (done != SG_OK) return done;
     }
     Gemm gx{}, gw{};
     gx.scale = gw.scale = p->gain * p->w_gain;
+    gx.rescale = gw.rescale = plan.ranged && products ? (const float*)(ws + plan.range) + kRangeBlocks : nullptr;
     gx.a = gw.a = plan.s.p; gx.lda = gw.lda = plan.s.ld; gx.a_padded = gw.a_padded = plan.s.padded;
     gx.partial = (float*)(ws + plan.partial);                      // [m, k] = s [m, n] w [n, k]
     gx.b = plan.w.p; gx.ldb = plan.w.ld; gx.b_padded = plan.w.padded;
