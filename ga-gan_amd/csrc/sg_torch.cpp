@@ -149,13 +149,17 @@ Tensor linear_forward(const Tensor& x_, const Tensor& w_, const Tensor& b_, cons
     return y;
 }
 
-// The layer from the framework's operators (differentiable to any order).
-Tensor linear_composite(const Tensor& x, const Tensor& w, const Tensor& b, const LinearConfig& c) {
+// The layer from the framework's operators (differentiable to any order), in float32 whatever the operands' type: a z rounded to 16
+// bits would choose other slopes than the forward pass did.  on: for relu and lrelu, where the forward pass had the slope of the
+// positive side.
+Tensor linear_composite(const Tensor& x_, const Tensor& w_, const Tensor& b_, const Tensor& on, const LinearConfig& c) {
+    auto wide = [](const Tensor& t) { return t.defined() ? t.to(at::kFloat) : t; };
+    const Tensor x = wide(x_), w = wide(w_), b = wide(b_);
     Tensor z = at::matmul(x, (c.w_gain != 1 ? w * c.w_gain : w).t());
     if (b.defined()) z = z + (c.b_gain != 1 ? b * c.b_gain : b);
     switch (c.act) {
-        case kRelu: z = at::relu(z); break;
-        case kLrelu: z = at::leaky_relu(z, c.alpha); break;
+        case kRelu: z = at::where(on, z, at::zeros_like(z)); break;
+        case kLrelu: z = at::where(on, z, z * c.alpha); break;
         case kTanh: z = at::tanh(z); break;
         case kSigmoid: z = at::sigmoid(z); break;
         case kElu: z = at::elu(z); break;
@@ -206,7 +210,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
             variable_list in{x_.view_as(x_), w_.view_as(w_), b.defined() ? b.view_as(b) : b}, wanted;
             for (int i = 0; i < 3; i++)
                 if (need[i]) wanted.push_back(in[i]);
-            const variable_list got = torch::autograd::grad({linear_composite(in[0], in[1], in[2], c)}, wanted, {dy}, true, true);
+            const Tensor on = kept == kY ? (c.gain < 0 ? aux < 0 : aux > 0) : kept == kPositive ? aux != 0 : Tensor();
+            const variable_list got = torch::autograd::grad({linear_composite(in[0], in[1], in[2], on, c)}, wanted, {dy.to(at::kFloat)}, true, true);
             for (int i = 0, k = 0; i < 3; i++)
                 if (need[i]) out[i] = got[k++];
             return out;

@@ -10,8 +10,9 @@ those of `bias_act`.
 
 What the backward pass keeps besides x and w: nothing for 'linear'; for 'relu' and 'lrelu' the output itself, whose sign
 is the pre-activation's, or - where a residual or float16's short range hides it - a byte per element; for the others the
-pre-activation values in float32 (rounded to 16 bits they would cost the gradient more accuracy than rounding the gradient itself does).  A
-backward pass that is asked for a graph of its own differentiates the same expression written with the framework's operators.
+pre-activation values in float32 (rounded to 16 bits they would cost the gradient more accuracy than rounding the gradient itself
+does).  A backward pass that is asked for a graph of its own (create_graph=True) differentiates the same expression written with the
+framework's operators, in float32 with one rounding per gradient, and with the slopes of the forward pass for 'relu' and 'lrelu'.
 
 At a pre-activation of exactly zero the slope is that of the negative side, as in `bias_act`."""
 import torch
