@@ -97,6 +97,10 @@ int dtype_code(const Tensor& t, const char* what) {
     }
 }
 
+// Whether t carries a tangent (forward-mode differentiation).  The functions below have no forward-mode derivative: a tensor that
+// carries one goes through Function::apply, which refuses it, whether or not gradients are wanted.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 Tensor or_undefined(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
 // (t or a dense copy, elements between its rows): unit stride within a row, rows that do not overlap and that lie less than the
@@ -204,6 +208,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         if (v[6] != 0 && ctx->needs_input_grad(b.defined() ? 3 : 2)) out[3] = dy;
         const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), b.defined() && ctx->needs_input_grad(2)};
         if (!need[0] && !need[1] && !need[2]) return out;
+        TORCH_CHECK(!dual(dy), "linear: the backward pass has no forward-mode derivative");
         const LinearConfig c{(int64_t)v[0], v[1], v[2], v[3], v[4]};
         const int kept = (int)v[5];
         if (at::GradMode::is_enabled()) {                        // a graph of its own is wanted: differentiate the operators' version
@@ -255,7 +260,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const optional<Tensor>& b_, cons
     const Tensor x2 = flat ? x : x.reshape({m, x.size(-1)}), r2 = flat || !residual.defined() ? residual : residual.reshape({m, w.size(0)});
     const bool graph = at::GradMode::is_enabled() &&
                        (x.requires_grad() || w.requires_grad() || (b.defined() && b.requires_grad()) || (residual.defined() && residual.requires_grad()));
-    const Tensor y = graph ? LinearFunction::apply(x2, w, b_, r2.defined() ? optional<Tensor>(r2) : c10::nullopt, c) : linear_forward(x2, w, b, r2, c, nullptr, nullptr);
+    const bool refused = dual(x) || dual(w) || dual(b) || dual(residual);
+    const Tensor y = graph || refused ? LinearFunction::apply(x2, w, b_, r2.defined() ? optional<Tensor>(r2) : c10::nullopt, c) : linear_forward(x2, w, b, r2, c, nullptr, nullptr);
     return flat ? y : y.reshape(shape);
 }
 
@@ -323,7 +329,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const auto gains = ctx->saved_data["gains"].toDoubleVector();
         const bool want_bias = shape[3] != 0 && ctx->needs_input_grad(1);
-        const variable_list got = at::GradMode::is_enabled()
+        const variable_list got = at::GradMode::is_enabled() || dual(grads[0])
             ? EmbeddingGradFunction::apply(grads[0], index, shape[0], shape[1], shape[2] != 0, gains[0], gains[1], want_bias)
             : EmbeddingGradFunction::run(grads[0].contiguous(), index, shape[0], shape[1], shape[2] != 0, gains[0], gains[1], want_bias);
         if (ctx->needs_input_grad(0)) out[0] = got[0];
@@ -344,7 +350,7 @@ Tensor embedding(const Tensor& index, const Tensor& table, const optional<Tensor
                 " must have one entry per column of the table ", table.sizes());
     const Tensor flat = index.reshape({-1}).contiguous();
     const bool graph = at::GradMode::is_enabled() && (table.requires_grad() || (b.defined() && b.requires_grad()));
-    const Tensor y = graph ? EmbeddingFunction::apply(table, b_, flat, w_gain, b_gain) : lookup(flat, table, b, w_gain, b_gain);
+    const Tensor y = graph || dual(table) || dual(b) ? EmbeddingFunction::apply(table, b_, flat, w_gain, b_gain) : lookup(flat, table, b, w_gain, b_gain);
     if (index.dim() == 1) return y;
     std::vector<int64_t> shape = index.sizes().vec();
     shape.push_back(table.size(1));
