@@ -186,12 +186,16 @@ def profile_begin():
 
 
 def _record(label, nbytes, flops, call):
-    """A launch from C++, on the current stream of the current device, as an entry of the recording."""
+    """A launch from C++, on the current stream of the current device, as an entry of the recording (of none, if it has ended
+    since: the launch may come from another thread's backward pass)."""
+    records = _profile
+    if records is None:
+        return call()
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     start.record()
     call()
     end.record()
-    _profile.append((label, nbytes, start, end, flops))
+    records.append((label, nbytes, start, end, flops))
 
 
 def profiling():
@@ -202,7 +206,7 @@ def profiling():
 def profile_end():
     """Stop recording; returns [(label, bytes, milliseconds, flops)] after synchronising."""
     global _profile
-    records, _profile = _profile or [], None
+    records, _profile = list(_profile or []), None       # (a copy: a launch under way in another thread may still add to the list)
     if _ext is not None:
         _ext.record(None)
     torch.cuda.synchronize()

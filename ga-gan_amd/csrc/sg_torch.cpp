@@ -6,6 +6,9 @@
 // the same file that ga_gan_amd._lib binds.
 #include <dlfcn.h>
 
+#include <atomic>
+#include <memory>
+
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/extension.h>
 
@@ -56,11 +59,19 @@ void bind(const std::string& path) {
 
 // ---- launching ----------------------------------------------------------------------------------------------------------
 
-py::object* recorder = nullptr;      // while launches are being recorded: recorder(label, bytes, flops, call)
+// While launches are being recorded: recorder(label, bytes, flops, call).  A launch may come from a backward pass's thread, which does
+// not hold the interpreter's lock, while another thread ends the recording: a launch keeps the object it saw until it is done
+// with it, and whoever holds it last gives it up under the lock.  (Never destroyed itself: the interpreter may be gone by then.)
+std::shared_ptr<py::object>& recorder = *new std::shared_ptr<py::object>;
 
 void record(const py::object& callback) {
-    delete recorder;
-    recorder = callback.is_none() ? nullptr : new py::object(callback);
+    std::shared_ptr<py::object> next;
+    if (!callback.is_none())
+        next = std::shared_ptr<py::object>(new py::object(callback), [](py::object* last) {
+            py::gil_scoped_acquire gil;
+            delete last;
+        });
+    std::atomic_store(&recorder, next);
 }
 
 // call(stream) on ref's device and the stream torch is enqueueing on there
@@ -68,11 +79,11 @@ template <class Call> void launch(const char* what, const char* label, double by
     const c10::DeviceGuard guard(ref.device());
     void* stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(ref.device().index()).stream();
     int rc = 0;
-    if (recorder == nullptr) {
-        rc = call(stream);
-    } else {
+    if (const auto recording = std::atomic_load(&recorder)) {
         py::gil_scoped_acquire gil;
-        (*recorder)(label, bytes, flops, py::cpp_function([&] { rc = call(stream); }));
+        (*recording)(label, bytes, flops, py::cpp_function([&] { rc = call(stream); }));
+    } else {
+        rc = call(stream);
     }
     TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", api.last_error());
 }
