@@ -8,6 +8,7 @@
 
 #include <atomic>
 #include <memory>
+#include <tuple>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/extension.h>
@@ -435,53 +436,85 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, double eps)
     return out.select(0, 0);
 }
 
-// One update; `scale` (float32, device) multiplies the sanitised gradients where it is given.
-void adam_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs,
-               const std::vector<Tensor>& exp_avg_sqs, const std::vector<int64_t>& steps, double lr, double beta1, double beta2, double eps,
-               double grad_limit, const optional<Tensor>& scale) {
-    const size_t count = params.size();
-    TORCH_CHECK(grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count && steps.size() == count, "adam_step: lists differ in length");
-    if (count == 0) return;
-    const std::vector<Tensor>* lists[4] = {&params, &grads, &exp_avgs, &exp_avg_sqs};
-    static const char* const names[4] = {"param", "grad", "exp_avg", "exp_avg_sq"};
-    const c10::Device device = params[0].device();
-    std::vector<void*> pointers(4 * count);
-    std::vector<int64_t> numels(count);
-    std::vector<int32_t> counts(count);
-    double bytes = 0;
-    for (size_t i = 0; i < count; i++) {
-        numels[i] = params[i].numel();
-        counts[i] = (int32_t)std::min<int64_t>(steps[i], INT32_MAX);
-        bytes += 32.0 * numels[i];
-        for (int k = 0; k < 4; k++) {
-            const Tensor& t = (*lists[k])[i];
-            TORCH_CHECK(t.is_cuda() && t.device() == device, names[k], " must reside on CUDA device ", device);
-            TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous(), names[k], " must be a dense float32 tensor");
-            TORCH_CHECK(t.sizes() == params[i].sizes(), "adam_step: ", names[k], " ", t.sizes(), " does not match its parameter ", params[i].sizes());
-            pointers[k * count + i] = ptr(t);
-        }
-    }
-    distinct(pointers, "adam_step");
-    float* const* base = reinterpret_cast<float* const*>(pointers.data());
+// One group of an optimizer's tensors, checked, as the library takes it (the vectors are what args points into).
+struct AdamGroup {
+    std::vector<void*> pointers;
+    std::vector<int64_t> numels;
+    std::vector<int32_t> counts;
     sg_adam_list args{};
-    args.param = base; args.grad = base + count; args.exp_avg = base + 2 * count; args.exp_avg_sq = base + 3 * count;
-    args.numel = numels.data(); args.step = counts.data();
-    args.count = (int32_t)count;
-    args.lr = (float)lr; args.beta1 = (float)beta1; args.beta2 = (float)beta2; args.eps = (float)eps; args.grad_limit = (float)grad_limit;
-    args.grad_scale = scale.has_value() ? (const float*)ptr(*scale) : nullptr;
-    launch("sg_adam_step_list", "adam_kernel", bytes, 0, params[0], [&](void* stream) { return api.adam_step_list(&args, stream); });
-    for (const auto* list : lists)
-        for (const Tensor& t : *list) t.unsafeGetTensorImpl()->bump_version();
+    double bytes = 0;
+
+    AdamGroup(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs,
+              const std::vector<int64_t>& steps, double lr, double beta1, double beta2, double eps, double grad_limit) {
+        const size_t count = params.size();
+        TORCH_CHECK(grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count && steps.size() == count,
+                    "adam_step: lists differ in length");
+        const std::vector<Tensor>* lists[4] = {&params, &grads, &exp_avgs, &exp_avg_sqs};
+        static const char* const names[4] = {"param", "grad", "exp_avg", "exp_avg_sq"};
+        pointers.resize(4 * count);
+        numels.resize(count);
+        counts.resize(count);
+        for (size_t i = 0; i < count; i++) {
+            const c10::Device device = params[i].device();
+            numels[i] = params[i].numel();
+            counts[i] = (int32_t)std::min<int64_t>(steps[i], INT32_MAX);
+            bytes += 32.0 * numels[i];
+            for (int k = 0; k < 4; k++) {
+                const Tensor& t = (*lists[k])[i];
+                TORCH_CHECK(t.is_cuda() && t.device() == device, names[k], " must reside on CUDA device ", device);
+                TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous(), names[k], " must be a dense float32 tensor");
+                TORCH_CHECK(t.sizes() == params[i].sizes(), "adam_step: ", names[k], " ", t.sizes(), " does not match its parameter ", params[i].sizes());
+                pointers[k * count + i] = ptr(t);
+            }
+            TORCH_CHECK(steps[i] >= 1, "adam_step: tensor ", i, ": step ", steps[i]);
+        }
+        args.lr = (float)lr; args.beta1 = (float)beta1; args.beta2 = (float)beta2; args.eps = (float)eps; args.grad_limit = (float)grad_limit;
+        TORCH_CHECK(args.beta1 >= 0 && args.beta1 < 1 && args.beta2 >= 0 && args.beta2 < 1 && args.eps >= 0 && args.grad_limit > 0,
+                    "adam_step: betas must lie in [0, 1), eps >= 0, grad_limit > 0");
+        float* const* base = reinterpret_cast<float* const*>(pointers.data());
+        args.param = base; args.grad = base + count; args.exp_avg = base + 2 * count; args.exp_avg_sq = base + 3 * count;
+        args.numel = numels.data(); args.step = counts.data();
+        args.count = (int32_t)count;
+    }
+    AdamGroup(const AdamGroup&) = delete;
+};
+
+using AdamArgs = std::tuple<std::vector<Tensor>, std::vector<Tensor>, std::vector<Tensor>, std::vector<Tensor>, std::vector<int64_t>, double, double, double, double, double>;
+
+std::vector<std::unique_ptr<AdamGroup>> checked(const std::vector<AdamArgs>& groups) {
+    std::vector<std::unique_ptr<AdamGroup>> found;
+    for (const AdamArgs& g : groups)
+        found.push_back(std::apply([](const auto&... a) { return std::make_unique<AdamGroup>(a...); }, g));
+    return found;
 }
 
-// The step clipped by the norm of its own sanitised gradients, which it returns.
-Tensor adam_step_clipped(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs,
-                         const std::vector<Tensor>& exp_avg_sqs, const std::vector<int64_t>& steps, double lr, double beta1, double beta2, double eps,
-                         double grad_limit, double max_norm, double norm_eps) {
-    TORCH_CHECK(!grads.empty() && grads.size() == params.size(), "adam_step: lists differ in length");
+// Whether a step of these groups would be refused: raises what it would raise, and launches nothing.
+void adam_check(const std::vector<AdamArgs>& groups) { checked(groups); }
+
+// One step of all groups (each: params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit), clipped by the norm of all
+// their sanitised gradients, which it returns.  Everything is checked before anything is launched.
+Tensor adam_step_clipped(const std::vector<AdamArgs>& groups, double max_norm, double norm_eps) {
+    const auto found = checked(groups);
+    std::vector<Tensor> grads;
+    std::vector<void*> pointers;
+    for (size_t i = 0; i < groups.size(); i++) {
+        const auto& of_group = std::get<1>(groups[i]);
+        grads.insert(grads.end(), of_group.begin(), of_group.end());
+        pointers.insert(pointers.end(), found[i]->pointers.begin(), found[i]->pointers.end());
+        TORCH_CHECK(found[i]->args.grad_limit == found[0]->args.grad_limit, "adam_step: groups that are clipped together must share grad_limit");
+    }
+    TORCH_CHECK(!grads.empty(), "adam_step: no tensors");
+    distinct(pointers, "adam_step");
     const GradList list(grads, "adam_step");
-    const Tensor out = norm_and_scale(list, grads[0], grad_limit, max_norm, norm_eps);
-    adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit, out.select(0, 1));
+    const Tensor out = norm_and_scale(list, grads[0], found[0]->args.grad_limit, max_norm, norm_eps);
+    for (size_t i = 0; i < groups.size(); i++) {
+        AdamGroup& group = *found[i];
+        if (group.args.count == 0) continue;
+        group.args.grad_scale = (const float*)ptr(out) + 1;
+        launch("sg_adam_step_list", "adam_kernel", group.bytes, 0, grads[0], [&](void* stream) { return api.adam_step_list(&group.args, stream); });
+        for (const auto* tensors : {&std::get<0>(groups[i]), &std::get<1>(groups[i]), &std::get<2>(groups[i]), &std::get<3>(groups[i])})
+            for (const Tensor& t : *tensors) t.unsafeGetTensorImpl()->bump_version();
+    }
     return out.select(0, 0);
 }
 
@@ -494,6 +527,6 @@ PYBIND11_MODULE(_sg_torch, m) {
     m.def("embedding", &embedding);
     m.def("grad_norm", &grad_norm);
     m.def("clip_grads", &clip_grads);
-    m.def("adam_step", &adam_step);
+    m.def("adam_check", &adam_check);
     m.def("adam_step_clipped", &adam_step_clipped);
 }

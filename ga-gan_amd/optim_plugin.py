@@ -94,9 +94,8 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps
         max_grad_norm = _max_norm(max_grad_norm, 'adam_step')
         if not params:
             return torch.zeros([])
-        if not grad_limit > 0:
-            raise RuntimeError('adam_step: grad_limit must be positive')
-        return _lib.ext().adam_step_clipped(params, grads, exp_avgs, exp_avg_sqs, [int(k) for k in steps], lr, beta1, beta2, eps, grad_limit, max_grad_norm, CLIP_EPS)
+        group = (params, grads, exp_avgs, exp_avg_sqs, [int(k) for k in steps], lr, beta1, beta2, eps, grad_limit)
+        return _lib.ext().adam_step_clipped([group], max_grad_norm, CLIP_EPS)
     for i in range(0, len(params), MAX_TENSORS):
         chunk = range(i, min(i + MAX_TENSORS, len(params)))
         table = (AdamTensor * len(chunk))()
@@ -139,7 +138,8 @@ def ema_(dsts, srcs, beta):
 class FusedAdam(torch.optim.Optimizer):
     """Adam without weight decay / amsgrad whose `step()` sanitises the gradients and updates every parameter
     that has one in a single launch per 64 tensors.  State layout (`step`, `exp_avg`, `exp_avg_sq` per parameter)
-    and `state_dict()` follow torch.optim.Adam, so checkpoints of one load into the other.
+    and `state_dict()` follow torch.optim.Adam, so checkpoints of one load into the other.  A step whose tensors or settings are
+    refused, in whichever group, changes no parameter, moment or count.
 
     `max_grad_norm` clips by the global norm of all the sanitised gradients of a step, over every parameter group: the norm
     costs one more read of the gradients, the scaling nothing (it happens as the update reads them; `.grad` keeps the
@@ -176,37 +176,35 @@ class FusedAdam(torch.optim.Optimizer):
             _max_norm(self.max_grad_norm, 'FusedAdam')
             if len({group['grad_limit'] for group in self.param_groups}) > 1:
                 raise RuntimeError('FusedAdam: parameter groups that are clipped together must share grad_limit')
-        work = []
+        # A step that is refused changes nothing: everything is checked first, and counts and new moments enter the state behind the launches.
+        work, states = [], []
         for group in self.param_groups:
             params, grads, ms, vs, steps = [], [], [], [], []
             for p in group['params']:
                 if p.grad is None:
                     continue
-                state = self.state[p]
+                state = self.state.get(p)
                 if not state:
-                    state['step'] = torch.tensor(0.0)          # (a host tensor, as torch.optim.Adam keeps it)
-                    state['exp_avg'] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                    state['exp_avg_sq'] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                state['step'] += 1
+                    state = dict(step=torch.tensor(0.0),          # (a host tensor, as torch.optim.Adam keeps it)
+                                 exp_avg=torch.zeros_like(p, memory_format=torch.contiguous_format),
+                                 exp_avg_sq=torch.zeros_like(p, memory_format=torch.contiguous_format))
                 if not p.grad.is_contiguous():
                     p.grad = p.grad.contiguous()
                 params.append(p)
                 grads.append(p.grad)
                 ms.append(state['exp_avg'])
                 vs.append(state['exp_avg_sq'])
-                steps.append(int(state['step']))
+                steps.append(int(state['step']) + 1)
+                states.append((p, state))
             if params:
-                work.append((group, (params, grads, ms, vs, steps)))
-        if self.max_grad_norm is None:
-            for group, lists in work:
-                adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'])
-        elif len(work) == 1:
-            group, lists = work[0]
-            self.last_grad_norm = adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], self.max_grad_norm)
+                work.append((params, grads, ms, vs, steps, group['lr'], *group['betas'], group['eps'], group['grad_limit']))
+        if work and self.max_grad_norm is not None:
+            self.last_grad_norm = _lib.ext().adam_step_clipped(work, self.max_grad_norm, CLIP_EPS)
         elif work:
-            ext = _lib.ext()
-            out = ext.grad_norm([g for _, lists in work for g in lists[1]], work[0][0]['grad_limit'], self.max_grad_norm, CLIP_EPS)
-            for group, lists in work:
-                ext.adam_step(*lists, group['lr'], *group['betas'], group['eps'], group['grad_limit'], out[1:])
-            self.last_grad_norm = out[0]
+            _lib.ext().adam_check(work)
+            for args in work:
+                adam_step(*args)
+        for p, state in states:
+            state['step'] += 1
+            self.state[p] = state
         return loss
