@@ -374,10 +374,14 @@ variable_list EmbeddingGradFunction::backward(AutogradContext* ctx, variable_lis
     const Tensor index = ctx->get_saved_variables()[0];
     const auto gains = ctx->saved_data["gains"].toDoubleVector();
     const Tensor ddbias = grads.size() > 1 ? grads[1] : Tensor();
-    if (grads[0].defined())
-        out[0] = embedding(index, grads[0], ddbias.defined() ? optional<Tensor>(ddbias) : c10::nullopt, gains[0], gains[1]);
-    else if (ddbias.defined())
-        out[0] = (ddbias * gains[1]).expand({index.numel(), ddbias.size(0)});
+    const Tensor from_bias = ddbias.defined() ? (ddbias * gains[1]).expand({index.numel(), ddbias.size(0)}) : Tensor();
+    out[0] = from_bias;
+    if (grads[0].defined()) {
+        // (a token outside the table added to no row: its dy has no part in the rows' gradient, where a lookup would read NaN)
+        const Tensor rows = embedding(index, grads[0], ddbias.defined() ? optional<Tensor>(ddbias) : c10::nullopt, gains[0], gains[1]);
+        const Tensor inside = at::logical_and(index >= 0, index < grads[0].size(0)).unsqueeze(1);
+        out[0] = at::where(inside, rows, from_bias.defined() ? from_bias : at::zeros_like(rows));
+    }
     return out;
 }
 
