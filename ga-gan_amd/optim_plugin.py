@@ -69,7 +69,8 @@ def clip_grad_norm_(parameters, max_norm):
     """Scale the gradients of `parameters` (a tensor or an iterable; those without one are skipped) in place by
     min(1, max_norm / (norm + 1e-6)) and return their global norm before that: torch.nn.utils.clip_grad_norm_ for the 2-norm, in
     a launch per 128 tensors and one more, then another pass over the gradients only if they are too long.  A norm that is not
-    finite makes the gradients NaN or zero, as there.  No gradient may overlap another.  `FusedAdam(max_grad_norm=...)` clips
+    finite makes the gradients NaN or zero, as there.  No gradient may overlap another; one that is not dense costs a copy there
+    and back, and one that overlaps itself (an expanded tensor) is replaced by a dense one.  `FusedAdam(max_grad_norm=...)` clips
     without the second pass."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
@@ -77,10 +78,17 @@ def clip_grad_norm_(parameters, max_norm):
     params = [p for p in parameters if p.grad is not None]
     if not params:
         return torch.zeros([])
-    for p in params:
-        if not p.grad.is_contiguous():
-            p.grad = p.grad.contiguous()
-    return _lib.ext().clip_grads([p.grad for p in params], max_norm, CLIP_EPS)
+    grads = [p.grad for p in params]
+    if len({id(g) for g in grads}) < len(grads):
+        raise RuntimeError('clip_grad_norm_: a tensor appears twice')
+    dense = [g.contiguous() for g in grads]
+    norm = _lib.ext().clip_grads(dense, max_norm, CLIP_EPS)
+    for p, g, d in zip(params, grads, dense):
+        if d is not g and torch._debug_has_internal_overlap(g) == 1:
+            p.grad = d
+        elif d is not g:
+            g.copy_(d)
+    return norm
 
 
 def adam_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, beta1, beta2, eps, grad_limit=1e5, max_grad_norm=None):
