@@ -1226,7 +1226,8 @@ template <class T, bool RA, bool RB> int route_gemm(Gemm& g, const Shape& s, Rou
     g.whole = runs_aligned<T>(g);
     r.thin = RA && (RB || ES == 4) && s.thin && aligned16(g.a) && g.lda % E == 0 &&
              (RB ? aligned16(g.b) && g.ldb % E == 0 : reinterpret_cast<uintptr_t>(g.b) % 8 == 0 && g.ldb % 2 == 0);
-    // (operands that travel by way of registers are those of small products: others are copied into packets first)
+    // (operands that travel by way of registers are those of small products: others are copied into packets first, but for a dy of a
+    // linear layer that starts between packets)
     r.tile = r.direct ? s.tile : 64;
     if (r.tile != s.tile) {
         g.tiles_i = (int)((g.ni + 63) / 64);
