@@ -5,7 +5,7 @@
 //   C[i, j] = sum over p of A(i, p) B(j, p),   each operand stored with p contiguous ("rows") or with i / j contiguous ("columns").
 // An operand is never transposed in memory.  Tiles of 128 bytes along p travel to LDS as they lie (16 bytes per lane, straight
 // into LDS where rows are 16-byte aligned), and a fragment of a "columns" operand is read by the transposing LDS read (16-bit)
-// or four rows at a time (float32).  16-bit operands multiply on v_mfma_f32_16x16x32, float32 ones on v_mfma_f32_16x16x4_f32,
+// or two rows at a time (float32).  16-bit operands multiply on v_mfma_f32_16x16x32, float32 ones on v_mfma_f32_16x16x4_f32,
 // whose products and sums are plain float32.  All sums are float32; every output is rounded once.
 // Large products are bound by the matrix unit at the clock that power leaves: bfloat16 8192 x 4096 -> 4096 with bias, activation and
 // residual 199 to 217 us (1270 to 1380 TFLOP/s), its gradients 200 to 207 each; float32 4096^3 915 to 975 (141 to 150).  Small ones
@@ -308,14 +308,15 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
 // Fragments of COUNT 16-row tiles from row `first` of an LDS tile, for half kk of a step.
 template <class T, int SIDE, bool ROWS, int THREADS, int COUNT> struct Frags {
     using Here = Tile<T, SIDE, ROWS, THREADS>;
-    static constexpr int V = sizeof(T) == 4 && !ROWS ? (COUNT >= 4 ? 4 : COUNT) : 1;   // tiles whose rows interleave
+    static constexpr int V = sizeof(T) == 4 && !ROWS ? 2 : 1;                          // tiles whose rows interleave
+    static_assert(COUNT % V == 0, "interleaved tiles come in pairs");
     uint4 q[COUNT];                                                                   // 8 16-bit values, or 4 float32 (ROWS)
     float f[sizeof(T) == 4 && !ROWS ? COUNT : 1][4];
 
     // row within the wave's share of element `r16` (0 .. 15) of tile t
     static __device__ __forceinline__ int row(int t, int r16) { return (t / V) * 16 * V + r16 * V + t % V; }
 
-    // tile t (with V > 1: tiles t .. t + V - 1, for t a multiple of V)
+    // tile t (with V == 2: tiles t and t + 1, for an even t)
     __device__ __forceinline__ void read(const unsigned char* lds, int first, int kk, int t) {
         const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
         if constexpr (ROWS) {
@@ -336,15 +337,8 @@ template <class T, int SIDE, bool ROWS, int THREADS, int COUNT> struct Frags {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const unsigned char* at = lds + (kk * 16 + g * 4 + e) * LINE + (first + t * 16 + l16 * V) * 4;
-                    if constexpr (V == 4) {
-                        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(at);
-                        f[t][e] = v.x; f[t + 1][e] = v.y; f[t + 2][e] = v.z; f[t + 3][e] = v.w;
-                    } else if constexpr (V == 2) {
-                        const f32x2_t v = *reinterpret_cast<const f32x2_t*>(at);
-                        f[t][e] = v.x; f[t + 1][e] = v.y;
-                    } else {
-                        f[t][e] = *reinterpret_cast<const float*>(at);
-                    }
+                    const f32x2_t v = *reinterpret_cast<const f32x2_t*>(at);
+                    f[t][e] = v.x; f[t + 1][e] = v.y;
                 }
         }
     }
@@ -619,13 +613,7 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
         for (int t = 0; t < TJ; t++) {
             if constexpr (FragB::V == 1) {
                 chunk_at(row, t * 4 + quad) = acc[t][s];
-            } else if constexpr (FragB::V == 4) {                        // tiles t .. t + 3 hold consecutive columns
-                if (t % 4 == 0)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        chunk_at(row, t / 4 * 16 + quad * 4 + r) = f32x4_t{acc[t][s][r], acc[t + 1][s][r], acc[t + 2][s][r], acc[t + 3][s][r]};
-            } else {
-                static_assert(FragB::V == 2 || FragB::V == 1 || FragB::V == 4, "interleaved tiles");
+            } else {                                                     // tiles t and t + 1 hold alternate columns
                 if (t % 2 == 0)
 #pragma unroll
                     for (int r = 0; r < 4; r += 2)
