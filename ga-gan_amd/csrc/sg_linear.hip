@@ -197,9 +197,13 @@ __device__ __forceinline__ i32x4_t descriptor(const void* p) {
 // assembly because of its wait: the compiler holds every LDS read behind all copies into LDS that came before it, those into the
 // other tiles included.  The kernel places the waits.  (One instruction sets the LDS address: a wave that has a SIMD to itself
 // issues one in four cycles, 32 in the time of 8 products, and a step is built to stay below that.)
+// (m0 is said to be overwritten, which is what is meant: the compiler warns, at every copy, that nobody saves it.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int PLACE> __device__ __forceinline__ void copy_to_lds(i32x4_t from, unsigned offset, unsigned lds) {
     asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" ::"s"(lds), "n"(PLACE), "v"(offset), "s"(from) : "m0", "scc");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
