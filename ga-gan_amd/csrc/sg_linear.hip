@@ -134,7 +134,8 @@ template <class T, bool FORWARD> __device__ __forceinline__ float scale_of(const
     else return g.scale;
 }
 
-template <class T, int N> struct alignas(N * sizeof(T)) Run { T v[N]; };
+// (of up to 16 bytes' alignment: longer runs are moved as packets)
+template <class T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Run { T v[N]; };
 
 template <class T, int N> __device__ __forceinline__ Run<T, N> bias_run(const Gemm& g, int64_t j) {
     return g.bias ? *reinterpret_cast<const Run<T, N>*>((const T*)g.bias + j) : Run<T, N>{};
@@ -207,6 +208,17 @@ template <int PLACE> __device__ __forceinline__ void copy_to_lds(i32x4_t from, u
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
+// 16 bytes from the address of any element of T.  (A plain vector: a class type would keep its own alignment within the packed struct,
+// and the load would claim an address that is a multiple of 16.)
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    sg_u32x4_t v;
+    static __device__ __forceinline__ uint4 load(const T* p) {
+        static_assert(alignof(Loose) == sizeof(T) && sizeof(Loose) == 16, "no more aligned than an element");
+        const sg_u32x4_t q = reinterpret_cast<const Loose*>(p)->v;
+        return make_uint4(q.x, q.y, q.z, q.w);
+    }
+};
+
 // One operand's tile of SIDE rows i (or j) by 128 bytes of p in LDS: slots of 16 bytes, slot k * THREADS + t filled by thread t.
 //   ROWS:  slot (row, c) holds the 16 bytes c ^ turn(row) of the row: the lanes that read at one time - 16 rows at one c, or 8 rows
 //          each at two - hit 16 different 16-byte banks.
@@ -273,7 +285,6 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
     }
     template <bool SHORT>
     static __device__ __forceinline__ void fetch(Regs& r, const Slots& s, const T* base, int64_t ld, int left_side, int left_p, int64_t extent_c) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Loose { uint4 v; };
         const int c = ROWS ? s.p : s.side, cut = cut_of(s, extent_c);
         const int64_t back = SHORT ? 0 : cut == E ? extent_c - E : c - cut;        // (a slot wholly outside reads what is inside)
 #pragma unroll
@@ -288,7 +299,7 @@ template <class T, int SIDE, bool ROWS, int THREADS> struct Tile {
                 }
                 __builtin_memcpy(&r.v[k], &q, 16);
             } else {
-                r.v[k] = reinterpret_cast<const Loose*>(line + back)->v;
+                r.v[k] = Loose<T>::load(line + back);
             }
         }
     }
@@ -1075,8 +1086,8 @@ template <class T> __global__ void __launch_bounds__(256) linear_pack_kernel(con
     const T* src = (const T*)m.src + row * m.ld + c;
     Pack<T> q;
     if (c + E <= m.cols) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Loose { Pack<T> v; };
-        q = reinterpret_cast<const Loose*>(src)->v;
+        const uint4 raw = Loose<T>::load(src);
+        __builtin_memcpy(&q, &raw, 16);
     } else {
 #pragma unroll
         for (int e = 0; e < E; e++) q.v[e] = c + e < m.cols ? src[e] : rounded<T>(0.f);
