@@ -501,6 +501,12 @@ class Trainer:
         phase.opt.zero_grad(set_to_none=True)
         self._graphs[phase.name] = (graph, static, grads)
 
+    def _is_recorded(self, phase, **inputs):
+        """Whether `phase` has a recording made from inputs of these shapes.  (Labels may come as rows or as class numbers, and a copy of
+        one into the other would broadcast where it fits; the phase is launched from the host then.)"""
+        recording = self._graphs.get(phase.name)
+        return recording is not None and all(recording[1][name].shape == t.shape for name, t in inputs.items())
+
     def _replay_phase(self, phase, r_img, r_c, g_z, g_c):
         graph, static, grads = self._graphs[phase.name]
         static['r_img'].copy_(r_img)
@@ -544,8 +550,7 @@ class Trainer:
         for phase, phase_gen_z, phase_gen_c in zip(self.phases, all_gen_z, all_gen_c):
             if self.batch_idx % phase.interval != 0:
                 continue
-            graphed = self.use_graphs and rounds == 1 and self._graphs.get(phase.name)
-            if graphed:
+            if self.use_graphs and rounds == 1 and self._is_recorded(phase, r_c=phase_real_c[0], g_c=phase_gen_c[0]):
                 self._replay_phase(phase, phase_real_img[0], phase_real_c[0], phase_gen_z[0], phase_gen_c[0])
             else:
                 phase.opt.zero_grad(set_to_none=True)
