@@ -1,9 +1,10 @@
 """Build the HIP library in-tree:  python -m ga_gan_amd.build  (hipcc, gfx950 only).
 
 Every csrc/*.hip is compiled to an object of its own (in parallel) and the objects are linked into
-libsgops.so; csrc/sg_torch.cpp (host code: the operators' PyTorch side) is compiled into _sg_torch.so.  Staleness is decided by content, not by time stamps: each object carries a stamp with the
-digest of its source, of every header and of the compiler flags, the way the reference keys its plugin build
-directory by a digest of the op's sources (torch_utils/custom_ops.py:88-104).  The whole build runs under an
+libsgops.so; csrc/sg_torch.cpp (host code: the operators' PyTorch side) is compiled into _sg_torch.so.  Staleness is
+decided by content, not by time stamps: each object carries a stamp with the digest of its source, of every header and of
+the compiler flags, the way the reference keys its plugin build directory by a digest of the op's sources
+(torch_utils/custom_ops.py:88-104).  The whole build runs under an
 exclusive file lock, so that several ranks importing a stale tree at once build it once and the others wait
 (the reference's FileBaton, torch_utils/custom_ops.py:105-115).
 """

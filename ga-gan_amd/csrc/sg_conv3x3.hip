@@ -97,8 +97,9 @@ template <class T> __device__ __forceinline__ float lo16(unsigned w) { return Pa
 template <class T> __device__ __forceinline__ float hi16(unsigned w) { return Pair<T>::hi(w); }
 template <class T> __device__ __forceinline__ unsigned pack16(float a, float b) { return Pair<T>::pack(a, b); }
 
-// The layer epilogue on four consecutive pixels of one channel, two at a time: x * scale + noise, + bias, leaky ReLU as max(z, z * slope) (0 <= slope <= 1, checked by the
-// dispatcher), gain, clamp as a median of three; scale 1, noise 0, bias 0, slope 1, clamp +-inf are no-ops.
+// The layer epilogue on four consecutive pixels of one channel, two at a time: x * scale + noise, + bias, leaky ReLU as
+// max(z, z * slope) (0 <= slope <= 1, checked by the dispatcher), gain, clamp as a median of three; scale 1, noise 0, bias 0,
+// slope 1, clamp +-inf are no-ops.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 template <class T>
 __device__ __forceinline__ uint2 finish4(const f32x4_t& a, float sc, f32x2_t nz01, f32x2_t nz23, float bs, float slope, float gain, float hi) {

@@ -9,7 +9,8 @@
 // whose products and sums are plain float32.  All sums are float32; every output is rounded once.
 // Large products are bound by the matrix unit at the clock that power leaves: bfloat16 8192 x 4096 -> 4096 with bias, activation and
 // residual 199 to 217 us (1270 to 1380 TFLOP/s), its gradients 200 to 207 each; float32 4096^3 915 to 975 (141 to 150).  Small ones
-// are bound by launches: one row of 512 -> 512 3.8 us, a training step of 32 rows 18 in four launches.
+// are bound by launches: one row of 512 -> 512 3.8 us, a training step of 32 rows 18 in four launches.  float16 gradients have a launch
+// more, which finds the largest |dy|: 3 us at 1000 x 1025.
 //
 // The gradient of the activation is s above without the gains: for the piecewise linear activations with slope 1 on one side
 // its 16-bit rounding is exact there, so that folding sqrt(2) into the products' scale keeps it that way.  float16, whose range a
@@ -793,7 +794,8 @@ __device__ __forceinline__ void gemm_tile(const Gemm& g, unsigned id, unsigned c
     }
 }
 
-// (64 x 64: five workgroups on a CU, as many as its LDS holds.  float32 10000 x 512 -> 512, 1256 of them: 55 us with four, 49 with five)
+// (64 x 64: five workgroups on a CU, as many as its LDS holds.  float32 10000 x 512 -> 512, 1256 of them: 55 us with four and 49 with
+// five when they were compared, 44 with the steps of today)
 template <class T, int BI, int BJ, int WI, int WJ, bool ROWS_A, bool ROWS_B, int MODE, int RING>
 __global__ void __launch_bounds__(WI * WJ * 64, BI == 64 && MODE == kDirect && RING == 2 ? 5 : 1) linear_gemm_kernel(const Gemm g) {
     __shared__ __attribute__((aligned(16))) unsigned char smem[kTileBytes<BI, BJ, RING>];

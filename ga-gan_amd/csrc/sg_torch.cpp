@@ -1,8 +1,8 @@
 // PyTorch side of the operators whose smallest calls are shorter than the host's work around them (fully connected layer,
 // table lookup, clipped optimizer step): argument checks, allocation, autograd and the calls of the C ABI, without the
 // interpreter in between.  A training step of one small layer spends its time on the host: with the same steps written in
-// Python, a forward and backward call of a 32 x 512 x 512 layer took 172 us of which the kernels need 18; so it takes 67, of
-// which autograd's change of threads is 34.  The entry points themselves are the library's (include/sg_ops.h), resolved from
+// Python, a forward and backward call of a 32 x 512 x 512 layer took 172 us of which the kernels need 18; so it takes 40 to 68, of
+// which autograd's change of threads is 10 to 34 (by where its thread runs).  The entry points themselves are the library's (include/sg_ops.h), resolved from
 // the same file that ga_gan_amd._lib binds.
 #include <dlfcn.h>
 
@@ -189,7 +189,8 @@ Tensor linear_composite(const Tensor& x_, const Tensor& w_, const Tensor& b_, co
 
 // What the backward pass keeps besides x and w: nothing for linear; for relu and lrelu the output itself, whose sign is the
 // pre-activation's, or - where a residual, a gain that may take positive values to zero (float16: any), or a negative slope
-// hides it - a byte per element; for the others the pre-activation values in float32 (rounded to 16 bits they would cost the gradient more accuracy than its own rounding does).
+// hides it - a byte per element; for the others the pre-activation values in float32 (rounded to 16 bits they would cost the
+// gradient more accuracy than its own rounding does).
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
     enum Kept { kNothing, kY, kPositive, kZ };
 

@@ -9,8 +9,8 @@ in the same layout).  The gradient sums the rows of dy that share an index in th
 atomics, so that the same inputs give the same bits (`sg_embedding`, `sg_embedding_backward`).  The pair of functions is
 closed under differentiation: the gradient's own gradient is a lookup again.
 
-Indices outside the table are not checked on the host (that would wait for the device): they read as rows of NaN and take
-no gradient."""
+Indices outside the table are not checked on the host (that would wait for the device): they read as rows of NaN and add to
+no row of the table's gradient (the bias's sums every token).  Forward-mode tangents are refused."""
 import torch
 
 from ... import _lib

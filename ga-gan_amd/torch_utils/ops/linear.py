@@ -24,7 +24,8 @@ from . import bias_act
 def linear(x, w, b=None, residual=None, act='linear', alpha=None, gain=None, w_gain=1.0, b_gain=1.0):
     """x [..., K], w [N, K], b [N] or None, residual [..., N] (the output's shape) or None -> [..., N]; one dtype (float32,
     float16 or bfloat16) and one device.  Rows of x, w and residual may lie any distance apart; tensors whose last dimension
-    is not contiguous, or whose rows are 2^23 bytes or more apart, are copied first, and rows of that length are refused.  `alpha` and `gain` default to the activation's."""
+    is not contiguous, or whose rows are 2^23 bytes or more apart, are copied first, and rows of that length are refused (the
+    output's by the backward pass).  `alpha` and `gain` default to the activation's.  Forward-mode tangents are refused."""
     assert isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor)
     spec = bias_act.activation_funcs[act]
     return _lib.ext().linear(x, w, b, residual, spec.cuda_idx, spec.def_alpha if alpha is None else alpha, spec.def_gain if gain is None else gain,

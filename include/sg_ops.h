@@ -578,11 +578,12 @@ int sg_lerp_multi(const sg_lerp_params* p, sg_stream_t stream);
  *
  * Backward: with s = dy * act'(z), dy [m, n] dense,
  *   dx [m, k] = s w * (gain w_gain)     dw [n, k] = s^T x * (gain w_gain)     db [n] = column sums of s * (gain b_gain)
- * each dense, of `dtype`, and skipped when its pointer is NULL; a dy that is not 16-byte aligned keeps a linear layer to small tiles.  The slope comes from exactly one of: y (the layer's output, for
- * relu / lrelu without a residual and with gain != 0), positive (relu / lrelu), z (every other activation but linear, which
- * takes none).  With y, a positive pre-activation value that the output rounds to zero counts as negative.  For dx and dw, 16-bit layers
- * round s to `dtype` (float16: times a power of two found from the largest |dy|, so that it neither overflows nor vanishes); db sums
- * it unrounded.  p->b and p->residual are not read.  `workspace`: device memory, 16-byte aligned, private to the call until the
+ * each dense, of `dtype`, and skipped when its pointer is NULL; a dy that is not 16-byte aligned keeps a linear layer to small
+ * tiles.  The slope comes from exactly one of: y (the layer's output, for relu / lrelu without a residual and with gain != 0),
+ * positive (relu / lrelu), z (every other activation but linear, which takes none).  With y, a positive pre-activation value that
+ * the output rounds to zero counts as negative.  relu's gradient is zero where it is off, whatever dy holds there.  For dx and dw,
+ * 16-bit layers round s to `dtype` (float16: times a power of two found from the largest |dy|, so that it neither overflows nor
+ * vanishes); db sums it unrounded.  p->b and p->residual are not read.  `workspace`: device memory, 16-byte aligned, private to the call until the
  * stream has passed it.  Sums run in an order that depends on the sizes, alignments and the outputs asked for alone. */
 typedef struct sg_linear_params {
     const void* x;
