@@ -2,8 +2,8 @@
 // table lookup, clipped optimizer step): argument checks, allocation, autograd and the calls of the C ABI, without the
 // interpreter in between.  A training step of one small layer spends its time on the host: with the same steps written in
 // Python, a forward and backward call of a 32 x 512 x 512 layer took 172 us of which the kernels need 18; so it takes 40 to 68, of
-// which autograd's change of threads is 10 to 34 (by where its thread runs).  The entry points themselves are the library's (include/sg_ops.h), resolved from
-// the same file that ga_gan_amd._lib binds.
+// which autograd's change of threads is 10 to 34 (by where its thread runs).  The entry points themselves are the library's
+// (include/sg_ops.h), resolved from the same file that ga_gan_amd._lib binds.
 #include <dlfcn.h>
 
 #include <atomic>
@@ -225,6 +225,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         const LinearConfig c{(int64_t)v[0], v[1], v[2], v[3], v[4]};
         const int kept = (int)v[5];
         if (at::GradMode::is_enabled()) {                        // a graph of its own is wanted: differentiate the operators' version
+            const c10::impl::ExcludeDispatchKeyGuard in_its_types(c10::autocast_dispatch_keyset);      // (the caller's autocast would round its products)
             variable_list in{x_.view_as(x_), w_.view_as(w_), b.defined() ? b.view_as(b) : b}, wanted;
             for (int i = 0; i < 3; i++)
                 if (need[i]) wanted.push_back(in[i]);
